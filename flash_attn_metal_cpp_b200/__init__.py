@@ -35,6 +35,10 @@ sys.modules.setdefault("_flash_attn_metal", _flash_attn_metal)
 initialize = _flash_attn_metal.initialize
 get_device_info = _flash_attn_metal.get_device_info
 forward = _flash_attn_metal.forward
+plan_pages = _flash_attn_metal.plan_pages
+store_kv = _flash_attn_metal.store_kv
+paged_forward = _flash_attn_metal.paged_forward
+shared_prefix_forward = _flash_attn_metal.shared_prefix_forward
 
 
 def _to_numpy(x):
@@ -72,4 +76,5 @@ def metal_attention(q, k, v, causal=False, softmax_scale=None, dropout_p=0.0):
     )
 
 
-__all__ = ["metal_attention", "initialize", "get_device_info", "forward", "LIB_PATH"]
+__all__ = ["metal_attention", "initialize", "get_device_info", "forward", "plan_pages", "store_kv", "paged_forward",
+           "shared_prefix_forward", "LIB_PATH"]

@@ -40,8 +40,11 @@ CU_SOURCES = [
     "fa_fwd_sm100_d64_full.cu",
     "fa_fwd_sm100_d128_causal.cu",
     "fa_fwd_sm100_d128_full.cu",
+    "fa_paged_api.cu",
+    "fa_paged_cache.cu",
+    "fa_paged_simt.cu",
 ]
-HEADERS = ["fa_internal.h", "fa_ptx.cuh", "fa_fwd_sm100.cuh", "fa_host.h"]
+HEADERS = ["fa_internal.h", "fa_ptx.cuh", "fa_fwd_sm100.cuh", "fa_host.h", "fa_paged.h", "fa_paged.cuh"]
 
 
 def _mtime(path: str) -> float:
@@ -78,15 +81,15 @@ def build(force: bool = False, jobs: int | None = None) -> tuple[str, str]:
     if force or _mtime(LIB) < max(_mtime(o) for o in objs):
         _run([NVCC, *ARCH, "-shared", "-Xcompiler", "-fPIC", "-o", LIB, *objs])
 
-    bsrc = os.path.join(CSRC, "bindings.cpp")
-    if force or _mtime(EXT) < max(_mtime(bsrc), _mtime(LIB), _mtime(os.path.join(INCLUDE, "fa_b200.h"))):
+    bsrcs = [os.path.join(CSRC, f) for f in ("bindings.cpp", "bindings_paged.cpp")]
+    if force or _mtime(EXT) < max(*map(_mtime, bsrcs), _mtime(LIB), _mtime(os.path.join(INCLUDE, "fa_b200.h"))):
         import pybind11
 
         py_inc = sysconfig.get_paths()["include"]
         _run([
             "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
             "-I", pybind11.get_include(), "-I", py_inc, "-I", INCLUDE,
-            bsrc, "-o", EXT, "-L", PKG, "-l:libfa_b200.so", "-Wl,-rpath,$ORIGIN",
+            *bsrcs, "-o", EXT, "-L", PKG, "-l:libfa_b200.so", "-Wl,-rpath,$ORIGIN",
         ])
     return LIB, EXT
 

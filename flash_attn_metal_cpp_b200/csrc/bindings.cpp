@@ -608,6 +608,8 @@ py::tuple py_pool_stats() {
 
 }  // namespace
 
+void bind_paged(py::module_& m);  // bindings_paged.cpp
+
 PYBIND11_MODULE(_flash_attn_metal, m) {
   m.doc() = "FlashAttention-2 forward for NVIDIA B200 (sm_100a), drop-in for the Metal module";
   m.def("initialize", &py_initialize, "Initialize the CUDA device");
@@ -622,7 +624,7 @@ PYBIND11_MODULE(_flash_attn_metal, m) {
         py::kw_only(), py::arg("out_dtype") = py::none(), py::arg("rope_theta") = py::none(),
         py::arg("return_lse") = false, py::arg("out") = py::none(), "Flash Attention forward pass");
   m.def("check_status", &py_check_status,
-        "Raise if a kernel recorded a timeout or range error since the last check");
+        "Raise if a kernel recorded a timeout or a bad index since the last check");
   m.def("launch_count", []() { return fa_launch_count(); },
         "Number of kernels this library launched on the calling thread");
   m.def("kernel_timing_enable", []() { fa_kernel_timing_enable(); },
@@ -666,4 +668,5 @@ PYBIND11_MODULE(_flash_attn_metal, m) {
     fa_status st = fa_ipc_free(reinterpret_cast<void*>(p));
     if (st != FA_OK) throw std::runtime_error(err_text(st));
   }, py::arg("address"));
+  bind_paged(m);
 }

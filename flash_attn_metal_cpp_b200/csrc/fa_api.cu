@@ -140,7 +140,7 @@ struct Lease {
 struct DeviceState {
   int device = -1;
   bool ready = false;
-  unsigned* status = nullptr;       // in-kernel status word
+  unsigned* status = nullptr;       // in-kernel status words: timeouts, bad indexes (paged operators)
   void* status_host = nullptr;      // pinned copy of it, read back by the host-pointer path
   cudaStream_t host_stream = nullptr;   // host-pointer path: compute
   cudaStream_t h2d_stream = nullptr;    // host-pointer path: copies in
@@ -201,8 +201,8 @@ fa_status device_state(DeviceState** out) {
     if (prop.major != 10)
       return fail(FA_ERR_UNSUPPORTED, std::string("device '") + prop.name +
                                           "' is not sm_100 (B200); this library is built for sm_100a only");
-    FA_CUDA(cudaMalloc(&ds->status, sizeof(unsigned)));
-    FA_CUDA(cudaMemset(ds->status, 0, sizeof(unsigned)));
+    FA_CUDA(cudaMalloc(&ds->status, 2 * sizeof(unsigned)));
+    FA_CUDA(cudaMemset(ds->status, 0, 2 * sizeof(unsigned)));
     ds->status_host = pinned_get(sizeof(unsigned));  // NULL: the host path reads the word synchronously
     FA_CUDA(cudaStreamCreateWithFlags(&ds->host_stream, cudaStreamNonBlocking));
     FA_CUDA(cudaStreamCreateWithFlags(&ds->h2d_stream, cudaStreamNonBlocking));
@@ -212,6 +212,15 @@ fa_status device_state(DeviceState** out) {
   }
   *out = ds;
   return FA_OK;
+}
+
+// Reads and clears the timeout word of the current device.
+fa_status take_timeout(DeviceState* ds) {
+  unsigned v = 0;
+  FA_CUDA(cudaMemcpy(&v, ds->status, sizeof(v), cudaMemcpyDeviceToHost));
+  if (v == 0) return FA_OK;
+  FA_CUDA(cudaMemset(ds->status, 0, sizeof(unsigned)));
+  return fail(FA_ERR_TIMEOUT, "a kernel wait exceeded its time limit; the kernel returned early and its output is invalid");
 }
 
 // ---------------------------------------------------------------- validation
@@ -657,6 +666,54 @@ fa_status run(Plan& pl, const void* q, const void* k, const void* v, const float
 
 void note_launch() { ++g_launches; }
 
+// ------------------------------------------- for the paged operators (fa_paged.h)
+fa_status paged_fail(fa_status st, const std::string& msg) { return fail(st, msg); }
+
+fa_status paged_status_words(unsigned** words) {
+  DeviceState* ds = nullptr;
+  fa_status st = device_state(&ds);
+  if (st == FA_OK) *words = ds->status;
+  return st;
+}
+
+fa_status paged_rope(float theta, int D, int rows, cudaStream_t stream, const float** cs, const float** sn) {
+  DeviceState* ds = nullptr;
+  fa_status st = device_state(&ds);
+  if (st != FA_OK) return st;
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  FA_CUDA(cudaStreamIsCapturing(stream, &cap));
+  if (cap != cudaStreamCaptureStatusNone) {
+    std::lock_guard<std::mutex> g(ds->mu);
+    auto it = ds->rope.find(std::make_pair(theta, D));
+    if (it == ds->rope.end() || !it->second.cs || it->second.rows < rows)
+      return fail(FA_ERR_INVALID_ARG, "the tables of this rope_theta are not built yet: make one call with them "
+                                      "before the stream is captured");
+    *cs = it->second.cs;
+    *sn = it->second.sn;
+    return FA_OK;
+  }
+  return rope_from_theta(ds, theta, D, rows, stream, cs, sn);
+}
+
+fa_status paged_encode(CUtensorMap* m, const void* base, bool bf16, int D, int H, int slots, int pages, int64_t sp,
+                       int64_t ss, int64_t sh, int box_rows) {
+  fa_status st = get_encode();
+  if (st != FA_OK) return st;
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)H, (cuuint64_t)slots, (cuuint64_t)pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)sh * 2, (cuuint64_t)ss * 2, (cuuint64_t)sp * 2};
+  const cuuint32_t box[4] = {64, 1, (cuuint32_t)box_rows, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = g_encode(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                        const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(FA_ERR_INVALID_ARG, "cuTensorMapEncodeTiled failed (code " + std::to_string((int)r) + ")");
+  return FA_OK;
+}
+
+unsigned long long paged_wait_limit_ns() { return g_wait_limit_ns.load(std::memory_order_relaxed); }
+
 }  // namespace fa
 
 using namespace fa;
@@ -1028,7 +1085,7 @@ fa_status fa_forward_host(const fa_params* p, const void* q, const void* k, cons
   // The in-kernel status word is read back with the results (no extra sync).
   unsigned* status_host = static_cast<unsigned*>(ds->status_host);
   auto finish_status = [&]() -> fa_status {
-    if (status_host == nullptr || *status_host != 0) return fa_check_device_status();
+    if (status_host == nullptr || *status_host != 0) return take_timeout(ds);
     return FA_OK;
   };
   // Pageable outputs: copy the staged results out with the workers (the
@@ -1200,11 +1257,15 @@ fa_status fa_check_device_status(void) {
   DeviceState* ds = nullptr;
   fa_status st = device_state(&ds);
   if (st != FA_OK) return st;
-  unsigned v = 0;
-  FA_CUDA(cudaMemcpy(&v, ds->status, sizeof(v), cudaMemcpyDeviceToHost));
-  if (v == 0) return FA_OK;
-  FA_CUDA(cudaMemset(ds->status, 0, sizeof(unsigned)));
-  return fail(FA_ERR_TIMEOUT, "a kernel wait exceeded its time limit; the kernel returned early and its output is invalid");
+  st = take_timeout(ds);
+  if (st != FA_OK) return st;
+  unsigned bad = 0;
+  FA_CUDA(cudaMemcpy(&bad, ds->status + 1, sizeof(bad), cudaMemcpyDeviceToHost));
+  if (bad == 0) return FA_OK;
+  FA_CUDA(cudaMemset(ds->status + 1, 0, sizeof(unsigned)));
+  return fail(FA_ERR_BAD_INDEX,
+              "a paged operator met a page, slot, position or length outside its cache, table or free list; it was "
+              "skipped and the rows that needed it are unspecified");
 }
 
 fa_status fa_set_wait_limit(double seconds) {

@@ -1,0 +1,230 @@
+// fa_paged.cuh - device side shared by the paged attention kernels: the view
+// of one request, the cut of a call's key tiles into equal runs, and the end
+// of a finished row (join with partial results, division, store).
+//
+// Lengths live on the device, so the host cannot balance a batch of requests
+// of very different lengths. Instead every block sums up the tiles of the
+// call itself: a unit is (request, KV head, chunk of packed query rows), its
+// key range is cut in tiles, all tiles of the call stand in one line, and
+// block c of n takes tiles [c * T / n, (c + 1) * T / n). A block so holds the
+// end of one unit, whole units, and the beginning of another; the two open
+// ends go to the block's two partial slots and a second kernel joins them in
+// the order of the blocks, so results do not depend on timing. Calls whose
+// keys are few by the table's width are not cut (PagedArgs::split): the line
+// then counts units and nothing is joined.
+#pragma once
+
+#include "fa_paged.h"
+#include "fa_ptx.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace fa {
+
+// Bit of the bad-index status word.
+enum : unsigned { FA_DEV_BAD_INDEX = 1u };
+
+__device__ __forceinline__ void note_bad_index(unsigned* status) { atomicOr(status + 1, FA_DEV_BAD_INDEX); }
+
+template <typename T>
+__device__ __forceinline__ float cvt_in(T x);
+template <>
+__device__ __forceinline__ float cvt_in<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ float cvt_in<__half>(__half x) { return __half2float(x); }
+template <>
+__device__ __forceinline__ float cvt_in<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+// One request: its query rows, its keys, and the key tiles any of its rows sees.
+struct ReqView {
+  int q0, qlen;      // query tokens
+  int klen;          // keys: shared ones in front, own ones behind
+  int key_lo;        // first key the sliding window leaves visible to any row
+  int tile_lo, tiles;
+  int units;         // chunks * Hk
+  // Tiles the request adds to the line; uncut work counts whole units.
+  __device__ __forceinline__ int per_unit(const PagedArgs& a) const { return a.split ? tiles : 1; }
+  __device__ __forceinline__ long long work(const PagedArgs& a) const { return (long long)units * per_unit(a); }
+};
+
+// Lengths outside the table and query ranges outside q are clipped (and noted
+// in the status word): a wrong length gives a wrong row, never a wrong access.
+template <int TN>
+__device__ __forceinline__ ReqView view_request(const PagedArgs& a, int i, int rows_per_unit) {
+  ReqView r;
+  bool bad = false;
+  if (a.cu_q != nullptr) {
+    int b = a.cu_q[i], e = a.cu_q[i + 1];
+    const int b0 = min(max(b, 0), a.total_q), e0 = min(max(e, b0), a.total_q);
+    bad = b0 != b || e0 != e;
+    r.q0 = b0;
+    r.qlen = e0 - b0;
+  } else {
+    r.q0 = i;
+    r.qlen = i < a.total_q ? 1 : 0;
+  }
+  const int len = a.seq_lens[i];
+  const int cap = (int)min((long long)a.max_pages * a.page_size, (long long)0x3fffffff);
+  const int own = min(max(len, 0), cap);
+  bad |= own != len;
+  if (bad) note_bad_index(a.status);
+  r.klen = a.pre + own;
+  r.key_lo = a.win_left >= 0 ? (int)max(0ll, (long long)r.klen - r.qlen - a.win_left) : 0;
+  r.key_lo = min(r.key_lo, r.klen);
+  r.tile_lo = r.key_lo / TN;
+  r.tiles = max(1, (r.klen + TN - 1) / TN - r.tile_lo);  // a row without keys is still written
+  const int chunks = (int)(((long long)r.qlen * a.group + rows_per_unit - 1) / rows_per_unit);
+  r.units = chunks * a.Hk;
+  return r;
+}
+
+// The run of tiles of one block.
+struct Run {
+  long long begin, end, total;
+  int n_runs;
+  int req;                 // request the run begins in
+  long long req_begin;     // first tile of that request
+};
+
+// Sums up the call's tiles and finds the block's run. Every thread of the
+// block calls it; `sh` is shared scratch. At least `min_tiles` tiles a run:
+// shorter runs cost more in joining than they save.
+struct RunScratch {
+  long long part[32];
+  long long req_begin;
+  int req;
+};
+template <int TN, int NTHREADS>
+__device__ __forceinline__ Run find_run(const PagedArgs& a, int rows_per_unit, int block, int n_blocks, int min_tiles,
+                                        RunScratch* sh) {
+  constexpr int NW = NTHREADS / 32;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int seg = (a.B + NTHREADS - 1) / NTHREADS;
+  const int i0 = min(tid * seg, a.B), i1 = min(i0 + seg, a.B);
+  long long sum = 0;
+  for (int i = i0; i < i1; ++i) sum += view_request<TN>(a, i, rows_per_unit).work(a);
+  long long inc = sum;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, inc, off);
+    if (lane >= off) inc += v;
+  }
+  if (lane == 31) sh->part[warp] = inc;
+  if (tid == 0) sh->req = -1;
+  __syncthreads();
+  long long before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    if (w < warp) before += sh->part[w];
+    total += sh->part[w];
+  }
+  Run r;
+  r.total = total;
+  r.n_runs = (int)min((long long)n_blocks, max(1ll, total / (a.split ? min_tiles : 1)));
+  r.begin = r.end = 0;
+  if (total > 0 && block < r.n_runs) {
+    r.begin = total * block / r.n_runs;
+    r.end = total * (block + 1) / r.n_runs;
+  }
+  long long at = before + inc - sum;
+  if (r.end > r.begin && sum > 0 && r.begin >= at && r.begin < at + sum) {
+    for (int i = i0; i < i1; ++i) {
+      const long long w = view_request<TN>(a, i, rows_per_unit).work(a);
+      if (r.begin < at + w) {
+        sh->req = i;
+        sh->req_begin = at;
+        break;
+      }
+      at += w;
+    }
+  }
+  __syncthreads();
+  r.req = sh->req;
+  r.req_begin = sh->req_begin;
+  return r;
+}
+
+// Physical page of key `key` of a request (-1 when the table names none of
+// the cache's pages) and its slot in the page.
+__device__ __forceinline__ int2 find_key(const PagedArgs& a, int req, int key) {
+  const bool shared = key < a.pre;
+  const int own = shared ? key : key - a.pre;
+  const int p = own / a.page_size;
+  const int slot = own - p * a.page_size;
+  int page = shared ? a.pre_table[p] : a.table[(int64_t)req * a.table_stride + p];
+  if ((unsigned)page >= (unsigned)a.num_pages) {
+    note_bad_index(a.status);
+    page = -1;
+  }
+  return make_int2(page, slot);
+}
+
+// Keys [lo, hi) visible to the query at key position `pos` of a request with
+// `klen` keys.
+__device__ __forceinline__ int2 visible_keys(const PagedArgs& a, int klen, int pos) {
+  long long hi = klen;
+  if (a.causal) hi = min(hi, (long long)pos + 1);
+  if (a.win_right >= 0) hi = min(hi, (long long)pos + a.win_right + 1);
+  long long lo = 0;
+  if (a.win_left >= 0) lo = max(lo, (long long)pos - a.win_left);
+  return make_int2((int)min(lo, (long long)klen), (int)max(hi, 0ll));
+}
+
+__device__ __forceinline__ void store_out4(void* base, int64_t idx, int out_dtype, const float (&x)[4], int n) {
+  if (out_dtype == kF32) {
+    float* p = reinterpret_cast<float*>(base) + idx;
+    if (n == 4 && (reinterpret_cast<uintptr_t>(p) & 15) == 0)
+      *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    else
+      for (int i = 0; i < n; ++i) p[i] = x[i];
+  } else if (out_dtype == kF16) {
+    __half* p = reinterpret_cast<__half*>(base) + idx;
+    if (n == 4 && (reinterpret_cast<uintptr_t>(p) & 7) == 0)
+      *reinterpret_cast<uint2*>(p) = make_uint2(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]));
+    else
+      for (int i = 0; i < n; ++i) p[i] = __float2half_rn(x[i]);
+  } else {
+    __nv_bfloat16* p = reinterpret_cast<__nv_bfloat16*>(base) + idx;
+    if (n == 4 && (reinterpret_cast<uintptr_t>(p) & 7) == 0)
+      *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf162(x[0], x[1]), pack_bf162(x[2], x[3]));
+    else
+      for (int i = 0; i < n; ++i) p[i] = __float2bfloat16_rn(x[i]);
+  }
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.69314718055994531f;
+
+// Columns [col, col + 4) of a finished row (token, head): x holds
+// sum exp2(s - m) v and l the sum of exp2(s - m), both over the row's keys
+// (m in log2 units, -inf for no key). Joins the call's partial results (a
+// normalised o and a natural-log lse each) and writes the quotient.
+__device__ __forceinline__ void finish_row4(const PagedArgs& a, int token, int head, int col, float (&x)[4], float m,
+                                            float l) {
+  float top = m;
+  for (int p = 0; p < a.n_parts; ++p)
+    top = fmaxf(top, a.parts_lse[((int64_t)p * a.Hq + head) * a.total_q + token] * kLog2e);
+  const float sub = top == -INFINITY ? 0.f : top;
+  const float f = m == -INFINITY ? 0.f : exp2f(m - sub);
+  l *= f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] *= f;
+  for (int p = 0; p < a.n_parts; ++p) {
+    const float lse = a.parts_lse[((int64_t)p * a.Hq + head) * a.total_q + token];
+    const float w = lse == -INFINITY ? 0.f : exp2f(lse * kLog2e - sub);
+    const float* src = a.parts_o + (((int64_t)p * a.total_q + token) * a.Hq + head) * a.D + col;
+    l += w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (col + i < a.D) x[i] = fmaf(w, src[i], x[i]);
+  }
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] *= inv;
+  store_out4(a.o, (int64_t)token * a.o_st + (int64_t)head * a.o_sh + col, a.out_dtype, x, min(4, a.D - col));
+  if (col == 0 && a.lse != nullptr)
+    a.lse[(int64_t)head * a.total_q + token] = l > 0.f ? sub * kLn2 + logf(l) : -INFINITY;
+}
+
+}  // namespace fa

@@ -1,0 +1,139 @@
+// fa_paged.h - declarations shared by the paged-cache operators: the page
+// planner, the cache append, the attention over a paged cache and their host
+// side (fa_paged_api.cu).
+#pragma once
+
+#include <cstdint>
+#include <string>
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include "../../include/fa_b200.h"
+#include "fa_internal.h"
+
+namespace fa {
+
+// ------------------------------------------------ host state kept in fa_api.cu
+fa_status paged_fail(fa_status st, const std::string& msg);
+// The current device's status words: [0] timeouts, [1] bad page, slot or length.
+fa_status paged_status_words(unsigned** words);
+// Cached RoPE tables of `theta` with at least `rows` rows. Refused while
+// `stream` is being captured unless they are there already (building them
+// allocates and synchronises).
+fa_status paged_rope(float theta, int D, int rows, cudaStream_t stream, const float** cs, const float** sn);
+// Tensor map of a [pages, slots, heads, D] cache of 16-bit values: boxes of
+// `box_rows` slots by 64 columns of one head, 128-byte swizzle.
+fa_status paged_encode(CUtensorMap* m, const void* base, bool bf16, int D, int H, int slots, int pages, int64_t sp,
+                       int64_t ss, int64_t sh, int box_rows);
+unsigned long long paged_wait_limit_ns();
+
+// ------------------------------------------------------------- page planning
+struct PlanArgs {
+  int B, max_pages, page_size, n_free, rows;
+  const int* cached;
+  const int* fresh;
+  const int* free_pages;
+  const int* free_begin;   // NULL = 0
+  int* table;
+  int64_t table_stride;
+  int* seq_lens;           // [B]
+  int* cu;                 // [B + 1]
+  int64_t* slots;          // [rows]
+  int* positions;          // [rows]
+  int* free_end;           // [1]
+  unsigned* status;        // bad-index word
+};
+constexpr int kPlanMaxRequests = 8192;
+cudaError_t launch_plan_pages(const PlanArgs& a, cudaStream_t stream);
+
+// -------------------------------------------------------------- cache append
+struct StoreArgs {
+  int T, Hq, Hk, D, page_size;
+  long long n_slots;       // num_pages * page_size
+  const int64_t* slots;
+  const int* positions;    // NULL: no rotation
+  int table_rows;
+  const float* cs;
+  const float* sn;
+  const void* k;
+  const void* v;
+  const void* q;           // NULL: none
+  int64_t k_st, k_sh, v_st, v_sh, q_st, q_sh;
+  void* kc;
+  void* vc;
+  int64_t kc_sp, kc_ss, kc_sh, vc_sp, vc_ss, vc_sh;
+  void* qo;                // contiguous [T, Hq, D]
+  unsigned* status;
+};
+cudaError_t launch_store_kv(const StoreArgs& a, int dtype, bool vec, cudaStream_t stream);
+
+// ----------------------------------------------------- attention over pages
+// One call's description for every paged attention kernel. The query tokens
+// of request i are rows [cu_q[i], cu_q[i + 1]) of q (row i alone when cu_q is
+// NULL). Its keys are, in order, the first `pre` slots of the pages in
+// pre_table and then the first seq_lens[i] slots of the pages in table row i;
+// query token j of n sits at key position pre + seq_lens[i] - n + j.
+struct PagedArgs {
+  int B, total_q, Hq, Hk, D, group;
+  int page_size, num_pages, max_pages;
+  const int* table;
+  int64_t table_stride;
+  const int* seq_lens;
+  const int* cu_q;
+  int pre;
+  const int* pre_table;
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t q_st, q_sh;
+  int64_t k_sp, k_ss, k_sh;
+  int64_t v_sp, v_ss, v_sh;
+  void* o;
+  int64_t o_st, o_sh;
+  int out_dtype;
+  float* lse;              // [Hq, total_q] natural log (NULL = not written)
+  float scale, scale_log2;
+  float softcap;           // > 0: x = softcap * tanh(scale * q.k / softcap)
+  int causal, win_left, win_right;
+  const float* alibi;      // [Hq] (NULL = none)
+  // Partial results already computed for every row and joined when a row is
+  // finished: o [n_parts, total_q, Hq, D] and lse [n_parts, Hq, total_q].
+  int n_parts;
+  const float* parts_o;
+  const float* parts_lse;
+  // Work that the kernels cut in n_ctas equal runs of key tiles (split = 1):
+  // per run two partial units of rows_per_unit rows, and where they belong.
+  int split;
+  int n_ctas;
+  int rows_per_unit;
+  float* slot_o;           // [n_ctas, 2, rows_per_unit, D] unnormalised
+  float2* slot_ml;         // [n_ctas, 2, rows_per_unit] running max (log2 units) and sum
+  struct RunMeta* meta;    // [n_ctas]
+  unsigned* status;        // [0] timeouts, [1] bad index
+  unsigned long long wait_limit_ns;
+};
+
+// Where one run of the cut work begins (written by the attention kernel, read
+// by the join).
+struct RunMeta {
+  long long begin;         // first key tile of the run, in tiles of the whole call
+  long long unit_begin;    // first and one past the last tile of the unit it begins in
+  long long unit_end;
+  long long total;         // tiles of the whole call
+  int n_runs;              // runs in use (0: run not in use)
+  int q0;                  // first query row of the unit's request
+  int row0;                // first packed row of the unit (row = token * group + head of the group)
+  int rows;                // packed rows of the unit
+  int hk;
+};
+
+// CUDA-core kernel: fp32 inputs, and 16-bit inputs the tensor cores' copies
+// cannot take (any head_dim <= 256, any strides and alignment).
+int simt_rows_per_unit(int dtype, bool vec, int D, long long rows);
+int simt_ctas(int D);
+cudaError_t launch_paged_simt(const PagedArgs& a, int dtype, bool vec, cudaStream_t stream);
+// Join of the runs' partial units.
+cudaError_t launch_paged_join(const PagedArgs& a, cudaStream_t stream);
+
+}  // namespace fa

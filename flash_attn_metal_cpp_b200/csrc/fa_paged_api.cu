@@ -1,0 +1,306 @@
+// fa_paged_api.cu - host side of the paged-cache operators: argument checks,
+// choice of kernel, scratch layout, launches (include/fa_b200.h).
+//
+// Nothing here reads device memory, allocates or synchronises (the RoPE
+// tables of a new theta excepted), so every call can be captured in a graph
+// and replayed while the lengths, pages and slots on the device change.
+#include "fa_paged.h"
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+namespace fa {
+namespace {
+
+size_t elem_size(int dt) { return dt == kF32 ? 4 : 2; }
+size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
+bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+fa_status cuda_status(cudaError_t e, const char* what) {
+  return e == cudaSuccess ? FA_OK : paged_fail(FA_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+}
+
+struct Checked {
+  PagedArgs a;
+  int dtype;
+  bool vec;              // strides are multiples of 16 bytes
+  int64_t nk[2], nv[2];  // strides of the new rows (append)
+};
+
+// `grouped`: query heads share the KV heads (the append takes any number).
+fa_status check(const fa_paged_params* p, Checked* c, bool grouped = true) {
+  if (!p) return paged_fail(FA_ERR_INVALID_ARG, "params is NULL");
+  if (p->dtype < 0 || p->dtype > 2) return paged_fail(FA_ERR_INVALID_ARG, "dtype must be 0 (f16), 1 (bf16) or 2 (f32)");
+  if (p->out_dtype > 2) return paged_fail(FA_ERR_INVALID_ARG, "out_dtype must be -1, 0, 1 or 2");
+  if (p->head_dim == 0 || p->head_dim > 256) return paged_fail(FA_ERR_UNSUPPORTED, "head_dim must be in [1, 256]");
+  if (p->num_heads_k == 0 || p->num_heads_q > 65535 || p->num_heads_k > 65535 ||
+      (grouped && p->num_heads_q % p->num_heads_k != 0))
+    return paged_fail(FA_ERR_INVALID_ARG, "num_heads_q must be a positive multiple of num_heads_k");
+  const uint64_t lim = 1ull << 30;
+  if (p->page_size == 0) return paged_fail(FA_ERR_INVALID_ARG, "page_size must be positive");
+  if (p->batch_size > lim || p->total_q > lim || p->page_size > lim || p->num_pages > lim || p->max_pages > lim ||
+      p->prefix_pages > lim)
+    return paged_fail(FA_ERR_INVALID_ARG, "tensor dimensions out of range");
+  if (p->prefix_len > lim / 2 || (uint64_t)p->prefix_len > (uint64_t)p->prefix_pages * p->page_size)
+    return paged_fail(FA_ERR_INVALID_ARG, "prefix_len is beyond the pages of the prefix table");
+  if (!std::isfinite(p->softmax_scale)) return paged_fail(FA_ERR_INVALID_ARG, "softmax_scale must be finite");
+  if (!std::isfinite(p->softcap) || p->softcap < 0.f)
+    return paged_fail(FA_ERR_INVALID_ARG, "softcap must be 0 (off) or positive and finite");
+
+  PagedArgs& a = c->a;
+  std::memset(&a, 0, sizeof(a));
+  a.B = (int)p->batch_size;
+  a.total_q = (int)p->total_q;
+  a.Hq = (int)p->num_heads_q;
+  a.Hk = (int)p->num_heads_k;
+  a.D = (int)p->head_dim;
+  a.group = a.Hq / a.Hk;
+  a.page_size = (int)p->page_size;
+  a.num_pages = (int)p->num_pages;
+  a.max_pages = (int)p->max_pages;
+  a.table_stride = p->table_stride ? p->table_stride : (int64_t)p->max_pages;
+  a.pre = (int)p->prefix_len;
+  const int64_t row_q = (int64_t)a.Hq * a.D, row_k = (int64_t)a.Hk * a.D;
+  auto two = [&](const int64_t in[2], int64_t row, int64_t* s0, int64_t* s1) {
+    const bool none = in[0] == 0 && in[1] == 0;
+    *s0 = none ? row : in[0];
+    *s1 = none ? a.D : in[1];
+    return *s0 >= 0 && *s1 >= 0;
+  };
+  auto three = [&](const int64_t in[3], int64_t* s0, int64_t* s1, int64_t* s2) {
+    const bool none = in[0] == 0 && in[1] == 0 && in[2] == 0;
+    *s0 = none ? row_k * a.page_size : in[0];
+    *s1 = none ? row_k : in[1];
+    *s2 = none ? a.D : in[2];
+    return *s0 >= 0 && *s1 >= 0 && *s2 >= 0;
+  };
+  bool ok = a.table_stride >= 0;
+  ok &= two(p->q_stride, row_q, &a.q_st, &a.q_sh);
+  ok &= two(p->o_stride, row_q, &a.o_st, &a.o_sh);
+  ok &= two(p->new_k_stride, row_k, &c->nk[0], &c->nk[1]);
+  ok &= two(p->new_v_stride, row_k, &c->nv[0], &c->nv[1]);
+  ok &= three(p->k_stride, &a.k_sp, &a.k_ss, &a.k_sh);
+  ok &= three(p->v_stride, &a.v_sp, &a.v_ss, &a.v_sh);
+  if (!ok) return paged_fail(FA_ERR_INVALID_ARG, "strides must be non-negative");
+  a.out_dtype = p->out_dtype < 0 ? p->dtype : p->out_dtype;
+  a.scale = p->softmax_scale;
+  a.scale_log2 = (float)((double)p->softmax_scale * 1.4426950408889634);
+  a.softcap = p->softcap;
+  a.causal = p->is_causal ? 1 : 0;
+  a.win_left = p->window_left < 0 ? -1 : p->window_left;
+  a.win_right = p->window_right < 0 ? -1 : p->window_right;
+  a.alibi = p->alibi_slopes;
+  c->dtype = p->dtype;
+  const int64_t m = 16 / (int64_t)elem_size(p->dtype);
+  auto al = [&](int64_t s) { return s % m == 0; };
+  c->vec = a.D % m == 0 && al(a.q_st) && al(a.q_sh) && al(a.k_sp) && al(a.k_ss) && al(a.k_sh) && al(a.v_sp) &&
+           al(a.v_ss) && al(a.v_sh);
+  return FA_OK;
+}
+
+// Most packed rows (query tokens times heads of a group) of one request.
+long long max_rows(const fa_paged_params* p, const PagedArgs& a, bool one_token) {
+  if (one_token) return a.group;
+  const long long q = p->max_seqlen_q ? std::min(p->max_seqlen_q, p->total_q) : p->total_q;
+  return std::max(1ll, q) * a.group;
+}
+
+// Scratch of the cut work: run records, running max and sum, partial rows.
+struct CutLayout {
+  size_t ml, o, bytes;
+};
+CutLayout cut_layout(int n_ctas, int rows, int D) {
+  CutLayout l;
+  l.ml = up256((size_t)n_ctas * sizeof(RunMeta));
+  l.o = l.ml + up256((size_t)n_ctas * 2 * rows * sizeof(float2));
+  l.bytes = l.o + up256((size_t)n_ctas * 2 * rows * ((D + 3) & ~3) * sizeof(float));
+  return l;
+}
+
+void place_cut(PagedArgs& a, const CutLayout& l, void* ws) {
+  uint8_t* w = static_cast<uint8_t*>(ws);
+  a.meta = reinterpret_cast<RunMeta*>(w);
+  a.slot_ml = reinterpret_cast<float2*>(w + l.ml);
+  a.slot_o = reinterpret_cast<float*>(w + l.o);
+}
+
+}  // namespace
+}  // namespace fa
+
+using namespace fa;
+
+extern "C" {
+
+void fa_paged_params_init(fa_paged_params* p) {
+  if (!p) return;
+  std::memset(p, 0, sizeof(*p));
+  p->window_left = -1;
+  p->window_right = -1;
+  p->dtype = FA_F16;
+  p->out_dtype = -1;
+}
+
+fa_status fa_plan_pages(uint32_t batch, uint32_t page_size, uint32_t max_pages, uint32_t n_free, uint32_t rows,
+                        const int32_t* cached, const int32_t* fresh, const int32_t* free_pages,
+                        const int32_t* free_begin, int32_t* table, int64_t table_stride, int32_t* seq_lens,
+                        int32_t* cu, int64_t* slots, int32_t* positions, int32_t* free_end, void* stream) {
+  if (batch > (uint32_t)kPlanMaxRequests)
+    return paged_fail(FA_ERR_UNSUPPORTED, "at most " + std::to_string(kPlanMaxRequests) + " requests a plan");
+  const uint32_t lim = 1u << 30;
+  if (page_size == 0 || page_size > lim || max_pages > lim || n_free > lim || rows > lim || table_stride < 0)
+    return paged_fail(FA_ERR_INVALID_ARG, "plan dimensions out of range");
+  if ((batch && (!cached || !fresh || !seq_lens || (max_pages && !table))) || !cu || !free_end ||
+      (rows && (!slots || !positions)) || (n_free && !free_pages))
+    return paged_fail(FA_ERR_INVALID_ARG, "NULL plan pointer");
+  if (free_begin == free_end) return paged_fail(FA_ERR_INVALID_ARG, "free_begin and free_end must not overlap");
+  unsigned* words = nullptr;
+  fa_status st = paged_status_words(&words);
+  if (st != FA_OK) return st;
+  PlanArgs a{};
+  a.B = (int)batch;
+  a.max_pages = (int)max_pages;
+  a.page_size = (int)page_size;
+  a.n_free = (int)n_free;
+  a.rows = (int)rows;
+  a.cached = cached;
+  a.fresh = fresh;
+  a.free_pages = free_pages;
+  a.free_begin = free_begin;
+  a.table = table;
+  a.table_stride = table_stride ? table_stride : (int64_t)max_pages;
+  a.seq_lens = seq_lens;
+  a.cu = cu;
+  a.slots = slots;
+  a.positions = positions;
+  a.free_end = free_end;
+  a.status = words;
+  return cuda_status(launch_plan_pages(a, static_cast<cudaStream_t>(stream)), "page planning");
+}
+
+fa_status fa_store_kv(const fa_paged_params* p, const void* k, const void* v, void* k_cache, void* v_cache,
+                      const int64_t* slots, const int32_t* positions, const float* cos, const float* sin,
+                      uint32_t table_rows, float rope_theta, const void* q, void* q_out, void* stream) {
+  Checked c;
+  fa_status st = check(p, &c, false);
+  if (st != FA_OK) return st;
+  const PagedArgs& g = c.a;
+  if (g.total_q == 0) return FA_OK;
+  if (!k || !v || !slots || (g.num_pages && (!k_cache || !v_cache)))
+    return paged_fail(FA_ERR_INVALID_ARG, "NULL tensor pointer");
+  if ((q == nullptr) != (q_out == nullptr)) return paged_fail(FA_ERR_INVALID_ARG, "q and q_out go together");
+  if ((cos == nullptr) != (sin == nullptr)) return paged_fail(FA_ERR_INVALID_ARG, "cos and sin tables go together");
+  if (table_rows > (1u << 30)) return paged_fail(FA_ERR_INVALID_ARG, "table_rows out of range");
+  const bool rotate = positions != nullptr;
+  if (rotate && !cos && (!(rope_theta > 0.f) || !std::isfinite(rope_theta)))
+    return paged_fail(FA_ERR_INVALID_ARG, "positions need cos/sin tables or rope_theta > 0");
+  if (rotate && !cos && g.D % 2 != 0)
+    return paged_fail(FA_ERR_UNSUPPORTED, "RoPE from rope_theta needs an even head_dim");
+  if (!rotate && (cos || rope_theta != 0.f))
+    return paged_fail(FA_ERR_INVALID_ARG, "cos/sin tables and rope_theta need positions");
+  StoreArgs a{};
+  st = paged_status_words(&a.status);
+  if (st != FA_OK) return st;
+  const float *cs = cos, *sn = sin;
+  if (rotate && !cos && table_rows > 0) {
+    st = paged_rope(rope_theta, g.D, (int)table_rows, static_cast<cudaStream_t>(stream), &cs, &sn);
+    if (st != FA_OK) return st;
+  }
+  a.T = g.total_q;
+  a.Hq = q ? g.Hq : 0;
+  a.Hk = g.Hk;
+  a.D = g.D;
+  a.page_size = g.page_size;
+  a.n_slots = (long long)g.num_pages * g.page_size;
+  a.slots = slots;
+  a.positions = positions;
+  a.table_rows = rotate ? (int)table_rows : 0;
+  a.cs = cs;
+  a.sn = sn;
+  a.k = k;
+  a.v = v;
+  a.q = q;
+  a.k_st = c.nk[0];
+  a.k_sh = c.nk[1];
+  a.v_st = c.nv[0];
+  a.v_sh = c.nv[1];
+  a.q_st = g.q_st;
+  a.q_sh = g.q_sh;
+  a.kc = k_cache;
+  a.vc = v_cache;
+  a.kc_sp = g.k_sp;
+  a.kc_ss = g.k_ss;
+  a.kc_sh = g.k_sh;
+  a.vc_sp = g.v_sp;
+  a.vc_ss = g.v_ss;
+  a.vc_sh = g.v_sh;
+  a.qo = q_out;
+  // 16-byte pieces of 8 columns in both halves of a row, from every tensor.
+  const int64_t m = 16 / (int64_t)elem_size(c.dtype);
+  auto al = [&](int64_t s) { return s % m == 0; };
+  bool vec = g.D % 16 == 0 && al(a.k_st) && al(a.k_sh) && al(a.v_st) && al(a.v_sh) && al(a.kc_sp) && al(a.kc_ss) &&
+             al(a.kc_sh) && al(a.vc_sp) && al(a.vc_ss) && al(a.vc_sh) && aligned(k, 16) && aligned(v, 16) &&
+             aligned(k_cache, 16) && aligned(v_cache, 16);
+  if (q) vec &= al(a.q_st) && al(a.q_sh) && aligned(q, 16) && aligned(q_out, 16);
+  if (rotate) vec &= aligned(cs, 16) && aligned(sn, 16);
+  return cuda_status(launch_store_kv(a, c.dtype, vec, static_cast<cudaStream_t>(stream)), "cache append");
+}
+
+size_t fa_paged_workspace_size(const fa_paged_params* p) {
+  Checked c;
+  if (check(p, &c) != FA_OK) return 0;
+  const PagedArgs& a = c.a;
+  // Whatever the tensors' base addresses allow: the largest of the kernels'.
+  size_t ws = cut_layout(simt_ctas(a.D), c.dtype == kF32 ? (a.D <= 128 ? 4 : 2) : 1, a.D).bytes;
+  return ws;
+}
+
+fa_status fa_paged_forward(const fa_paged_params* p, const void* q, const void* k_cache, const void* v_cache,
+                           const int32_t* block_table, const int32_t* seq_lens, const int32_t* cu_seqlens_q,
+                           const int32_t* prefix_table, void* o, float* lse, void* workspace,
+                           size_t workspace_bytes, void* stream) {
+  Checked c;
+  fa_status st = check(p, &c);
+  if (st != FA_OK) return st;
+  PagedArgs& a = c.a;
+  if (a.total_q == 0 || a.B == 0 || a.Hq == 0) return FA_OK;
+  if (!q || !o || !seq_lens || (a.max_pages && !block_table) || (a.pre && !prefix_table) ||
+      (a.num_pages && (!k_cache || !v_cache)))
+    return paged_fail(FA_ERR_INVALID_ARG, "NULL tensor pointer");
+  const size_t need = fa_paged_workspace_size(p);
+  if (!workspace || workspace_bytes < need)
+    return paged_fail(FA_ERR_INVALID_ARG, "workspace smaller than fa_paged_workspace_size()");
+  if (!aligned(workspace, 256)) return paged_fail(FA_ERR_INVALID_ARG, "workspace must be 256-byte aligned");
+  st = paged_status_words(&a.status);
+  if (st != FA_OK) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  a.table = block_table;
+  a.seq_lens = seq_lens;
+  a.cu_q = cu_seqlens_q;
+  a.pre_table = prefix_table;
+  a.q = q;
+  a.k = k_cache;
+  a.v = v_cache;
+  a.o = o;
+  a.lse = lse;
+  a.wait_limit_ns = paged_wait_limit_ns();
+  const bool vec = c.vec && aligned(q, 16) && aligned(k_cache, 16) && aligned(v_cache, 16);
+  const long long rows = max_rows(p, a, cu_seqlens_q == nullptr);
+  const long long keys = (long long)a.pre + (long long)a.max_pages * a.page_size;
+
+  // CUDA cores.
+  a.rows_per_unit = simt_rows_per_unit(c.dtype, vec, a.D, rows);
+  a.n_ctas = simt_ctas(a.D);
+  a.split = keys > 256;
+  if (!a.split) {
+    const long long chunks = cu_seqlens_q ? ((long long)a.total_q * a.group) / a.rows_per_unit + a.B
+                                          : (long long)a.B * ((a.group + a.rows_per_unit - 1) / a.rows_per_unit);
+    a.n_ctas = (int)std::min<long long>(chunks * a.Hk, 148 * 16);
+  }
+  place_cut(a, cut_layout(a.n_ctas, a.rows_per_unit, a.D), workspace);
+  st = cuda_status(launch_paged_simt(a, c.dtype, vec, s), "paged attention (CUDA cores)");
+  if (st == FA_OK && a.split) st = cuda_status(launch_paged_join(a, s), "paged attention (join)");
+  return st;
+}
+
+}  // extern "C"

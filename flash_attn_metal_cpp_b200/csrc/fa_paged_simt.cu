@@ -1,0 +1,337 @@
+// fa_paged_simt.cu - CUDA-core attention over a paged cache, and the join of
+// partial units that it shares with the tensor-core decoding kernel.
+//
+// Right for every case: fp32 (kept in fp32 end to end), any head_dim up to
+// 256, any strides and alignment, any number of query rows. Online softmax in
+// log2 units as in the other kernels: x = scale q.k (capped, biased), running
+// m and l, o = sum exp2(x - m) v.
+//
+// One block of 4 warps works through its run of tiles (fa_paged.cuh). In a
+// warp 8 lanes share one key (each holds every 8th 16-byte piece of its row),
+// so 4 keys are in work at once and a dot product needs 3 shuffles; every
+// group of 8 lanes keeps its own m, l and o until the unit ends. A unit has 1
+// row (one query head on a KV head) or 4 rows (2 for head_dim above 128) that
+// use each key row loaded. fp32 decoding is bound by memory latency, so the
+// grid asks for several blocks an SM.
+#include "fa_paged.cuh"
+
+#include <algorithm>
+
+namespace fa {
+namespace {
+
+constexpr int kTile = 64;
+constexpr int kThreads = 128;
+
+// DPL elements of a row: lane `sub` of 8 holds vectors sub, sub + 8, ...
+template <typename T, int DPL, bool VEC>
+__device__ __forceinline__ void load_slice(const T* row, int sub, int D, float (&x)[DPL]) {
+  if constexpr (VEC) {
+    static_assert(sizeof(T) == 4, "vector slices are used for fp32 only");
+#pragma unroll
+    for (int i = 0; i < DPL / 4; ++i) {
+      const int col = (i * 8 + sub) * 4;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (col < D) v = *reinterpret_cast<const float4*>(row + col);
+      x[4 * i] = v.x;
+      x[4 * i + 1] = v.y;
+      x[4 * i + 2] = v.z;
+      x[4 * i + 3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < DPL; ++i) {
+      const int col = i * 8 + sub;
+      x[i] = col < D ? cvt_in<T>(row[col]) : 0.f;
+    }
+  }
+}
+
+template <int DPL, bool VEC>
+__device__ __forceinline__ int slice_col(int sub, int i) {
+  return VEC ? ((i / 4) * 8 + sub) * 4 + (i & 3) : i * 8 + sub;
+}
+
+template <typename T, int DM, int R, bool VEC>
+__global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a) {
+  constexpr int DPL = DM / 8;
+  __shared__ RunScratch scratch;
+  __shared__ float sm_o[4][R][DM];
+  __shared__ float sm_m[4][R], sm_l[4][R];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int sub = lane & 7, kg = lane >> 3;
+  const int sd = (a.D + 3) & ~3;
+
+  grid_dep_wait();
+  grid_dep_launch_dependents();
+  const Run run = find_run<kTile, kThreads>(a, R, blockIdx.x, gridDim.x, 1, &scratch);
+  if (run.end <= run.begin) {
+    if (a.split && tid == 0) a.meta[blockIdx.x].n_runs = 0;
+    return;
+  }
+  const T* Q = reinterpret_cast<const T*>(a.q);
+  const T* K = reinterpret_cast<const T*>(a.k);
+  const T* V = reinterpret_cast<const T*>(a.v);
+
+  int req = run.req;
+  long long req_begin = run.req_begin;
+  ReqView v = view_request<kTile>(a, req, R);
+  long long at = run.begin;
+  while (at < run.end) {
+    const int per = v.per_unit(a);
+    const long long off = at - req_begin;
+    if (off >= (long long)v.units * per) {
+      req_begin += (long long)v.units * per;
+      v = view_request<kTile>(a, ++req, R);
+      continue;
+    }
+    const int unit = (int)(off / per);
+    const int t0 = v.tile_lo + (a.split ? (int)(off - (long long)unit * per) : 0);
+    const int t_end = v.tile_lo + v.tiles;
+    const int t1 = a.split ? (int)min((long long)t_end, t0 + (run.end - at)) : t_end;
+    const int hk = unit % a.Hk;
+    const int row0 = unit / a.Hk * R;
+    const int rows = min(R, v.qlen * a.group - row0);
+    if (a.split && at == run.begin && tid == 0) {
+      RunMeta& mt = a.meta[blockIdx.x];
+      mt.begin = run.begin;
+      mt.unit_begin = req_begin + (long long)unit * per;
+      mt.unit_end = mt.unit_begin + per;
+      mt.total = run.total;
+      mt.n_runs = run.n_runs;
+      mt.q0 = v.q0;
+      mt.row0 = row0;
+      mt.rows = rows;
+      mt.hk = hk;
+    }
+
+    float q[R][DPL], o[R][DPL], m[R], l[R];
+    int2 vis[R];
+    float slope[R];
+    int qpos[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int row = row0 + min(r, rows - 1);
+      const int j = row / a.group, head = hk * a.group + row % a.group;
+      load_slice<T, DPL, VEC>(Q + (int64_t)(v.q0 + j) * a.q_st + (int64_t)head * a.q_sh, sub, a.D, q[r]);
+      qpos[r] = v.klen - v.qlen + j;
+      vis[r] = visible_keys(a, v.klen, qpos[r]);
+      slope[r] = a.alibi ? a.alibi[head] : 0.f;
+      m[r] = -INFINITY;
+      l[r] = 0.f;
+#pragma unroll
+      for (int i = 0; i < DPL; ++i) o[r][i] = 0.f;
+    }
+    const int key_end = min(v.klen, t1 * kTile);
+    for (int base = t0 * kTile + warp * 4; base < key_end; base += 16) {
+      const int key = base + kg;
+      float kx[DPL], vx[DPL];
+      bool on = key < key_end && key >= v.key_lo;
+      if (on) {
+        const int2 ps = find_key(a, req, key);
+        on = ps.x >= 0;
+        if (on) {
+          load_slice<T, DPL, VEC>(K + (int64_t)ps.x * a.k_sp + (int64_t)ps.y * a.k_ss + (int64_t)hk * a.k_sh, sub, a.D, kx);
+          load_slice<T, DPL, VEC>(V + (int64_t)ps.x * a.v_sp + (int64_t)ps.y * a.v_ss + (int64_t)hk * a.v_sh, sub, a.D, vx);
+        }
+      }
+      if (!on) {
+#pragma unroll
+        for (int i = 0; i < DPL; ++i) kx[i] = vx[i] = 0.f;
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < DPL; ++i) s = fmaf(q[r][i], kx[i], s);
+        s += __shfl_xor_sync(0xffffffffu, s, 1);
+        s += __shfl_xor_sync(0xffffffffu, s, 2);
+        s += __shfl_xor_sync(0xffffffffu, s, 4);
+        if (on && key >= vis[r].x && key < vis[r].y) {
+          float x;
+          if (a.softcap > 0.f) x = a.softcap * tanhf(s * a.scale / a.softcap);
+          else x = s * a.scale;
+          x = fmaf(slope[r], (float)(key - qpos[r]), x) * kLog2e;
+          // (a score of -inf, an overflow, leaves the row as it is)
+          if (x > m[r]) {
+            const float f = m[r] == -INFINITY ? 0.f : exp2f(m[r] - x);
+            l[r] *= f;
+#pragma unroll
+            for (int i = 0; i < DPL; ++i) o[r][i] *= f;
+            m[r] = x;
+          }
+          const float p = x == -INFINITY ? 0.f : exp2f(x - m[r]);
+          l[r] += p;
+#pragma unroll
+          for (int i = 0; i < DPL; ++i) o[r][i] = fmaf(p, vx[i], o[r][i]);
+        }
+      }
+    }
+    // The warp's four key groups, then the block's four warps.
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float top = fmaxf(m[r], __shfl_xor_sync(0xffffffffu, m[r], 8));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+      const float f = m[r] == -INFINITY ? 0.f : exp2f(m[r] - top);
+      float ls = l[r] * f;
+      ls += __shfl_xor_sync(0xffffffffu, ls, 8);
+      ls += __shfl_xor_sync(0xffffffffu, ls, 16);
+#pragma unroll
+      for (int i = 0; i < DPL; ++i) {
+        float x = o[r][i] * f;
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        if (kg == 0) sm_o[warp][r][slice_col<DPL, VEC>(sub, i)] = x;
+      }
+      if (lane == 0) {
+        sm_m[warp][r] = top;
+        sm_l[warp][r] = ls;
+      }
+    }
+    __syncthreads();
+    const bool whole = t0 == v.tile_lo && t1 == t_end;
+    const int slot = blockIdx.x * 2 + (at == run.begin ? 0 : 1);
+    for (int e = tid; e < rows * (DM / 4); e += kThreads) {
+      const int r = e / (DM / 4), col = e % (DM / 4) * 4;
+      if (col >= a.D) continue;
+      float top = sm_m[0][r];
+#pragma unroll
+      for (int w = 1; w < 4; ++w) top = fmaxf(top, sm_m[w][r]);
+      float x[4] = {0.f, 0.f, 0.f, 0.f}, ls = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float f = sm_m[w][r] == -INFINITY ? 0.f : exp2f(sm_m[w][r] - top);
+        ls = fmaf(f, sm_l[w][r], ls);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = fmaf(f, sm_o[w][r][col + i], x[i]);
+      }
+      if (whole) {
+        const int row = row0 + r;
+        finish_row4(a, v.q0 + row / a.group, hk * a.group + row % a.group, col, x, top, ls);
+      } else {
+        const int64_t sr = (int64_t)slot * a.rows_per_unit + r;
+        *reinterpret_cast<float4*>(a.slot_o + sr * sd + col) = make_float4(x[0], x[1], x[2], x[3]);
+        if (col == 0) a.slot_ml[sr] = make_float2(top, ls);
+      }
+    }
+    __syncthreads();
+    at += a.split ? t1 - t0 : 1;
+  }
+}
+
+// One block joins one row of one unit that was cut between runs: the block of
+// the unit's first cut does it, the others return. The maximum first, then
+// the weighted sums, eight runs at a time (a single long request on one KV
+// head leaves as many partial rows as there are runs); the order is fixed.
+constexpr int kJoinWarps = 8;
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const PagedArgs a) {
+  __shared__ float sm_o[kJoinWarps][256];
+  __shared__ float sm_l[kJoinWarps];
+  grid_dep_wait();
+  grid_dep_launch_dependents();
+  const int b = blockIdx.x + 1, r = blockIdx.y;
+  const RunMeta mt = a.meta[b];
+  if (mt.n_runs == 0 || r >= mt.rows || mt.begin == mt.unit_begin) return;
+  const long long prev = mt.total * (b - 1) / mt.n_runs;
+  if (prev > mt.unit_begin) return;
+  const int first = b - 1;
+  int last = b;  // one past the last run with tiles of the unit
+  while (last < mt.n_runs && mt.total * last / mt.n_runs < mt.unit_end) ++last;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int sd = (a.D + 3) & ~3;
+  auto row_of = [&](int run) {
+    const int slot = run * 2 + ((run == first && prev != mt.unit_begin) ? 1 : 0);
+    return (int64_t)slot * a.rows_per_unit + r;
+  };
+  float top = -INFINITY;
+  for (int j = first + lane; j < last; j += 32) top = fmaxf(top, a.slot_ml[row_of(j)].x);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+  float acc[2][4] = {}, l = 0.f;
+#pragma unroll 4
+  for (int j = first + warp; j < last; j += kJoinWarps) {
+    const int64_t sr = row_of(j);
+    const float2 ml = a.slot_ml[sr];
+    const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
+    l = fmaf(f, ml.y, l);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int col = c * 128 + lane * 4;
+      if (col < a.D) {
+        const float4 x = *reinterpret_cast<const float4*>(a.slot_o + sr * sd + col);
+        acc[c][0] = fmaf(f, x.x, acc[c][0]);
+        acc[c][1] = fmaf(f, x.y, acc[c][1]);
+        acc[c][2] = fmaf(f, x.z, acc[c][2]);
+        acc[c][3] = fmaf(f, x.w, acc[c][3]);
+      }
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sm_o[warp][c * 128 + lane * 4 + i] = acc[c][i];
+  if (lane == 0) sm_l[warp] = l;
+  __syncthreads();
+  const int col = threadIdx.x * 4;
+  if (col >= a.D) return;
+  float x[4] = {0.f, 0.f, 0.f, 0.f}, ls = 0.f;
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) {
+    ls += sm_l[w];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] += sm_o[w][col + i];
+  }
+  const int row = mt.row0 + r;
+  finish_row4(a, mt.q0 + row / a.group, mt.hk * a.group + row % a.group, col, x, top, ls);
+}
+
+template <typename T, int DM, int R, bool VEC>
+cudaError_t launch_one(const PagedArgs& a, cudaStream_t st) {
+  cudaError_t e = launch_pdl(paged_simt_kernel<T, DM, R, VEC>, dim3((unsigned)a.n_ctas), dim3(kThreads), 0, st, a);
+  note_launch();
+  return e;
+}
+
+template <typename T, bool VEC>
+cudaError_t launch_dm(const PagedArgs& a, cudaStream_t st) {
+  const bool one = a.rows_per_unit == 1;
+  if constexpr (VEC) {
+    if (a.D <= 64) return one ? launch_one<T, 64, 1, true>(a, st) : launch_one<T, 64, 4, true>(a, st);
+    if (a.D <= 128) return one ? launch_one<T, 128, 1, true>(a, st) : launch_one<T, 128, 4, true>(a, st);
+    return one ? launch_one<T, 256, 1, true>(a, st) : launch_one<T, 256, 2, true>(a, st);
+  } else {
+    if (a.D <= 64) return launch_one<T, 64, 1, false>(a, st);
+    if (a.D <= 128) return launch_one<T, 128, 1, false>(a, st);
+    return launch_one<T, 256, 1, false>(a, st);
+  }
+}
+
+}  // namespace
+
+// Rows a unit: the 16-byte path of fp32 takes 4 (2 above 128 columns, where
+// q and o of 4 rows would not fit the registers) as soon as a request has
+// more than one row on a KV head.
+int simt_rows_per_unit(int dtype, bool vec, int D, long long rows) {
+  if (dtype != kF32 || !vec || rows <= 1) return 1;
+  return D <= 128 ? 4 : 2;
+}
+
+int simt_ctas(int D) { return 148 * (D <= 64 ? 8 : 4); }
+
+cudaError_t launch_paged_simt(const PagedArgs& a, int dtype, bool vec, cudaStream_t st) {
+  switch (dtype) {
+    case kF16: return launch_dm<__half, false>(a, st);
+    case kBF16: return launch_dm<__nv_bfloat16, false>(a, st);
+    default: return vec ? launch_dm<float, true>(a, st) : launch_dm<float, false>(a, st);
+  }
+}
+
+cudaError_t launch_paged_join(const PagedArgs& a, cudaStream_t st) {
+  if (a.n_ctas < 2) return cudaSuccess;
+  cudaError_t e = launch_pdl(paged_join_kernel, dim3((unsigned)(a.n_ctas - 1), (unsigned)a.rows_per_unit),
+                             dim3(kJoinWarps * 32), 0, st, a);
+  note_launch();
+  return e;
+}
+
+}  // namespace fa

@@ -28,6 +28,9 @@
  *   fa_forward_range     <- (no counterpart) row/key-range forward with optional
  *                           output routing to peer devices (split-KV over NVLink)
  *   fa_ipc_*             <- (no counterpart) CUDA IPC staging buffers for the routing
+ *   fa_plan_pages, fa_store_kv, fa_paged_forward
+ *                       <- (no counterpart) KV cache in pages: planning of a step,
+ *                           append, and attention over it
  *   fa_last_error       <- std::cerr messages / RuntimeError text
  *                                                            python/bindings.cpp:46-49,224-232
  *
@@ -63,7 +66,9 @@ typedef enum fa_status {
     FA_ERR_RANGE = 5,         /* reserved: no longer returned (operands beyond the fp16
                                  range are rescaled by a power of two, see fa_forward) */
     FA_ERR_NOT_INITIALIZED = 6,
-    FA_ERR_NO_DEVICE = 7
+    FA_ERR_NO_DEVICE = 7,
+    FA_ERR_BAD_INDEX = 8      /* a paged operator met a page, slot, position or length outside
+                                 its cache, table or free list (fa_check_device_status) */
 } fa_status;
 
 typedef enum fa_dtype {
@@ -259,10 +264,11 @@ fa_status fa_pool_stats(uint64_t* hits, uint64_t* misses, uint64_t* bytes_reserv
  * host threads must have finished enqueuing. */
 fa_status fa_pool_clear(void);
 
-/* Read and clear the in-kernel status word of the current device (after the
+/* Read and clear the in-kernel status words of the current device (after the
  * stream has been synchronised). Returns FA_ERR_TIMEOUT when a kernel of
  * this library (other than fa_forward_noalloc's) gave up a wait since the
- * last call, else FA_OK. */
+ * last call, FA_ERR_BAD_INDEX when a paged operator met an index on the
+ * device that it had to skip (see the paged operators), else FA_OK. */
 fa_status fa_check_device_status(void);
 
 /* Wall-clock limit of every in-kernel wait of later launches, in seconds
@@ -320,6 +326,121 @@ fa_status fa_forward_noalloc(const fa_params* p, const void* q, const void* k,
  * cudaMemcpy / cudaMemset, allocating nothing. FA_ERR_TIMEOUT when a wait
  * ran out since the last call (that call's output is invalid), else FA_OK. */
 fa_status fa_noalloc_check_status(void);
+
+/* ------------------------------------------------------------------------
+ * KV cache in pages (no counterpart in the reference).
+ *
+ * A cache is two tensors, K and V, of num_pages pages of page_size slots:
+ * [num_pages, page_size, num_heads_k, head_dim] with any element strides
+ * (head_dim stride 1). Row i of the block table lists the pages of request i
+ * in order: token p of the request lives in page table[i][p / page_size],
+ * slot p % page_size. A slot's number is page * page_size + slot. A serving
+ * step is fa_plan_pages once, then fa_store_kv and fa_paged_forward for each
+ * layer, all on device lengths, so a step can be captured in a CUDA graph
+ * and replayed for other lengths.
+ *
+ * Lengths, pages and slots live on the device, so the host cannot check
+ * them. The kernels do: an index outside its cache, table or free list is
+ * skipped, never followed, the rows that needed it are unspecified, and
+ * fa_check_device_status then reports FA_ERR_BAD_INDEX. All entry points
+ * enqueue on `stream` and return without synchronising; none allocates
+ * (except the first use of a rope_theta, see fa_store_kv). */
+
+/* One step's pages, from the requests' lengths. For request i with cached[i]
+ * tokens in the cache and fresh[i] tokens to append:
+ *   table        row i gets the pages that the new tokens need behind the ones
+ *                it holds, taken from free_pages in the order of the requests;
+ *                all other entries are left as they were
+ *   seq_lens[i]  = cached[i] + fresh[i]
+ *   cu           [batch + 1] first new token of each request, and their sum
+ *   slots[t]     slot number of new token t (cu order), -1 for the rows behind
+ *                the last token; positions[t] its position (0 behind the last)
+ *   free_end     [1] first entry of free_pages that is still free
+ * free_pages is read from entry free_begin[0] on (NULL = 0). When it runs out,
+ * or a request outgrows its table row, the tokens without a page get slot -1
+ * (and table entries -1) and the status word is set. All arrays are device
+ * memory; free_end and free_begin must not overlap. batch <= 8192,
+ * rows <= 2^30. */
+fa_status fa_plan_pages(uint32_t batch, uint32_t page_size, uint32_t max_pages, uint32_t n_free, uint32_t rows,
+                        const int32_t* cached, const int32_t* fresh, const int32_t* free_pages,
+                        const int32_t* free_begin, int32_t* table, int64_t table_stride, int32_t* seq_lens,
+                        int32_t* cu, int64_t* slots, int32_t* positions, int32_t* free_end, void* stream);
+
+/* Parameters of the cache operators. */
+typedef struct fa_paged_params {
+    uint32_t batch_size;      /* requests */
+    uint32_t total_q;         /* query tokens (fa_store_kv: tokens), packed: rows of q */
+    uint32_t max_seqlen_q;    /* most query tokens of one request, as a hint for the choice of
+                                 kernel (0 = unknown); more tokens are still computed */
+    uint32_t num_heads_q;
+    uint32_t num_heads_k;
+    uint32_t head_dim;
+    uint32_t page_size;       /* slots of a page */
+    uint32_t num_pages;       /* pages of the cache */
+    uint32_t max_pages;       /* columns of the block table */
+    float softmax_scale;      /* used as given, as in fa_params */
+    float softcap;            /* > 0: scores are softcap * tanh(scale * q.k / softcap); 0 = off */
+    int32_t is_causal;        /* key position <= query position (see fa_paged_forward) */
+    int32_t window_left;      /* as in fa_params, on these positions */
+    int32_t window_right;
+    int32_t dtype;            /* fa_dtype of q, k, v and the cache */
+    int32_t out_dtype;        /* -1 = dtype */
+    uint32_t prefix_len;      /* shared keys in front of every request's own ones */
+    uint32_t prefix_pages;    /* entries of the prefix table */
+    int64_t q_stride[2];      /* element strides (token, head); all zero = contiguous */
+    int64_t o_stride[2];
+    int64_t new_k_stride[2];  /* fa_store_kv: the new rows of K and V */
+    int64_t new_v_stride[2];
+    int64_t k_stride[3];      /* cache: (page, slot, head); all zero = contiguous */
+    int64_t v_stride[3];
+    int64_t table_stride;     /* row stride of the block table; 0 = max_pages */
+    const float* alibi_slopes; /* float32 [num_heads_q] in device memory; NULL = none */
+} fa_paged_params;
+
+/* Defaults: no cap, no mask, contiguous tensors, out_dtype -1. */
+void fa_paged_params_init(fa_paged_params* p);
+
+/* Append: K and V rows of token t go to slot slots[t] of the cache (slots of
+ * one call are distinct; a negative slot is skipped). With `positions`, K is
+ * rotated on the way by rotate-half RoPE at positions[t], and so is q, whose
+ * rotated rows go to q_out ([total_q, num_heads_q, head_dim], contiguous; q
+ * may be NULL, and q rows are written whether or not their slot is skipped).
+ * The angles come from cos/sin tables ([table_rows, head_dim/2] float32, as
+ * in fa_forward) or, when they are NULL, from the library's tables of
+ * rope_theta with table_rows rows: the first call with a new theta or more
+ * rows builds them (allocating and synchronising, so it is refused while the
+ * stream is being captured). A position without a table row leaves its row
+ * unrotated and sets the status word. Rotation is computed in float32 and
+ * rounded once. */
+fa_status fa_store_kv(const fa_paged_params* p, const void* k, const void* v, void* k_cache, void* v_cache,
+                      const int64_t* slots, const int32_t* positions, const float* cos, const float* sin,
+                      uint32_t table_rows, float rope_theta, const void* q, void* q_out, void* stream);
+
+/* Bytes of device scratch fa_paged_forward needs (0 for invalid parameters). */
+size_t fa_paged_workspace_size(const fa_paged_params* p);
+
+/* Attention of packed query tokens over a paged cache.
+ *   q, o         [total_q, num_heads_q, head_dim]
+ *   cu_seqlens_q [batch + 1]: request i has query rows [cu[i], cu[i+1]);
+ *                NULL: row i is request i's only token
+ *   seq_lens     [batch]: request i's keys in the cache, the new tokens' own
+ *                included
+ *   prefix_table pages of prefix_len keys that stand in front of every
+ *                request's own keys (NULL when prefix_len is 0)
+ *   lse          optional [num_heads_q, total_q] float32, natural log
+ * Query token j of the n of request i has position
+ * prefix_len + seq_lens[i] - n + j, its keys the positions 0, 1, ...: the new
+ * tokens are the last ones of their sequence, so is_causal is the mask of a
+ * prompt chunk and changes nothing for a single token. Rows that see no key
+ * get O = 0 and LSE = -inf; rows behind the last sequence are left as they
+ * were. Slots no query of the request sees (behind its end, before its
+ * window) are not read into the result whatever they hold.
+ * workspace: device scratch of fa_paged_workspace_size bytes, 256-byte
+ * aligned; calls that may overlap on the GPU need one each. */
+fa_status fa_paged_forward(const fa_paged_params* p, const void* q, const void* k_cache, const void* v_cache,
+                           const int32_t* block_table, const int32_t* seq_lens, const int32_t* cu_seqlens_q,
+                           const int32_t* prefix_table, void* o, float* lse, void* workspace,
+                           size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
