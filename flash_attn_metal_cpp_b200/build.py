@@ -43,8 +43,11 @@ CU_SOURCES = [
     "fa_paged_api.cu",
     "fa_paged_cache.cu",
     "fa_paged_simt.cu",
+    "fa_paged_decode_f16.cu",
+    "fa_paged_decode_bf16.cu",
 ]
-HEADERS = ["fa_internal.h", "fa_ptx.cuh", "fa_fwd_sm100.cuh", "fa_host.h", "fa_paged.h", "fa_paged.cuh"]
+HEADERS = ["fa_internal.h", "fa_ptx.cuh", "fa_fwd_sm100.cuh", "fa_host.h", "fa_paged.h", "fa_paged.cuh",
+           "fa_paged_decode.cuh"]
 
 
 def _mtime(path: str) -> float:

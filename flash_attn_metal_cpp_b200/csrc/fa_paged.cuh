@@ -196,6 +196,18 @@ __device__ __forceinline__ void store_out4(void* base, int64_t idx, int out_dtyp
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.69314718055994531f;
 
+// tanh for the score cap of the tensor-core kernels: the odd series up to y^9
+// below 1/4 (its next term is under 2^-26 of the value there), else
+// 1 - 2 / (1 + e^(2y)) with hardware exponential and division. Relative error
+// below 2^-19, so the cap may be of any size.
+__device__ __forceinline__ float cap_tanh(float y) {
+  const float y2 = y * y;
+  const float series =
+      y * fmaf(y2, fmaf(y2, fmaf(y2, fmaf(y2, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
+  const float quot = 1.f - __fdividef(2.f, 1.f + ex2_approx(y * (2.f * kLog2e)));
+  return fabsf(y) < 0.25f ? series : quot;
+}
+
 // Columns [col, col + 4) of a finished row (token, head): x holds
 // sum exp2(s - m) v and l the sum of exp2(s - m), both over the row's keys
 // (m in log2 units, -inf for no key). Joins the call's partial results (a

@@ -107,6 +107,7 @@ struct PagedArgs {
   int split;
   int n_ctas;
   int rows_per_unit;
+  int join_rows;           // most rows a unit can have here (for the join's grid)
   float* slot_o;           // [n_ctas, 2, rows_per_unit, D] unnormalised
   float2* slot_ml;         // [n_ctas, 2, rows_per_unit] running max (log2 units) and sum
   struct RunMeta* meta;    // [n_ctas]
@@ -133,6 +134,10 @@ struct RunMeta {
 int simt_rows_per_unit(int dtype, bool vec, int D, long long rows);
 int simt_ctas(int D);
 cudaError_t launch_paged_simt(const PagedArgs& a, int dtype, bool vec, cudaStream_t stream);
+// Tensor-core kernel for few rows (16-bit, rows of 16-byte pieces).
+int decode_rows_per_unit(int D, long long rows);
+int decode_ctas(int D, int rows_per_unit);
+cudaError_t launch_paged_decode(const PagedArgs& a, int dtype, cudaStream_t stream);
 // Join of the runs' partial units.
 cudaError_t launch_paged_join(const PagedArgs& a, cudaStream_t stream);
 

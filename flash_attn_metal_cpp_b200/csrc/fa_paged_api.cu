@@ -252,6 +252,9 @@ size_t fa_paged_workspace_size(const fa_paged_params* p) {
   const PagedArgs& a = c.a;
   // Whatever the tensors' base addresses allow: the largest of the kernels'.
   size_t ws = cut_layout(simt_ctas(a.D), c.dtype == kF32 ? (a.D <= 128 ? 4 : 2) : 1, a.D).bytes;
+  if (c.dtype != kF32 && c.vec) {
+    for (int rows : {16, 32}) ws = std::max(ws, cut_layout(decode_ctas(a.D, rows), rows, a.D).bytes);
+  }
   return ws;
 }
 
@@ -288,9 +291,18 @@ fa_status fa_paged_forward(const fa_paged_params* p, const void* q, const void* 
   const long long rows = max_rows(p, a, cu_seqlens_q == nullptr);
   const long long keys = (long long)a.pre + (long long)a.max_pages * a.page_size;
 
-  // CUDA cores.
-  a.rows_per_unit = simt_rows_per_unit(c.dtype, vec, a.D, rows);
-  a.n_ctas = simt_ctas(a.D);
+  // 16-bit rows of whole 16-byte pieces go to the tensor cores; fp32 and
+  // everything that cannot be copied in such pieces to the CUDA cores.
+  const bool tensor = c.dtype != kF32 && vec && a.num_pages > 0;
+  if (tensor) {
+    a.rows_per_unit = decode_rows_per_unit(a.D, rows);
+    a.n_ctas = decode_ctas(a.D, a.rows_per_unit);
+  } else {
+    a.rows_per_unit = simt_rows_per_unit(c.dtype, vec, a.D, rows);
+    a.n_ctas = simt_ctas(a.D);
+  }
+  const long long most = (cu_seqlens_q ? (long long)a.total_q : 1ll) * a.group;
+  a.join_rows = (int)std::min<long long>(a.rows_per_unit, most);
   a.split = keys > 256;
   if (!a.split) {
     const long long chunks = cu_seqlens_q ? ((long long)a.total_q * a.group) / a.rows_per_unit + a.B
@@ -298,7 +310,8 @@ fa_status fa_paged_forward(const fa_paged_params* p, const void* q, const void* 
     a.n_ctas = (int)std::min<long long>(chunks * a.Hk, 148 * 16);
   }
   place_cut(a, cut_layout(a.n_ctas, a.rows_per_unit, a.D), workspace);
-  st = cuda_status(launch_paged_simt(a, c.dtype, vec, s), "paged attention (CUDA cores)");
+  st = tensor ? cuda_status(launch_paged_decode(a, c.dtype, s), "paged attention (few rows)")
+              : cuda_status(launch_paged_simt(a, c.dtype, vec, s), "paged attention (CUDA cores)");
   if (st == FA_OK && a.split) st = cuda_status(launch_paged_join(a, s), "paged attention (join)");
   return st;
 }

@@ -328,7 +328,7 @@ cudaError_t launch_paged_simt(const PagedArgs& a, int dtype, bool vec, cudaStrea
 
 cudaError_t launch_paged_join(const PagedArgs& a, cudaStream_t st) {
   if (a.n_ctas < 2) return cudaSuccess;
-  cudaError_t e = launch_pdl(paged_join_kernel, dim3((unsigned)(a.n_ctas - 1), (unsigned)a.rows_per_unit),
+  cudaError_t e = launch_pdl(paged_join_kernel, dim3((unsigned)(a.n_ctas - 1), (unsigned)a.join_rows),
                              dim3(kJoinWarps * 32), 0, st, a);
   note_launch();
   return e;
