@@ -45,9 +45,13 @@ CU_SOURCES = [
     "fa_paged_simt.cu",
     "fa_paged_decode_f16.cu",
     "fa_paged_decode_bf16.cu",
+    "fa_paged_sm100_d64_f16.cu",
+    "fa_paged_sm100_d64_bf16.cu",
+    "fa_paged_sm100_d128_f16.cu",
+    "fa_paged_sm100_d128_bf16.cu",
 ]
 HEADERS = ["fa_internal.h", "fa_ptx.cuh", "fa_fwd_sm100.cuh", "fa_host.h", "fa_paged.h", "fa_paged.cuh",
-           "fa_paged_decode.cuh"]
+           "fa_paged_decode.cuh", "fa_paged_sm100.cuh"]
 
 
 def _mtime(path: str) -> float:

@@ -138,6 +138,24 @@ cudaError_t launch_paged_simt(const PagedArgs& a, int dtype, bool vec, cudaStrea
 int decode_rows_per_unit(int D, long long rows);
 int decode_ctas(int D, int rows_per_unit);
 cudaError_t launch_paged_decode(const PagedArgs& a, int dtype, cudaStream_t stream);
+// Tensor-core kernel for many rows (16-bit, head_dim <= 128, pages of 8 slots
+// or more): what it needs besides PagedArgs.
+struct PagedTc {
+  int shared;        // 1: the rows of all requests against the prefix
+  int n_blocks;      // blocks of 256 packed rows (an upper bound)
+  int n_split;       // parts the keys of a block are cut in
+  int box_rows;      // slots of one TMA box
+  int partial;       // 1: normalised partial results to part0 + split
+  int part0;
+  float* parts_o;    // [parts, total_q, Hq, D]
+  float* parts_lse;  // [parts, Hq, total_q]
+};
+cudaError_t launch_paged_tc_d64_f16(const PagedArgs&, const PagedTc&, const CUtensorMap&, const CUtensorMap&, cudaStream_t);
+cudaError_t launch_paged_tc_d64_bf16(const PagedArgs&, const PagedTc&, const CUtensorMap&, const CUtensorMap&, cudaStream_t);
+cudaError_t launch_paged_tc_d128_f16(const PagedArgs&, const PagedTc&, const CUtensorMap&, const CUtensorMap&, cudaStream_t);
+cudaError_t launch_paged_tc_d128_bf16(const PagedArgs&, const PagedTc&, const CUtensorMap&, const CUtensorMap&, cudaStream_t);
+// Join of whole-row partial results (PagedArgs::parts_*) into o and lse.
+cudaError_t launch_paged_merge(const PagedArgs& a, cudaStream_t stream);
 // Join of the runs' partial units.
 cudaError_t launch_paged_join(const PagedArgs& a, cudaStream_t stream);
 

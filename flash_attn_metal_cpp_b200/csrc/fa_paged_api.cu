@@ -42,6 +42,8 @@ fa_status check(const fa_paged_params* p, Checked* c, bool grouped = true) {
   if (p->batch_size > lim || p->total_q > lim || p->page_size > lim || p->num_pages > lim || p->max_pages > lim ||
       p->prefix_pages > lim)
     return paged_fail(FA_ERR_INVALID_ARG, "tensor dimensions out of range");
+  if (grouped && (uint64_t)p->total_q * p->num_heads_q > lim)
+    return paged_fail(FA_ERR_INVALID_ARG, "total_q * num_heads_q must not exceed 2^30");
   if (p->prefix_len > lim / 2 || (uint64_t)p->prefix_len > (uint64_t)p->prefix_pages * p->page_size)
     return paged_fail(FA_ERR_INVALID_ARG, "prefix_len is beyond the pages of the prefix table");
   if (!std::isfinite(p->softmax_scale)) return paged_fail(FA_ERR_INVALID_ARG, "softmax_scale must be finite");
@@ -123,6 +125,108 @@ void place_cut(PagedArgs& a, const CutLayout& l, void* ws) {
   a.meta = reinterpret_cast<RunMeta*>(w);
   a.slot_ml = reinterpret_cast<float2*>(w + l.ml);
   a.slot_o = reinterpret_cast<float*>(w + l.o);
+}
+
+// Which kernels a call takes, and its scratch.
+struct Choice {
+  bool tensor;     // few-rows tensor-core kernel, else CUDA cores
+  bool many;       // the requests' own keys go to the many-rows kernel
+  bool shared;     // the prefix is computed once for all rows (many-rows kernel)
+  int box;         // slots of a TMA box
+  int own_split, pre_split;        // parts the keys are cut in
+  int own_blocks, pre_blocks;      // blocks of 256 packed rows
+  int rows_per_unit, n_ctas, join_rows, split;
+  CutLayout cut;
+  size_t parts_lse, parts_o, bytes;  // offsets of the partial results
+};
+
+// Parts that the keys of `blocks` blocks (256 rows, up to `tiles` tiles of
+// 128 keys) are cut in. A wave of 148 blocks takes one tile in about 2.1 us
+// (D = 128), a block about 2 tiles more to begin and end; every part writes
+// and reads its partial rows once (about 5 TB/s). One part needs no join.
+int choose_parts(long long blocks, long long tiles, int D, double row_bytes, bool join_anyway) {
+  const double tile = D <= 64 ? 1.3e-6 : 2.1e-6;
+  const int top = (int)std::max(1ll, std::min(32ll, tiles / 2));
+  int best = 1;
+  double best_cost = 0;
+  for (int n = 1; n <= top; ++n) {
+    const double waves = (double)((blocks * n + 147) / 148);
+    double cost = waves * (double)((tiles + n - 1) / n + 2) * tile;
+    if (n > 1 || join_anyway) cost += 2.0 * n * row_bytes / 5e12;
+    if (n > 1 && !join_anyway) cost += 3e-6;  // the join's own launch
+    if (n == 1 || cost < best_cost) {
+      best = n;
+      best_cost = cost;
+    }
+  }
+  return best;
+}
+
+int gcd(int a, int b) {
+  while (b) {
+    const int t = a % b;
+    a = b;
+    b = t;
+  }
+  return a;
+}
+
+// `one`: one query token a request (no cu_seqlens_q).
+Choice choose(const fa_paged_params* p, const Checked& c, bool vec, bool one) {
+  const PagedArgs& a = c.a;
+  Choice h{};
+  const long long rows = max_rows(p, a, one);
+  const long long all_rows = (long long)a.total_q * a.group;
+  const long long own_keys = (long long)a.max_pages * a.page_size;
+  // 16-bit rows of whole 16-byte pieces go to the tensor cores; fp32 and
+  // everything that cannot be copied in such pieces to the CUDA cores.
+  h.tensor = c.dtype != kF32 && vec && a.num_pages > 0;
+  h.box = gcd(a.page_size, 128);
+  const bool tma = h.tensor && a.D <= 128 && h.box >= 8 && a.k_sp > 0 && a.k_ss > 0 && a.k_sh > 0 && a.v_sp > 0 &&
+                   a.v_ss > 0 && a.v_sh > 0;
+  h.many = tma && rows > 32;
+  h.shared = tma && a.pre > 0 &&
+             (h.many || (a.pre >= 256 && (double)a.B * a.pre * a.Hk * a.D * 4 >= 16e6));
+  const double row_bytes = (double)a.total_q * a.Hq * a.D * 4;
+  if (h.shared) {
+    h.pre_blocks = (int)((all_rows + 255) / 256);
+    h.pre_split = choose_parts((long long)h.pre_blocks * a.Hk, (a.pre + 127) / 128, a.D, row_bytes, true);
+  }
+  if (h.many) {
+    h.own_blocks = (int)(one ? (long long)a.B * ((a.group + 255) / 256) : (all_rows + 255) / 256 + a.B);
+    h.own_split = choose_parts((long long)h.own_blocks * a.Hk, (own_keys + 127) / 128, a.D, row_bytes, h.shared);
+  }
+  if (!h.many) {
+    if (h.tensor) {
+      h.rows_per_unit = decode_rows_per_unit(a.D, rows);
+      h.n_ctas = decode_ctas(a.D, h.rows_per_unit);
+    } else {
+      h.rows_per_unit = simt_rows_per_unit(c.dtype, vec, a.D, rows);
+      h.n_ctas = simt_ctas(a.D);
+    }
+    h.join_rows = (int)std::min<long long>(h.rows_per_unit, one ? (long long)a.group : all_rows);
+    const long long keys = own_keys + (h.shared ? 0 : a.pre);
+    h.split = keys > 256;
+    if (!h.split) {
+      const long long chunks = one ? (long long)a.B * ((a.group + h.rows_per_unit - 1) / h.rows_per_unit)
+                                   : all_rows / h.rows_per_unit + a.B;
+      h.n_ctas = (int)std::min<long long>(chunks * a.Hk, 148 * 16);
+    }
+    h.cut = cut_layout(h.n_ctas, h.rows_per_unit, a.D);
+    h.bytes = h.cut.bytes;
+  }
+  const size_t parts = (size_t)h.pre_split + ((h.many && (h.shared || h.own_split > 1)) ? h.own_split : 0);
+  h.parts_lse = h.bytes;
+  h.parts_o = h.parts_lse + up256(parts * a.Hq * a.total_q * sizeof(float));
+  h.bytes = h.parts_o + up256(parts * (size_t)a.total_q * a.Hq * a.D * sizeof(float));
+  return h;
+}
+
+cudaError_t launch_tc(const PagedArgs& a, const PagedTc& t, int dtype, const CUtensorMap& tk, const CUtensorMap& tv,
+                      cudaStream_t s) {
+  if (a.D <= 64)
+    return dtype == kF16 ? launch_paged_tc_d64_f16(a, t, tk, tv, s) : launch_paged_tc_d64_bf16(a, t, tk, tv, s);
+  return dtype == kF16 ? launch_paged_tc_d128_f16(a, t, tk, tv, s) : launch_paged_tc_d128_bf16(a, t, tk, tv, s);
 }
 
 }  // namespace
@@ -250,10 +354,11 @@ size_t fa_paged_workspace_size(const fa_paged_params* p) {
   Checked c;
   if (check(p, &c) != FA_OK) return 0;
   const PagedArgs& a = c.a;
-  // Whatever the tensors' base addresses allow: the largest of the kernels'.
-  size_t ws = cut_layout(simt_ctas(a.D), c.dtype == kF32 ? (a.D <= 128 ? 4 : 2) : 1, a.D).bytes;
-  if (c.dtype != kF32 && c.vec) {
-    for (int rows : {16, 32}) ws = std::max(ws, cut_layout(decode_ctas(a.D, rows), rows, a.D).bytes);
+  // Whatever the tensors' base addresses and cu_seqlens_q turn out to be.
+  size_t ws = 0;
+  for (int i = 0; i < 4; ++i) {
+    if ((i & 1) && !c.vec) continue;
+    ws = std::max(ws, choose(p, c, (i & 1) != 0, (i & 2) != 0).bytes);
   }
   return ws;
 }
@@ -288,30 +393,55 @@ fa_status fa_paged_forward(const fa_paged_params* p, const void* q, const void* 
   a.lse = lse;
   a.wait_limit_ns = paged_wait_limit_ns();
   const bool vec = c.vec && aligned(q, 16) && aligned(k_cache, 16) && aligned(v_cache, 16);
-  const long long rows = max_rows(p, a, cu_seqlens_q == nullptr);
-  const long long keys = (long long)a.pre + (long long)a.max_pages * a.page_size;
-
-  // 16-bit rows of whole 16-byte pieces go to the tensor cores; fp32 and
-  // everything that cannot be copied in such pieces to the CUDA cores.
-  const bool tensor = c.dtype != kF32 && vec && a.num_pages > 0;
-  if (tensor) {
-    a.rows_per_unit = decode_rows_per_unit(a.D, rows);
-    a.n_ctas = decode_ctas(a.D, a.rows_per_unit);
-  } else {
-    a.rows_per_unit = simt_rows_per_unit(c.dtype, vec, a.D, rows);
-    a.n_ctas = simt_ctas(a.D);
+  const Choice h = choose(p, c, vec, cu_seqlens_q == nullptr);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  float* parts_lse = reinterpret_cast<float*>(ws + h.parts_lse);
+  float* parts_o = reinterpret_cast<float*>(ws + h.parts_o);
+  CUtensorMap tk, tv;
+  PagedTc t{};
+  t.box_rows = h.box;
+  t.parts_o = parts_o;
+  t.parts_lse = parts_lse;
+  if (h.shared || h.many) {
+    const bool bf = c.dtype == kBF16;
+    st = paged_encode(&tk, k_cache, bf, a.D, a.Hk, a.page_size, a.num_pages, a.k_sp, a.k_ss, a.k_sh, h.box);
+    if (st == FA_OK)
+      st = paged_encode(&tv, v_cache, bf, a.D, a.Hk, a.page_size, a.num_pages, a.v_sp, a.v_ss, a.v_sh, h.box);
+    if (st != FA_OK) return st;
   }
-  const long long most = (cu_seqlens_q ? (long long)a.total_q : 1ll) * a.group;
-  a.join_rows = (int)std::min<long long>(a.rows_per_unit, most);
-  a.split = keys > 256;
-  if (!a.split) {
-    const long long chunks = cu_seqlens_q ? ((long long)a.total_q * a.group) / a.rows_per_unit + a.B
-                                          : (long long)a.B * ((a.group + a.rows_per_unit - 1) / a.rows_per_unit);
-    a.n_ctas = (int)std::min<long long>(chunks * a.Hk, 148 * 16);
+  if (h.shared) {
+    t.shared = 1;
+    t.n_blocks = h.pre_blocks;
+    t.n_split = h.pre_split;
+    t.partial = 1;
+    st = cuda_status(launch_tc(a, t, c.dtype, tk, tv, s), "shared prefix attention");
+    if (st != FA_OK) return st;
+    a.pre = 0;  // what follows sees each request's own keys
+    a.pre_table = nullptr;
+    a.n_parts = h.pre_split;
+    a.parts_o = parts_o;
+    a.parts_lse = parts_lse;
   }
-  place_cut(a, cut_layout(a.n_ctas, a.rows_per_unit, a.D), workspace);
-  st = tensor ? cuda_status(launch_paged_decode(a, c.dtype, s), "paged attention (few rows)")
-              : cuda_status(launch_paged_simt(a, c.dtype, vec, s), "paged attention (CUDA cores)");
+  if (h.many) {
+    t.shared = 0;
+    t.n_blocks = h.own_blocks;
+    t.n_split = h.own_split;
+    t.partial = h.shared || h.own_split > 1;
+    t.part0 = a.n_parts;
+    st = cuda_status(launch_tc(a, t, c.dtype, tk, tv, s), "paged attention (many rows)");
+    if (st != FA_OK || !t.partial) return st;
+    a.n_parts += h.own_split;
+    a.parts_o = parts_o;
+    a.parts_lse = parts_lse;
+    return cuda_status(launch_paged_merge(a, s), "paged attention (merge)");
+  }
+  a.rows_per_unit = h.rows_per_unit;
+  a.n_ctas = h.n_ctas;
+  a.join_rows = h.join_rows;
+  a.split = h.split;
+  place_cut(a, h.cut, workspace);
+  st = h.tensor ? cuda_status(launch_paged_decode(a, c.dtype, s), "paged attention (few rows)")
+                : cuda_status(launch_paged_simt(a, c.dtype, vec, s), "paged attention (CUDA cores)");
   if (st == FA_OK && a.split) st = cuda_status(launch_paged_join(a, s), "paged attention (join)");
   return st;
 }

@@ -285,6 +285,20 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const Paged
   finish_row4(a, mt.q0 + row / a.group, mt.hk * a.group + row % a.group, col, x, top, ls);
 }
 
+// Rows whose every part is a whole-row partial result: one warp a row.
+__global__ void __launch_bounds__(256) paged_merge_kernel(const PagedArgs a) {
+  grid_dep_wait();
+  grid_dep_launch_dependents();
+  const int last = a.cu_q ? min(max(a.cu_q[a.B], 0), a.total_q) : min(a.B, a.total_q);
+  const long long r = blockIdx.x * 8ll + (threadIdx.x >> 5);
+  const int tok = (int)(r / a.Hq), head = (int)(r - (long long)tok * a.Hq);
+  if (tok >= last) return;  // rows behind the last sequence
+  for (int col = (threadIdx.x & 31) * 4; col < a.D; col += 128) {
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    finish_row4(a, tok, head, col, x, -INFINITY, 0.f);
+  }
+}
+
 template <typename T, int DM, int R, bool VEC>
 cudaError_t launch_one(const PagedArgs& a, cudaStream_t st) {
   cudaError_t e = launch_pdl(paged_simt_kernel<T, DM, R, VEC>, dim3((unsigned)a.n_ctas), dim3(kThreads), 0, st, a);
@@ -324,6 +338,14 @@ cudaError_t launch_paged_simt(const PagedArgs& a, int dtype, bool vec, cudaStrea
     case kBF16: return launch_dm<__nv_bfloat16, false>(a, st);
     default: return vec ? launch_dm<float, true>(a, st) : launch_dm<float, false>(a, st);
   }
+}
+
+cudaError_t launch_paged_merge(const PagedArgs& a, cudaStream_t st) {
+  const long long blocks = ((long long)a.total_q * a.Hq + 7) / 8;
+  if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
+  cudaError_t e = launch_pdl(paged_merge_kernel, dim3((unsigned)blocks), dim3(256), 0, st, a);
+  note_launch();
+  return e;
 }
 
 cudaError_t launch_paged_join(const PagedArgs& a, cudaStream_t st) {

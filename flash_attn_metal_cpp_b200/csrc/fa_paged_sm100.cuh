@@ -1,0 +1,655 @@
+// fa_paged_sm100.cuh - attention of many query rows over a paged cache
+// (fp16 / bf16) on the 5th-generation tensor cores: prompt chunks, runs of
+// tokens to verify, and the shared prefix of a batch, whose keys meet the
+// query rows of all requests at once.
+//
+// The rows that read the same keys are packed: row r = token * group + head
+// of the group, so a KV head's whole group (and, for a shared prefix, the
+// whole batch) fills the 128 rows of an MMA. One block takes 256 packed rows
+// (two tiles) of one KV head and a range of the keys. The mapping on the SM
+// is that of the contiguous kernel (fa_fwd_sm100.cuh): two softmax
+// warpgroups, one per tile, that ping-pong with one MMA thread; S and P in
+// TMEM, O in TMEM, lazily rescaled. What differs:
+//   * K and V come page by page: a tile of 128 keys is up to 16 TMA boxes of
+//     gcd(page_size, 128) slots by 64 columns, each sent by its own lane of
+//     the producer warp, which looked its page up one tile earlier.
+//   * Slots outside the visible range hold anything, NaN included. Scores of
+//     such keys are masked by selection; their V rows (0 * NaN is NaN) are
+//     zeroed by the V producer after its copies landed and before the MMA
+//     thread is told: only edge tiles pay for that.
+//   * Q rows are gathered by the softmax threads (one row each) into the
+//     swizzled layout the MMA reads, so any packing and stride is fine.
+//   * P has V's type (one MMA takes one type): rounded to bf16 or fp16, half
+//     a step of 2^-8 or 2^-11 of each weight; everything else is fp32.
+//   * Columns beyond head_dim (below 64 or 128) are zero-filled by the TMA.
+// What bounds it: the tensor cores and the exponentials together, like the
+// contiguous kernel; K and V are read from L2 by the blocks of one KV head.
+#pragma once
+
+#include "fa_paged.cuh"
+
+#include <type_traits>
+
+namespace fa {
+namespace paged_tc {
+
+constexpr int BM = 128, NT = 2, BN = 128;
+constexpr int kThreads = 384;
+constexpr int kKWarp = 8, kMmaWarp = 9, kVWarp = 10;
+// As in fa_fwd_sm100.cuh: 384 x 168 registers at launch = 2 x 128 x 216 + 128 x 72.
+constexpr uint32_t kRegsLaunch = 168, kRegsSoftmax = 216, kRegsOther = 72;
+static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsOther <= kThreads * kRegsLaunch, "register split exceeds launch");
+constexpr uint32_t kTmemCols = 512, kColS = 0, kColO = 256;
+constexpr float kRescaleThreshold = 8.0f;
+
+template <int D>
+struct Cfg {
+  static constexpr int NBOX = D / 64;
+  static constexpr int BOX_BYTES = 128 * 128;
+  static constexpr int TILE_BYTES = NBOX * BOX_BYTES;
+  static constexpr int NS = (D == 128) ? 2 : 4;
+  static constexpr int OFF_Q = 0;
+  static constexpr int OFF_K = NT * TILE_BYTES;
+  static constexpr int OFF_V = OFF_K + NS * TILE_BYTES;
+  static constexpr int OFF_BAR = OFF_V + NS * TILE_BYTES;
+  static constexpr int SMEM_BYTES = OFF_BAR + 1024 + 1024;  // barriers and scratch, alignment slack
+};
+
+struct Bars {
+  uint64_t q_full[NT], s_full[NT], p_full[NT][2], o_full[NT];
+  uint64_t mma_final, v_raw;
+  uint64_t k_full[4], v_full[4], k_empty[4], v_empty[4];
+  uint32_t tmem_base;
+  int abort_flag;
+  // block search
+  int part[kThreads / 32];
+  int req, blk, min_ahead;
+};
+static_assert(sizeof(Bars) <= 1024, "barrier space");
+
+// Which rows and keys the block works on.
+struct Block {
+  int q0, qlen, klen;   // query tokens and keys of its request (shared prefix: all tokens, the prefix)
+  int req;
+  int row0, rows;       // packed rows [row0, min(row0 + 256, rows))
+};
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack_p(float lo, float hi) {
+  if constexpr (std::is_same<T, __half>::value) return pack_half2(lo, hi);
+  else return pack_bf162(lo, hi);
+}
+
+// Sum of one int per thread before the calling thread (and the total).
+__device__ __forceinline__ int scan_block(int x, int* part, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int inc = x;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, inc, off);
+    if (lane >= off) inc += y;
+  }
+  if (lane == 31) part[warp] = inc;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += part[w];
+    all += part[w];
+  }
+  *total = all;
+  return before + inc - x;
+}
+
+// XF: what a score goes through before the softmax. 0: scale alone (positive);
+// 1: any scale, ALiBi; 2: the tanh cap, any scale, ALiBi.
+template <int D, typename T, int XF>
+__global__ void __launch_bounds__(kThreads, 1)
+    paged_attn_sm100(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                     const PagedArgs a, const PagedTc tc) {
+  using C = Cfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Bars* bars = reinterpret_cast<Bars*>(smem + C::OFF_BAR);
+  const uint32_t sQ = smem_addr(smem + C::OFF_Q), sK = smem_addr(smem + C::OFF_K), sV = smem_addr(smem + C::OFF_V);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const unsigned long long wlim = a.wait_limit_ns ? a.wait_limit_ns : kWaitLimitNs;
+
+  grid_dep_wait();
+  grid_dep_launch_dependents();
+
+  // ------------------------------------------------------------ work item
+  // Blocks of a request's rows stand in one line over the requests, the last
+  // ones first (under a causal mask they have the most keys); within a block
+  // the KV heads, within a head the parts of the keys.
+  const int split = blockIdx.x % tc.n_split;
+  const int hk = blockIdx.x / tc.n_split % a.Hk;
+  const int bi = blockIdx.x / tc.n_split / a.Hk;
+  Block b;
+  if (tc.shared) {
+    const int last = a.cu_q ? min(max(a.cu_q[a.B], 0), a.total_q) : min(a.B, a.total_q);
+    b.req = -1;
+    b.q0 = 0;
+    b.qlen = last;
+    b.klen = a.pre;
+    b.rows = last * a.group;
+    b.row0 = bi * NT * BM;
+    if (b.row0 >= b.rows) return;
+    if (a.win_left >= 0) {
+      // The window may leave most of the prefix unseen: the earliest query of
+      // the batch says how much.
+      int ahead = 0x7fffffff;
+      for (int i = threadIdx.x; i < a.B; i += kThreads) {
+        const ReqView v = view_request<BN>(a, i, BM);
+        if (v.qlen > 0) ahead = min(ahead, v.klen - v.qlen);
+      }
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) ahead = min(ahead, __shfl_xor_sync(0xffffffffu, ahead, off));
+      if (lane == 0) bars->part[warp] = ahead;
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        for (int w = 1; w < kThreads / 32; ++w) ahead = min(ahead, bars->part[w]);
+        bars->min_ahead = ahead;
+      }
+    }
+  } else {
+    const int seg = (a.B + kThreads - 1) / kThreads;
+    const int i0 = min((int)threadIdx.x * seg, a.B), i1 = min(i0 + seg, a.B);
+    int n = 0;
+    for (int i = i0; i < i1; ++i)
+      n += (int)(((long long)view_request<BN>(a, i, BM).qlen * a.group + NT * BM - 1) / (NT * BM));
+    if (threadIdx.x == 0) bars->req = -1;
+    int total;
+    int at = scan_block(n, bars->part, &total);
+    const int want = total - 1 - bi;
+    if (want < 0) return;
+    if (want >= at && want < at + n) {
+      for (int i = i0; i < i1; ++i) {
+        const int nb = (int)(((long long)view_request<BN>(a, i, BM).qlen * a.group + NT * BM - 1) / (NT * BM));
+        if (want < at + nb) {
+          bars->req = i;
+          bars->blk = want - at;
+          break;
+        }
+        at += nb;
+      }
+    }
+    __syncthreads();
+    b.req = bars->req;
+    const ReqView v = view_request<BN>(a, b.req, BM);
+    b.q0 = v.q0;
+    b.qlen = v.qlen;
+    b.klen = v.klen;
+    b.rows = v.qlen * a.group;
+    b.row0 = bars->blk * NT * BM;
+  }
+
+  if (threadIdx.x == kKWarp * 32) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      mbar_init(smem_addr(&bars->q_full[t]), 4);
+      mbar_init(smem_addr(&bars->s_full[t]), 1);
+      mbar_init(smem_addr(&bars->p_full[t][0]), 4);
+      mbar_init(smem_addr(&bars->p_full[t][1]), 4);
+      mbar_init(smem_addr(&bars->o_full[t]), 1);
+    }
+    mbar_init(smem_addr(&bars->mma_final), 1);
+    mbar_init(smem_addr(&bars->v_raw), 1);
+    for (int s = 0; s < C::NS; ++s) {
+      mbar_init(smem_addr(&bars->k_full[s]), 1);
+      mbar_init(smem_addr(&bars->v_full[s]), 1);
+      mbar_init(smem_addr(&bars->k_empty[s]), 1);
+      mbar_init(smem_addr(&bars->v_empty[s]), 1);
+    }
+    bars->abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(smem_addr(&bars->tmem_base), kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+  volatile int* abort_flag = &bars->abort_flag;
+
+  // Key tiles of each row tile (absolute, in tiles of 128 keys), then the
+  // part of them that this split takes. All threads compute the same.
+  int lo_t[NT], hi_t[NT];
+  int k_lo = 0x7fffffff, k_hi = 0;   // keys any row of the block sees
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int r0 = b.row0 + t * BM;
+    int lo = 0, hi = 0;
+    if (r0 < b.rows) {
+      hi = b.klen;
+      if (tc.shared) {
+        if (a.win_left >= 0) lo = (int)max(0ll, (long long)bars->min_ahead - a.win_left);
+      } else {
+        const int r1 = min(r0 + BM, b.rows) - 1;
+        const int p0 = b.klen - b.qlen + r0 / a.group, p1 = b.klen - b.qlen + r1 / a.group;
+        lo = visible_keys(a, b.klen, p0).x;
+        hi = visible_keys(a, b.klen, p1).y;
+      }
+      if (lo >= hi) lo = hi = 0;
+      else {
+        k_lo = min(k_lo, lo);
+        k_hi = max(k_hi, hi);
+      }
+    }
+    lo_t[t] = lo / BN;
+    hi_t[t] = (hi + BN - 1) / BN;
+  }
+  int j_min = 0, n_kv = 0, s_lo[NT], n_kv_t[NT];
+  {
+    int first = 0, last = 0;
+    if (k_hi > k_lo) {
+      const int t0 = k_lo / BN, n = (k_hi + BN - 1) / BN - t0;
+      first = t0 + (int)((long long)n * split / tc.n_split);
+      last = t0 + (int)((long long)n * (split + 1) / tc.n_split);
+    }
+    j_min = first;
+    n_kv = 0;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int lo = max(lo_t[t], first), hi = min(hi_t[t], last);
+      s_lo[t] = lo - first;
+      n_kv_t[t] = max(0, hi - lo);
+      if (n_kv_t[t] > 0) n_kv = max(n_kv, hi - first);
+    }
+  }
+
+  if (warp >= 8) {
+    reg_alloc_dec<kRegsOther>();
+    if ((warp == kKWarp || warp == kVWarp) && n_kv > 0) {
+      // ------------------------------------------------------ producers
+      const bool is_k = warp == kKWarp;
+      const CUtensorMap* tm = is_k ? &tm_k : &tm_v;
+      const uint32_t ring = is_k ? sK : sV;
+      uint64_t* full = is_k ? bars->k_full : bars->v_full;
+      uint64_t* empty = is_k ? bars->k_empty : bars->v_empty;
+      const uint32_t raw = smem_addr(&bars->v_raw);
+      if (lane == 0) prefetch_tmap(tm);
+      const int box = tc.box_rows, boxes = BN / box;
+      const int* table = tc.shared ? a.pre_table : a.table + (int64_t)b.req * a.table_stride;
+      // Page of this lane's box in tile j (-1: nothing to load).
+      auto look_up = [&](int j) {
+        const int key = (j_min + j) * BN + lane * box;
+        if (lane >= boxes || j >= n_kv || key >= k_hi || key + box <= k_lo) return -1;
+        const int page = table[key / a.page_size];
+        if ((unsigned)page < (unsigned)a.num_pages) return page;
+        note_bad_index(a.status);
+        return -1;
+      };
+      int page = look_up(0), raw_phase = 0, issued = 0;
+      for (int j = 0; j < n_kv; ++j) {
+        const int st = j % C::NS;
+        bool ok = true;
+        if (lane == 0) {
+          ok = !*abort_flag && fa_wait(smem_addr(&empty[st]), ((j / C::NS) + 1) & 1, a.status, wlim);
+          if (!ok) *abort_flag = 1;
+        }
+        if (!__shfl_sync(0xffffffffu, (int)ok, 0)) break;
+        const int kv0 = (j_min + j) * BN;
+        const unsigned on = __ballot_sync(0xffffffffu, page >= 0);
+        const uint32_t bytes = (uint32_t)__popc(on) * box * 128 * C::NBOX;
+        // Edge tile: some of its rows are not of visible keys.
+        const bool edge = __popc(on) != boxes || kv0 < k_lo || kv0 + BN > k_hi;
+        const bool clean = !is_k && edge;
+        const uint32_t bfull = smem_addr(&full[st]);
+        const uint32_t bar = clean ? raw : bfull;
+        if (lane == 0) {
+          if (bytes) mbar_arrive_expect_tx(bar, bytes);
+          else mbar_arrive(bar);
+        }
+        __syncwarp();
+        if (page >= 0) {
+          const int slot = (kv0 + lane * box) % a.page_size;
+          const uint32_t dst = ring + st * C::TILE_BYTES + lane * box * 128;
+#pragma unroll
+          for (int bx = 0; bx < C::NBOX; ++bx)
+            tma_load_4d(dst + bx * C::BOX_BYTES, tm, bar, bx * 64, hk, slot, page);
+        }
+        __syncwarp();
+        page = look_up(j + 1);
+        if (clean) {
+          if (lane == 0) ok = fa_wait(raw, raw_phase, a.status, wlim);
+          if (!__shfl_sync(0xffffffffu, (int)ok, 0)) {
+            if (lane == 0) {
+              *abort_flag = 1;
+              fa_wait(raw, raw_phase, a.status, wlim);  // its copies are still on their way
+            }
+            break;
+          }
+          raw_phase ^= 1;
+          uint8_t* tile = smem + C::OFF_V + st * C::TILE_BYTES;
+          for (int e = lane; e < BN * 8; e += 32) {
+            const int row = e >> 3, key = kv0 + row;
+            if (key >= k_lo && key < k_hi && ((on >> (row / box)) & 1)) continue;
+#pragma unroll
+            for (int bx = 0; bx < C::NBOX; ++bx)
+              *reinterpret_cast<uint4*>(tile + bx * C::BOX_BYTES + e * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bfull);
+        }
+        issued = j + 1;
+      }
+      // Never leave the CTA with bulk copies still writing shared memory.
+      if (lane == 0)
+        for (int j = max(0, issued - C::NS); j < issued; ++j)
+          fa_wait(smem_addr(&full[j % C::NS]), (j / C::NS) & 1, a.status, wlim);
+    } else if (warp == kMmaWarp && lane == 0 && n_kv > 0) {
+      // ------------------------------------------------------ MMA issuer
+      constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+      constexpr uint32_t idesc_s = make_idesc(BM, BN, fmt, 0, 0);
+      constexpr uint32_t idesc_o = make_idesc(BM, D, fmt, 0, 1 /*V is MN-major*/);
+      const uint64_t qk_desc0 = smem_desc(smem_addr(smem), 16, 1024);
+      const uint64_t v_desc0 = smem_desc(sV, C::BOX_BYTES, 1024);
+      const uint32_t qk_lo0 = (uint32_t)qk_desc0, qk_hi = (uint32_t)(qk_desc0 >> 32);
+      const uint32_t v_lo0 = (uint32_t)v_desc0, v_hi = (uint32_t)(v_desc0 >> 32);
+      bool ok = true;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+        if (ok && n_kv_t[t] > 0) ok = fa_wait(smem_addr(&bars->q_full[t]), 0, a.status, wlim);
+      for (int j = 0; ok && j <= n_kv; ++j) {
+        if (*abort_flag) { ok = false; break; }
+        bool k_ready = false, v_ready = false;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const uint32_t tS = tmem + kColS + t * 128, tO = tmem + kColO + t * 128;
+          if (j >= 1 && j - 1 >= s_lo[t] && j - 1 < s_lo[t] + n_kv_t[t]) {
+            const int i = j - 1, it = i - s_lo[t];
+            if (!v_ready) {
+              if (!fa_wait(smem_addr(&bars->v_full[i % C::NS]), (i / C::NS) & 1, a.status, wlim)) { ok = false; break; }
+              v_ready = true;
+            }
+            const uint32_t v_lo = v_lo0 + (uint32_t)((i % C::NS) * C::TILE_BYTES >> 4);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              if (!fa_wait(smem_addr(&bars->p_full[t][half]), it & 1, a.status, wlim)) { ok = false; break; }
+              tc_fence_after();
+#pragma unroll
+              for (int kk = half * 4; kk < half * 4 + 4; ++kk)
+                mma_ts_lohi(tO, tS + kk * 8, v_lo + kk * (16 * 128 >> 4), v_hi, idesc_o, (it > 0 || kk > 0) ? 1u : 0u);
+            }
+            if (!ok) break;
+            if (it == n_kv_t[t] - 1) mma_commit(smem_addr(&bars->o_full[t]));
+          }
+          if (j >= s_lo[t] && j < s_lo[t] + n_kv_t[t]) {
+            if (!k_ready) {
+              if (!fa_wait(smem_addr(&bars->k_full[j % C::NS]), (j / C::NS) & 1, a.status, wlim)) { ok = false; break; }
+              k_ready = true;
+            }
+            tc_fence_after();
+            const uint32_t q_lo = qk_lo0 + (uint32_t)((C::OFF_Q + t * C::TILE_BYTES) >> 4);
+            const uint32_t k_lo_d = qk_lo0 + (uint32_t)((C::OFF_K + (j % C::NS) * C::TILE_BYTES) >> 4);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t off = ((kk >> 2) * C::BOX_BYTES + (kk & 3) * 32) >> 4;
+              mma_ss_lohi(tS, q_lo + off, qk_hi, k_lo_d + off, qk_hi, idesc_s, kk > 0 ? 1u : 0u);
+            }
+            mma_commit(smem_addr(&bars->s_full[t]));
+          }
+        }
+        if (!ok) break;
+        // A stage that neither row tile used is released as well, once its
+        // copies have landed.
+        if (j < n_kv) {
+          if (!k_ready && !fa_wait(smem_addr(&bars->k_full[j % C::NS]), (j / C::NS) & 1, a.status, wlim)) { ok = false; break; }
+          mma_commit(smem_addr(&bars->k_empty[j % C::NS]));
+        }
+        if (j >= 1) {
+          const int i = j - 1;
+          if (!v_ready && !fa_wait(smem_addr(&bars->v_full[i % C::NS]), (i / C::NS) & 1, a.status, wlim)) { ok = false; break; }
+          mma_commit(smem_addr(&bars->v_empty[i % C::NS]));
+        }
+      }
+      if (!ok) *abort_flag = 1;
+      mma_commit(smem_addr(&bars->mma_final));
+      fa_wait(smem_addr(&bars->mma_final), 0, a.status, wlim);
+    }
+  } else {
+    // ---------------------------------------------------------- softmax
+    reg_alloc_inc<kRegsSoftmax>();
+    const int t = warp >> 2;
+    const int row = threadIdx.x & 127;
+    const int pr = b.row0 + t * BM + row;      // packed row
+    const bool row_ok = pr < b.rows;
+    const int my_kv = (t == 0) ? n_kv_t[0] : n_kv_t[1];
+    const int my_lo = j_min + ((t == 0) ? s_lo[0] : s_lo[1]);
+    const int tok = row_ok ? b.q0 + pr / a.group : 0;
+    const int head = hk * a.group + pr % a.group;
+    if (my_kv > 0) {
+      const T* qrow = reinterpret_cast<const T*>(a.q) + (int64_t)tok * a.q_st + (int64_t)head * a.q_sh;
+      uint8_t* dst = smem + C::OFF_Q + t * C::TILE_BYTES + row * 128;
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (row_ok && c * 8 < a.D) x = *reinterpret_cast<const uint4*>(qrow + c * 8);
+        *reinterpret_cast<uint4*>(dst + (c >> 3) * C::BOX_BYTES + (((c & 7) ^ (row & 7)) << 4)) = x;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_addr(&bars->q_full[t]));
+    }
+    // Key position of the row's query, and the keys [row_lo, row_hi) it sees.
+    int qpos = 0, row_lo = 0, row_hi = 0x7fffffff;
+    if (row_ok) {
+      if (tc.shared) {
+        row_hi = b.klen;
+        if (a.causal || a.win_left >= 0 || a.win_right >= 0 || XF != 0) {
+          int i = tok;
+          if (a.cu_q != nullptr) {
+            int lo = 0, hi = a.B;  // the last request that begins at or before the token
+            while (hi - lo > 1) {
+              const int mid = (lo + hi) >> 1;
+              if (a.cu_q[mid] <= tok) lo = mid;
+              else hi = mid;
+            }
+            i = lo;
+          }
+          const ReqView v = view_request<BN>(a, i, BM);
+          qpos = v.klen - v.qlen + (tok - v.q0);
+          const int2 see = visible_keys(a, v.klen, qpos);
+          row_lo = see.x;
+          row_hi = min(see.y, b.klen);
+        }
+      } else {
+        qpos = b.klen - b.qlen + pr / a.group;
+        const int2 see = visible_keys(a, b.klen, qpos);
+        row_lo = see.x;
+        row_hi = see.y;
+      }
+    }
+    const float slope = (XF != 0 && a.alibi != nullptr) ? a.alibi[head] * kLog2e : 0.f;
+    const float cap_in = XF == 2 ? a.scale / a.softcap : 0.f, cap_log2 = a.softcap * kLog2e;
+    const float sl2 = XF == 0 ? a.scale_log2 : 1.f;
+    const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t tS = lane_base + kColS + t * 128;
+    const uint32_t tO = lane_base + kColO + t * 128;
+    const uint32_t b_s_full = smem_addr(&bars->s_full[t]);
+    const uint32_t b_p_full = smem_addr(&bars->p_full[t][0]);
+    float m_run = -INFINITY, l_run = 0.f;
+    bool ok = true;
+
+    for (int j = 0; j < my_kv; ++j) {
+      if (*abort_flag) { ok = false; break; }
+      const bool got = fa_wait(b_s_full, j & 1, a.status, wlim);
+      if (!__all_sync(0xffffffffu, got)) { ok = false; *abort_flag = 1; break; }
+      tc_fence_after();
+      float s[BN];
+      tmem_ld128(tS, s);
+      const int kv0 = (my_lo + j) * BN;
+      const int key_beg = row_lo - kv0, key_lim = row_hi - kv0;
+      const bool need_mask = __any_sync(0xffffffffu, key_beg > 0 || key_lim < BN);
+      if constexpr (XF == 1) {
+        const float base = (float)(kv0 - qpos);
+#pragma unroll
+        for (int c = 0; c < BN; ++c) s[c] = fmaf(s[c], a.scale_log2, slope * (base + (float)c));
+      }
+      if constexpr (XF == 2) {
+        const float base = (float)(kv0 - qpos);
+#pragma unroll
+        for (int c = 0; c < BN; ++c) s[c] = fmaf(cap_log2, cap_tanh(s[c] * cap_in), slope * (base + (float)c));
+      }
+      float ext;
+      if (!need_mask) {
+        ext = row_max128(s);
+      } else {
+        ext = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < BN; ++c) ext = fmaxf(ext, (c < key_lim && c >= key_beg) ? s[c] : -INFINITY);
+      }
+      const float m_new = fmaxf(m_run, ext * sl2);
+      const bool grow = m_new > m_run + kRescaleThreshold;
+      const bool any_grow = __any_sync(0xffffffffu, grow);
+      const float m_use = any_grow ? m_new : m_run;
+      const float m_sub = (m_use == -INFINITY) ? 0.f : m_use;
+      const float alpha = (m_use == m_run || m_use == -INFINITY) ? 1.f : ex2_approx(m_run - m_use);
+      if (any_grow && j > 0) {
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t r[32];
+          tmem_ld32(tO + c * 32, r);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
+          tmem_st32(tO + c * 32, r);
+        }
+      }
+      float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
+      const float2 sc2 = make_float2(sl2, sl2), nm2 = make_float2(-m_sub, -m_sub);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t p[32];
+        if (need_mask) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const int c = h * 64 + 2 * i;
+            const float p0 = (c < key_lim && c >= key_beg) ? ex2_approx(fmaf(s[c], sl2, -m_sub)) : 0.f;
+            const float p1 = (c + 1 < key_lim && c + 1 >= key_beg) ? ex2_approx(fmaf(s[c + 1], sl2, -m_sub)) : 0.f;
+            acc0 = __fadd2_rn(acc0, make_float2(p0, p1));
+            p[i] = pack_p<T>(p0, p1);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const int c = h * 64 + 2 * i;
+            const float2 x = __ffma2_rn(make_float2(s[c], s[c + 1]), sc2, nm2);
+            const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+            if (i & 1) acc1 = __fadd2_rn(acc1, e);
+            else acc0 = __fadd2_rn(acc0, e);
+            p[i] = pack_p<T>(e.x, e.y);
+          }
+        }
+        tmem_st32(tS + h * 32, p);
+        if (h == 0) {
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(b_p_full);
+        }
+      }
+      l_run = l_run * alpha + (acc0.x + acc0.y) + (acc1.x + acc1.y);
+      m_run = m_use;
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(b_p_full + 8);
+    }
+
+    // -------------------------------------------------------- epilogue
+    if (ok && my_kv > 0) {
+      const bool got = fa_wait(smem_addr(&bars->o_full[t]), 0, a.status, wlim);
+      if (!__all_sync(0xffffffffu, got)) { ok = false; *abort_flag = 1; }
+      tc_fence_after();
+    }
+    if (ok && b.row0 + t * BM < b.rows) {
+      const float inv_l = (l_run > 0.f) ? 1.f / l_run : 0.f;
+      const float lse = (l_run > 0.f) ? (m_run + log2f(l_run)) * kLn2 : -INFINITY;
+      float ov[D];
+      if (my_kv > 0) {
+        if constexpr (D == 128) tmem_ld128(tO, ov);
+        else tmem_ld64(tO, ov);
+#pragma unroll
+        for (int i = 0; i < D; ++i) ov[i] *= inv_l;
+      } else {
+#pragma unroll
+        for (int i = 0; i < D; ++i) ov[i] = 0.f;
+      }
+      if (row_ok) {
+        if (tc.partial) {
+          const int part = tc.part0 + split;
+          float* dst = tc.parts_o + (((int64_t)part * a.total_q + tok) * a.Hq + head) * a.D;
+          tc.parts_lse[((int64_t)part * a.Hq + head) * a.total_q + tok] = lse;
+#pragma unroll
+          for (int c = 0; c < D / 4; ++c)
+            if (c * 4 < a.D)
+              *reinterpret_cast<float4*>(dst + 4 * c) = make_float4(ov[4 * c], ov[4 * c + 1], ov[4 * c + 2], ov[4 * c + 3]);
+        } else {
+          if (a.lse != nullptr) a.lse[(int64_t)head * a.total_q + tok] = lse;
+          const int64_t at = (int64_t)tok * a.o_st + (int64_t)head * a.o_sh;
+          const int elem = a.out_dtype == kF32 ? 4 : 2;
+          uint8_t* dst = reinterpret_cast<uint8_t*>(a.o) + at * elem;
+          if ((reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c) {
+              if (c * 8 >= a.D) continue;
+              const float* x = ov + c * 8;
+              if (a.out_dtype == kF32) {
+                reinterpret_cast<float4*>(dst)[2 * c] = make_float4(x[0], x[1], x[2], x[3]);
+                reinterpret_cast<float4*>(dst)[2 * c + 1] = make_float4(x[4], x[5], x[6], x[7]);
+              } else if (a.out_dtype == kF16) {
+                reinterpret_cast<uint4*>(dst)[c] = make_uint4(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]),
+                                                              pack_half2(x[4], x[5]), pack_half2(x[6], x[7]));
+              } else {
+                reinterpret_cast<uint4*>(dst)[c] = make_uint4(pack_bf162(x[0], x[1]), pack_bf162(x[2], x[3]),
+                                                              pack_bf162(x[4], x[5]), pack_bf162(x[6], x[7]));
+              }
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < D / 4; ++c) {
+              if (c * 4 >= a.D) continue;
+              const float x[4] = {ov[4 * c], ov[4 * c + 1], ov[4 * c + 2], ov[4 * c + 3]};
+              store_out4(a.o, at + 4 * c, a.out_dtype, x, 4);
+            }
+          }
+        }
+      }
+    }
+  }
+
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+template <int D, typename T, int XF>
+cudaError_t launch_xf(const PagedArgs& a, const PagedTc& tc, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t st) {
+  auto kern = paged_attn_sm100<D, T, XF>;
+  constexpr int smem = Cfg<D>::SMEM_BYTES;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  const long long blocks = (long long)tc.n_blocks * a.Hk * tc.n_split;
+  if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
+  e = launch_pdl(kern, dim3((unsigned)blocks), dim3(kThreads), smem, st, tk, tv, a, tc);
+  note_launch();
+  return e;
+}
+
+template <int D, typename T>
+cudaError_t launch_dt(const PagedArgs& a, const PagedTc& tc, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t st) {
+  if (a.softcap > 0.f) return launch_xf<D, T, 2>(a, tc, tk, tv, st);
+  if (a.alibi != nullptr || !(a.scale > 0.f)) return launch_xf<D, T, 1>(a, tc, tk, tv, st);
+  return launch_xf<D, T, 0>(a, tc, tk, tv, st);
+}
+
+}  // namespace paged_tc
+}  // namespace fa

@@ -1,0 +1,11 @@
+// Instantiations of the many-rows paged attention kernel: head_dim up to 64, bf16.
+#include "fa_paged_sm100.cuh"
+
+namespace fa {
+
+cudaError_t launch_paged_tc_d64_bf16(const PagedArgs& a, const PagedTc& tc, const CUtensorMap& tk, const CUtensorMap& tv,
+                                   cudaStream_t st) {
+  return paged_tc::launch_dt<64, __nv_bfloat16>(a, tc, tk, tv, st);
+}
+
+}  // namespace fa
