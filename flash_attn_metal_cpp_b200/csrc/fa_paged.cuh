@@ -210,33 +210,23 @@ __device__ __forceinline__ float cap_tanh(float y) {
 
 // Columns [col, col + 4) of a finished row (token, head): x holds
 // sum exp2(s - m) v and l the sum of exp2(s - m), both over the row's keys
-// (m in log2 units, -inf for no key). Joins the call's partial results (a
-// normalised o and a natural-log lse each) and writes the quotient.
+// (m in log2 units, -inf for no key). Writes the quotient and the row's lse,
+// to the output or, when more partial results of the row are to be joined,
+// to the call's own part of them.
 __device__ __forceinline__ void finish_row4(const PagedArgs& a, int token, int head, int col, float (&x)[4], float m,
                                             float l) {
-  float top = m;
-  for (int p = 0; p < a.n_parts; ++p)
-    top = fmaxf(top, a.parts_lse[((int64_t)p * a.Hq + head) * a.total_q + token] * kLog2e);
-  const float sub = top == -INFINITY ? 0.f : top;
-  const float f = m == -INFINITY ? 0.f : exp2f(m - sub);
-  l *= f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] *= f;
-  for (int p = 0; p < a.n_parts; ++p) {
-    const float lse = a.parts_lse[((int64_t)p * a.Hq + head) * a.total_q + token];
-    const float w = lse == -INFINITY ? 0.f : exp2f(lse * kLog2e - sub);
-    const float* src = a.parts_o + (((int64_t)p * a.total_q + token) * a.Hq + head) * a.D + col;
-    l += w;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (col + i < a.D) x[i] = fmaf(w, src[i], x[i]);
-  }
   const float inv = l > 0.f ? 1.f / l : 0.f;
+  const float lse = l > 0.f ? m * kLn2 + logf(l) : -INFINITY;
 #pragma unroll
   for (int i = 0; i < 4; ++i) x[i] *= inv;
-  store_out4(a.o, (int64_t)token * a.o_st + (int64_t)head * a.o_sh + col, a.out_dtype, x, min(4, a.D - col));
-  if (col == 0 && a.lse != nullptr)
-    a.lse[(int64_t)head * a.total_q + token] = l > 0.f ? sub * kLn2 + logf(l) : -INFINITY;
+  if (a.own_part >= 0) {
+    const int64_t row = ((int64_t)a.own_part * a.total_q + token) * a.Hq + head;
+    store_out4(a.parts_o, row * a.D + col, kF32, x, min(4, a.D - col));
+    if (col == 0) a.parts_lse[row] = lse;
+  } else {
+    store_out4(a.o, (int64_t)token * a.o_st + (int64_t)head * a.o_sh + col, a.out_dtype, x, min(4, a.D - col));
+    if (col == 0 && a.lse != nullptr) a.lse[(int64_t)head * a.total_q + token] = lse;
+  }
 }
 
 }  // namespace fa

@@ -97,11 +97,12 @@ struct PagedArgs {
   float softcap;           // > 0: x = softcap * tanh(scale * q.k / softcap)
   int causal, win_left, win_right;
   const float* alibi;      // [Hq] (NULL = none)
-  // Partial results already computed for every row and joined when a row is
-  // finished: o [n_parts, total_q, Hq, D] and lse [n_parts, Hq, total_q].
+  // Partial results of whole rows, joined by a last kernel: normalised o
+  // [n_parts, total_q, Hq, D] and natural-log lse [n_parts, total_q, Hq].
   int n_parts;
-  const float* parts_o;
-  const float* parts_lse;
+  int own_part;            // part that the few-rows and CUDA-core kernels write (-1: the output)
+  float* parts_o;
+  float* parts_lse;
   // Work that the kernels cut in n_ctas equal runs of key tiles (split = 1):
   // per run two partial units of rows_per_unit rows, and where they belong.
   int split;
@@ -147,8 +148,6 @@ struct PagedTc {
   int box_rows;      // slots of one TMA box
   int partial;       // 1: normalised partial results to part0 + split
   int part0;
-  float* parts_o;    // [parts, total_q, Hq, D]
-  float* parts_lse;  // [parts, Hq, total_q]
 };
 cudaError_t launch_paged_tc_d64_f16(const PagedArgs&, const PagedTc&, const CUtensorMap&, const CUtensorMap&, cudaStream_t);
 cudaError_t launch_paged_tc_d64_bf16(const PagedArgs&, const PagedTc&, const CUtensorMap&, const CUtensorMap&, cudaStream_t);

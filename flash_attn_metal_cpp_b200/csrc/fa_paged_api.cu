@@ -136,6 +136,7 @@ struct Choice {
   int own_split, pre_split;        // parts the keys are cut in
   int own_blocks, pre_blocks;      // blocks of 256 packed rows
   int rows_per_unit, n_ctas, join_rows, split;
+  int n_parts;                     // whole-row partial results to join (0: none)
   CutLayout cut;
   size_t parts_lse, parts_o, bytes;  // offsets of the partial results
 };
@@ -215,7 +216,10 @@ Choice choose(const fa_paged_params* p, const Checked& c, bool vec, bool one) {
     h.cut = cut_layout(h.n_ctas, h.rows_per_unit, a.D);
     h.bytes = h.cut.bytes;
   }
-  const size_t parts = (size_t)h.pre_split + ((h.many && (h.shared || h.own_split > 1)) ? h.own_split : 0);
+  // Whole-row partial results: the prefix's, then the own keys' (the few-rows
+  // kernel makes one part of them).
+  h.n_parts = h.pre_split + (h.many ? (h.shared || h.own_split > 1 ? h.own_split : 0) : (h.shared ? 1 : 0));
+  const size_t parts = (size_t)h.n_parts;
   h.parts_lse = h.bytes;
   h.parts_o = h.parts_lse + up256(parts * a.Hq * a.total_q * sizeof(float));
   h.bytes = h.parts_o + up256(parts * (size_t)a.total_q * a.Hq * a.D * sizeof(float));
@@ -395,13 +399,13 @@ fa_status fa_paged_forward(const fa_paged_params* p, const void* q, const void* 
   const bool vec = c.vec && aligned(q, 16) && aligned(k_cache, 16) && aligned(v_cache, 16);
   const Choice h = choose(p, c, vec, cu_seqlens_q == nullptr);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  float* parts_lse = reinterpret_cast<float*>(ws + h.parts_lse);
-  float* parts_o = reinterpret_cast<float*>(ws + h.parts_o);
+  a.n_parts = h.n_parts;
+  a.own_part = h.n_parts > 0 && !h.many ? h.pre_split : -1;
+  a.parts_lse = reinterpret_cast<float*>(ws + h.parts_lse);
+  a.parts_o = reinterpret_cast<float*>(ws + h.parts_o);
   CUtensorMap tk, tv;
   PagedTc t{};
   t.box_rows = h.box;
-  t.parts_o = parts_o;
-  t.parts_lse = parts_lse;
   if (h.shared || h.many) {
     const bool bf = c.dtype == kBF16;
     st = paged_encode(&tk, k_cache, bf, a.D, a.Hk, a.page_size, a.num_pages, a.k_sp, a.k_ss, a.k_sh, h.box);
@@ -418,31 +422,25 @@ fa_status fa_paged_forward(const fa_paged_params* p, const void* q, const void* 
     if (st != FA_OK) return st;
     a.pre = 0;  // what follows sees each request's own keys
     a.pre_table = nullptr;
-    a.n_parts = h.pre_split;
-    a.parts_o = parts_o;
-    a.parts_lse = parts_lse;
   }
   if (h.many) {
     t.shared = 0;
     t.n_blocks = h.own_blocks;
     t.n_split = h.own_split;
-    t.partial = h.shared || h.own_split > 1;
-    t.part0 = a.n_parts;
+    t.partial = h.n_parts > 0;
+    t.part0 = h.pre_split;
     st = cuda_status(launch_tc(a, t, c.dtype, tk, tv, s), "paged attention (many rows)");
-    if (st != FA_OK || !t.partial) return st;
-    a.n_parts += h.own_split;
-    a.parts_o = parts_o;
-    a.parts_lse = parts_lse;
-    return cuda_status(launch_paged_merge(a, s), "paged attention (merge)");
+  } else {
+    a.rows_per_unit = h.rows_per_unit;
+    a.n_ctas = h.n_ctas;
+    a.join_rows = h.join_rows;
+    a.split = h.split;
+    place_cut(a, h.cut, workspace);
+    st = h.tensor ? cuda_status(launch_paged_decode(a, c.dtype, s), "paged attention (few rows)")
+                  : cuda_status(launch_paged_simt(a, c.dtype, vec, s), "paged attention (CUDA cores)");
+    if (st == FA_OK && a.split) st = cuda_status(launch_paged_join(a, s), "paged attention (join)");
   }
-  a.rows_per_unit = h.rows_per_unit;
-  a.n_ctas = h.n_ctas;
-  a.join_rows = h.join_rows;
-  a.split = h.split;
-  place_cut(a, h.cut, workspace);
-  st = h.tensor ? cuda_status(launch_paged_decode(a, c.dtype, s), "paged attention (few rows)")
-                : cuda_status(launch_paged_simt(a, c.dtype, vec, s), "paged attention (CUDA cores)");
-  if (st == FA_OK && a.split) st = cuda_status(launch_paged_join(a, s), "paged attention (join)");
+  if (st == FA_OK && h.n_parts > 0) st = cuda_status(launch_paged_merge(a, s), "paged attention (merge)");
   return st;
 }
 

@@ -285,18 +285,58 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const Paged
   finish_row4(a, mt.q0 + row / a.group, mt.hk * a.group + row % a.group, col, x, top, ls);
 }
 
-// Rows whose every part is a whole-row partial result: one warp a row.
+// Join of whole-row partial results: LSE = log sum_p exp(lse_p),
+// o = sum_p exp(lse_p - LSE) o_p. One warp a row; the lanes first take one
+// part's lse each, then 4 columns each of all parts, several parts in flight.
 __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedArgs a) {
   grid_dep_wait();
   grid_dep_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const int64_t row = blockIdx.x * 8ll + (threadIdx.x >> 5);  // token * Hq + head
+  const int64_t rows = (int64_t)a.total_q * a.Hq;
+  if (row >= rows) return;
+  const int tok = (int)(row / a.Hq), head = (int)(row - (int64_t)tok * a.Hq);
   const int last = a.cu_q ? min(max(a.cu_q[a.B], 0), a.total_q) : min(a.B, a.total_q);
-  const long long r = blockIdx.x * 8ll + (threadIdx.x >> 5);
-  const int tok = (int)(r / a.Hq), head = (int)(r - (long long)tok * a.Hq);
-  if (tok >= last) return;  // rows behind the last sequence
-  for (int col = (threadIdx.x & 31) * 4; col < a.D; col += 128) {
-    float x[4] = {0.f, 0.f, 0.f, 0.f};
-    finish_row4(a, tok, head, col, x, -INFINITY, 0.f);
+  const int first = a.cu_q ? min(max(a.cu_q[0], 0), a.total_q) : 0;
+  if (tok < first || tok >= last) return;  // of no sequence
+  float top = -INFINITY;
+  for (int p = lane; p < a.n_parts; p += 32) top = fmaxf(top, a.parts_lse[p * rows + row]);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+  const float sub = top == -INFINITY ? 0.f : top;
+  float x[2][4] = {}, l = 0.f;
+  for (int p0 = 0; p0 < a.n_parts; p0 += 32) {
+    const int n = min(32, a.n_parts - p0);
+    float w = 0.f;
+    if (lane < n) w = expf(a.parts_lse[(p0 + lane) * rows + row] - sub);
+#pragma unroll 4
+    for (int p = 0; p < n; ++p) {
+      const float f = __shfl_sync(0xffffffffu, w, p);
+      l += f;
+      const float* src = a.parts_o + ((p0 + p) * rows + row) * a.D;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int col = c * 128 + lane * 4;
+        if (col < a.D) {
+          const float4 y = *reinterpret_cast<const float4*>(src + col);
+          x[c][0] = fmaf(f, y.x, x[c][0]);
+          x[c][1] = fmaf(f, y.y, x[c][1]);
+          x[c][2] = fmaf(f, y.z, x[c][2]);
+          x[c][3] = fmaf(f, y.w, x[c][3]);
+        }
+      }
+    }
   }
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const int col = c * 128 + lane * 4;
+    if (col >= a.D) continue;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[c][i] *= inv;
+    store_out4(a.o, (int64_t)tok * a.o_st + (int64_t)head * a.o_sh + col, a.out_dtype, x[c], 4);
+  }
+  if (lane == 0 && a.lse != nullptr) a.lse[(int64_t)head * a.total_q + tok] = l > 0.f ? sub + logf(l) : -INFINITY;
 }
 
 template <typename T, int DM, int R, bool VEC>

@@ -582,8 +582,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (row_ok) {
         if (tc.partial) {
           const int part = tc.part0 + split;
-          float* dst = tc.parts_o + (((int64_t)part * a.total_q + tok) * a.Hq + head) * a.D;
-          tc.parts_lse[((int64_t)part * a.Hq + head) * a.total_q + tok] = lse;
+          const int64_t prow = ((int64_t)part * a.total_q + tok) * a.Hq + head;
+          float* dst = a.parts_o + prow * a.D;
+          a.parts_lse[prow] = lse;
 #pragma unroll
           for (int c = 0; c < D / 4; ++c)
             if (c * 4 < a.D)
