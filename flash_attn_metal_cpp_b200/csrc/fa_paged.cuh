@@ -145,19 +145,22 @@ __device__ __forceinline__ Run find_run(const PagedArgs& a, int rows_per_unit, i
   return r;
 }
 
-// Physical page of key `key` of a request (-1 when the table names none of
-// the cache's pages) and its slot in the page.
+// Table entry of key `key` of a request and its slot in the page. The entry
+// is not checked here, so that the load can stay in flight: valid_page does.
 __device__ __forceinline__ int2 find_key(const PagedArgs& a, int req, int key) {
   const bool shared = key < a.pre;
   const int own = shared ? key : key - a.pre;
   const int p = own / a.page_size;
   const int slot = own - p * a.page_size;
-  int page = shared ? a.pre_table[p] : a.table[(int64_t)req * a.table_stride + p];
-  if ((unsigned)page >= (unsigned)a.num_pages) {
-    note_bad_index(a.status);
-    page = -1;
-  }
-  return make_int2(page, slot);
+  const int* entry = shared ? a.pre_table + p : a.table + (int64_t)req * a.table_stride + p;
+  return make_int2(*entry, slot);
+}
+
+// The page, or -1 (and a note) when the table names none of the cache's.
+__device__ __forceinline__ int valid_page(const PagedArgs& a, int page) {
+  if ((unsigned)page < (unsigned)a.num_pages) return page;
+  note_bad_index(a.status);
+  return -1;
 }
 
 // Keys [lo, hi) visible to the query at key position `pos` of a request with

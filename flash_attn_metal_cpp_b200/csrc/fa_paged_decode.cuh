@@ -57,7 +57,7 @@ template <int NS, int MT>
 struct Shared {
   RunScratch scratch;
   TileDesc desc[NS + 1];
-  int2 page[NS + 1][kTile];
+  longlong2 at[NS + 1][kTile];   // element offsets of each key's K and V row (negative: no row)
   float red_m[4][MT * 16], red_l[4][MT * 16];
 };
 
@@ -104,6 +104,7 @@ template <int MR>
 struct Cursor {
   long long left;   // tiles (uncut work: units) still to come
   int req, unit, tile;
+  int hk, row0;     // of the unit
   ReqView v;
   bool at_begin;    // the current piece is the run's first
   bool new_piece;
@@ -118,16 +119,16 @@ struct Cursor {
     const int per = v.per_unit(a);
     unit = (int)(off / per);
     tile = v.tile_lo + (a.split ? (int)(off - (long long)unit * per) : 0);
+    hk = unit % a.Hk;
+    row0 = unit / a.Hk * MR;
   }
-  __device__ __forceinline__ int hk(const PagedArgs& a) const { return unit % a.Hk; }
-  __device__ __forceinline__ int row0(const PagedArgs& a) const { return unit / a.Hk * MR; }
 
   // Describes the current tile and moves on.
   __device__ __forceinline__ void next(const PagedArgs& a, TileDesc& d) {
     d.rows = 0;
     if (left <= 0) return;
-    d.hk = hk(a);
-    d.row0 = row0(a);
+    d.hk = hk;
+    d.row0 = row0;
     d.rows = min(MR, v.qlen * a.group - d.row0);
     d.q0 = v.q0;
     d.qlen = v.qlen;
@@ -145,8 +146,12 @@ struct Cursor {
     if (d.last) at_begin = false;
     ++tile;
     if (unit_end && left > 0) {
+      if (++hk == a.Hk) {
+        hk = 0;
+        row0 += MR;
+      }
       if (++unit == v.units) {
-        unit = 0;
+        unit = hk = row0 = 0;
         do {
           v = view_request<kTile>(a, ++req, MR);
         } while (v.units == 0);
@@ -186,40 +191,49 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
     mt.total = run.total;
     mt.n_runs = run.n_runs;
     mt.q0 = cur.v.q0;
-    mt.row0 = cur.row0(a);
+    mt.row0 = cur.row0;
     mt.rows = min(MR, cur.v.qlen * a.group - mt.row0);
-    mt.hk = cur.hk(a);
+    mt.hk = cur.hk;
   }
 
-  // Page and slot of key `tid` of a tile (page -1: not loaded).
+  // Table entry and slot of key `tid` of a tile (slot -1: no key).
+  // put_rows() checks the entry and turns it into row offsets a tile later:
+  // the load is in flight until then, and the copies need one addition each.
   auto look_up = [&](const TileDesc& d, int req) {
-    int2 ps = make_int2(-1, 0);
+    int2 ps = make_int2(-1, -1);
     if (tid < kTile && d.rows > 0) {
       const int key = d.tile * kTile + tid;
       if (key >= d.key_lo && key < d.klen) ps = find_key(a, req, key);
     }
     return ps;
   };
-  auto put = [&](int i, const TileDesc& d, int2 ps) {
-    if (tid < kTile) sh.page[i][tid] = ps;
-    if (tid == 0) sh.desc[i] = d;
+  auto put_rows = [&](int i, int2 ps, int hk) {
+    if (tid >= kTile) return;
+    longlong2 at = make_longlong2(-1, -1);
+    if (ps.y >= 0 && valid_page(a, ps.x) >= 0) {
+      at.x = (int64_t)ps.x * a.k_sp + (int64_t)ps.y * a.k_ss + (int64_t)hk * a.k_sh;
+      at.y = (int64_t)ps.x * a.v_sp + (int64_t)ps.y * a.v_ss + (int64_t)hk * a.v_sh;
+    }
+    sh.at[i][tid] = at;
   };
   // Copies of tile `i` (slot i of desc and page) into stage `st`.
   auto issue = [&](int i, int st) {
     const TileDesc& d = sh.desc[i];
     if (d.rows > 0) {
       const uint32_t sk = ring_addr + st * C::STAGE, sv = sk + C::KV_BYTES;
-      const int64_t kh = (int64_t)d.hk * a.k_sh, vh = (int64_t)d.hk * a.v_sh;
+      // A thread copies the same 16-byte column of every row it takes.
+      const int c = tid % CPR, row0 = tid / CPR;
+      const bool col_on = c * 8 < a.D;
+      const T* kc = K + c * 8;
+      const T* vc = V + c * 8;
 #pragma unroll
       for (int n = 0; n < kTile * CPR / kThreads; ++n) {
-        const int e = n * kThreads + tid, row = e / CPR, c = e % CPR;
-        const int2 ps = sh.page[i][row];
-        const bool on = ps.x >= 0 && c * 8 < a.D;
+        const int row = row0 + n * (kThreads / CPR);
+        const longlong2 at = sh.at[i][row];
+        const bool on = at.x >= 0 && col_on;
         const uint32_t off = row * (DM * 2) + ((c ^ (row & 7)) << 4);
-        const T* ks = on ? K + (int64_t)ps.x * a.k_sp + (int64_t)ps.y * a.k_ss + kh + c * 8 : K;
-        const T* vs = on ? V + (int64_t)ps.x * a.v_sp + (int64_t)ps.y * a.v_ss + vh + c * 8 : V;
-        cp_async16(sk + off, ks, on);
-        cp_async16(sv + off, vs, on);
+        cp_async16(sk + off, on ? kc + at.x : K, on);
+        cp_async16(sv + off, on ? vc + at.y : V, on);
       }
       if (d.first) {
         const uint32_t sq = sk + 2 * C::KV_BYTES;
@@ -241,6 +255,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
     // Prologue: page numbers of the first NS tiles together, then the copies
     // of NS - 1 of them.
     int2 ps[NS];
+    int hks[NS];
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
       TileDesc d;
@@ -248,10 +263,10 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
       cur.next(a, d);
       if (tid == 0) sh.desc[i] = d;
       ps[i] = look_up(d, req);
+      hks[i] = d.hk;
     }
 #pragma unroll
-    for (int i = 0; i < NS; ++i)
-      if (tid < kTile) sh.page[i][tid] = ps[i];
+    for (int i = 0; i < NS; ++i) put_rows(i, ps[i], hks[i]);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < NS - 1; ++i) issue(i, i);
@@ -261,6 +276,8 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
   float o[MT][NB][4];
   float m[MT][2], l[MT][2], slope[MT][2];
   int lo[MT][2], hi[MT][2], qpos[MT][2];
+  int full_lo = 0, full_hi = 0;  // keys that every row of the unit sees
+  const bool plain = a.softcap == 0.f && a.alibi == nullptr && a.scale > 0.f;
   const float cap_in = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
   const float cap_log2 = a.softcap * kLog2e;
 
@@ -268,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
   while (true) {
     cp_async_wait<NS - 2>();
     __syncthreads();
-    const TileDesc d = sh.desc[di];
+    const TileDesc& d = sh.desc[di];
     if (d.rows == 0) break;
     const int di_issue = di + NS - 1 > NS ? di - 2 : di + NS - 1;   // (di + NS - 1) mod (NS + 1)
     issue(di_issue, st == 0 ? NS - 1 : st - 1);
@@ -279,6 +296,9 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
 
     const uint32_t sk = ring_addr + st * C::STAGE, sv = sk + C::KV_BYTES;
     if (d.first) {
+      const int p0 = d.klen - d.qlen + d.row0 / a.group, p1 = d.klen - d.qlen + (d.row0 + d.rows - 1) / a.group;
+      full_hi = plain ? visible_keys(a, d.klen, p0).y : 0;
+      full_lo = max(visible_keys(a, d.klen, p1).x, d.key_lo);
       const uint32_t sq = sk + 2 * C::KV_BYTES;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
@@ -326,32 +346,43 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
         }
       }
     }
-    // Online softmax of the warp's rows (log2 units).
-    const int key0 = d.tile * kTile + warp * 16 + (lane & 3) * 2;
+    // Online softmax of the warp's rows (log2 units). A tile that every row
+    // sees whole, with nothing but a positive scale on the scores, needs no
+    // masks and folds the scale into the exponent.
+    const bool fast = d.tile * kTile >= full_lo && (d.tile + 1) * kTile <= full_hi;
     uint32_t p[MT][4];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      float top[2] = {-INFINITY, -INFINITY};
+      float top[2];
+      if (fast) {
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+        for (int e = 0; e < 2; ++e)
+          top[e] = fmaxf(fmaxf(s[mt][0][2 * e], s[mt][0][2 * e + 1]), fmaxf(s[mt][1][2 * e], s[mt][1][2 * e + 1]));
+      } else {
+        const int key0 = d.tile * kTile + warp * 16 + (lane & 3) * 2;
+        top[0] = top[1] = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int e = i >> 1, key = key0 + n * 8 + (i & 1);
-          float x;
-          if (a.softcap > 0.f) x = cap_log2 * cap_tanh(s[mt][n][i] * cap_in);
-          else x = s[mt][n][i] * a.scale_log2;
-          x = fmaf(slope[mt][e], (float)(key - qpos[mt][e]), x);
-          x = (key >= lo[mt][e] && key < hi[mt][e]) ? x : -INFINITY;
-          s[mt][n][i] = x;
-          top[e] = fmaxf(top[e], x);
-        }
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int e = i >> 1, key = key0 + n * 8 + (i & 1);
+            float x;
+            if (a.softcap > 0.f) x = cap_log2 * cap_tanh(s[mt][n][i] * cap_in);
+            else x = s[mt][n][i] * a.scale_log2;
+            x = fmaf(slope[mt][e], (float)(key - qpos[mt][e]), x);
+            x = (key >= lo[mt][e] && key < hi[mt][e]) ? x : -INFINITY;
+            s[mt][n][i] = x;
+            top[e] = fmaxf(top[e], x);
+          }
+      }
+      const float mul = fast ? a.scale_log2 : 1.f;
       float f[2], sub[2];
       bool grow = false;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
         top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
-        const float nm = fmaxf(m[mt][e], top[e]);
+        const float nm = fmaxf(m[mt][e], top[e] * mul);
         grow |= nm > m[mt][e];
         sub[e] = nm == -INFINITY ? 0.f : nm;
         f[e] = ex2_approx(m[mt][e] - sub[e]);  // 0 for the first keys of a row
@@ -372,10 +403,9 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
       for (int n = 0; n < 2; ++n) {
         float x[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[i] = ex2_approx(s[mt][n][i] - sub[i >> 1]);
-          l[mt][i >> 1] += x[i];
-        }
+        for (int i = 0; i < 4; ++i) x[i] = ex2_approx(fmaf(s[mt][n][i], mul, -sub[i >> 1]));
+        l[mt][0] += x[0] + x[1];
+        l[mt][1] += x[2] + x[3];
         p[mt][2 * n] = pack2<T>(x[0], x[1]);
         p[mt][2 * n + 1] = pack2<T>(x[2], x[3]);
       }
@@ -462,7 +492,9 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
       }
     }
     // Slot (di + NS) mod (NS + 1) was the tile before this one: free again.
-    put(di == 0 ? NS : di - 1, dn, pn);
+    const int dp = di == 0 ? NS : di - 1;
+    put_rows(dp, pn, dn.hk);
+    if (tid == 0) sh.desc[dp] = dn;
     di = di == NS ? 0 : di + 1;
     st = st == NS - 1 ? 0 : st + 1;
   }

@@ -128,7 +128,8 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
       float kx[DPL], vx[DPL];
       bool on = key < key_end && key >= v.key_lo;
       if (on) {
-        const int2 ps = find_key(a, req, key);
+        int2 ps = find_key(a, req, key);
+        ps.x = valid_page(a, ps.x);
         on = ps.x >= 0;
         if (on) {
           load_slice<T, DPL, VEC>(K + (int64_t)ps.x * a.k_sp + (int64_t)ps.y * a.k_ss + (int64_t)hk * a.k_sh, sub, a.D, kx);
