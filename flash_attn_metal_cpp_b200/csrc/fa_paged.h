@@ -103,10 +103,11 @@ struct PagedArgs {
   int own_part;            // part that the few-rows and CUDA-core kernels write (-1: the output)
   float* parts_o;
   float* parts_lse;
-  // Work that the kernels cut in n_ctas equal runs of key tiles (split = 1):
+  // Work that the kernels cut in n_ctas equal runs (split = 1, fa_paged.cuh):
   // per run two partial units of rows_per_unit rows, and where they belong.
   int split;
   int n_ctas;
+  int min_run;             // least length of a run
   int rows_per_unit;
   int join_rows;           // most rows a unit can have here (for the join's grid)
   float* slot_o;           // [n_ctas, 2, rows_per_unit, D] unnormalised
@@ -119,10 +120,10 @@ struct PagedArgs {
 // Where one run of the cut work begins (written by the attention kernel, read
 // by the join).
 struct RunMeta {
-  long long begin;         // first key tile of the run, in tiles of the whole call
-  long long unit_begin;    // first and one past the last tile of the unit it begins in
+  long long begin;         // of the run, in the call's line of work
+  long long unit_begin;    // of the unit it begins in
   long long unit_end;
-  long long total;         // tiles of the whole call
+  long long total;         // length of the line
   int n_runs;              // runs in use (0: run not in use)
   int q0;                  // first query row of the unit's request
   int row0;                // first packed row of the unit (row = token * group + head of the group)

@@ -102,25 +102,34 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 // Steps through the tiles of a run: request, unit (chunk of rows, KV head), tile.
 template <int MR>
 struct Cursor {
-  long long left;   // tiles (uncut work: units) still to come
-  int req, unit, tile;
-  int hk, row0;     // of the unit
+  long long left;        // of the line, from the unit's beginning on
+  int req, unit, per;    // per: a unit's stretch of the line
+  int hk, row0;          // of the unit
+  int tile, tile_end;    // of the current piece, from the unit's first tile
+  bool run_first;        // the current piece is the run's first
+  bool new_piece, whole;
   ReqView v;
-  bool at_begin;    // the current piece is the run's first
-  bool new_piece;
 
+  __device__ __forceinline__ void begin_piece(const PagedArgs& a, int first) {
+    tile = first;
+    tile_end = a.split && left < per ? tile_at(left) : v.tiles;
+    whole = first == 0 && tile_end == v.tiles;
+    new_piece = true;
+  }
   __device__ __forceinline__ void start(const PagedArgs& a, const Run& run) {
-    left = run.end - run.begin;
-    at_begin = new_piece = true;
-    if (left <= 0) return;
+    left = 0;
+    run_first = true;
+    if (run.end <= run.begin) return;
     req = run.req;
     v = view_request<kTile>(a, req, MR);
+    per = v.per_unit(a);
     const long long off = run.begin - run.req_begin;
-    const int per = v.per_unit(a);
     unit = (int)(off / per);
-    tile = v.tile_lo + (a.split ? (int)(off - (long long)unit * per) : 0);
+    const long long in_unit = off - (long long)unit * per;
+    left = run.end - run.begin + in_unit;
     hk = unit % a.Hk;
     row0 = unit / a.Hk * MR;
+    begin_piece(a, a.split ? tile_at(in_unit) : 0);
   }
 
   // Describes the current tile and moves on.
@@ -129,37 +138,36 @@ struct Cursor {
     if (left <= 0) return;
     d.hk = hk;
     d.row0 = row0;
-    d.rows = min(MR, v.qlen * a.group - d.row0);
+    d.rows = min(MR, v.qlen * a.group - row0);
     d.q0 = v.q0;
     d.qlen = v.qlen;
     d.klen = v.klen;
     d.key_lo = v.key_lo;
-    d.tile = tile;
+    d.tile = v.tile_lo + tile;
     d.first = new_piece;
-    const bool unit_end = tile + 1 == v.tile_lo + v.tiles;
-    if (new_piece) piece_tile = tile;
-    if (a.split || unit_end) --left;
-    d.last = unit_end || left == 0;
-    d.whole = unit_end && piece_tile == v.tile_lo;
-    d.slot = at_begin ? 0 : 1;
-    new_piece = d.last;
-    if (d.last) at_begin = false;
-    ++tile;
-    if (unit_end && left > 0) {
-      if (++hk == a.Hk) {
-        hk = 0;
-        row0 += MR;
+    d.whole = whole;
+    d.slot = run_first ? 0 : 1;
+    new_piece = false;
+    d.last = ++tile == tile_end;
+    if (d.last) {
+      run_first = false;
+      left -= per;
+      if (left > 0) {
+        if (++hk == a.Hk) {
+          hk = 0;
+          row0 += MR;
+        }
+        if (++unit == v.units) {
+          unit = hk = row0 = 0;
+          do {
+            v = view_request<kTile>(a, ++req, MR);
+          } while (v.units == 0);
+          per = v.per_unit(a);
+        }
+        begin_piece(a, 0);
       }
-      if (++unit == v.units) {
-        unit = hk = row0 = 0;
-        do {
-          v = view_request<kTile>(a, ++req, MR);
-        } while (v.units == 0);
-      }
-      tile = v.tile_lo;
     }
   }
-  int piece_tile;
 };
 
 template <typename T, int DM, int MT>
@@ -176,7 +184,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
 
   grid_dep_wait();
   grid_dep_launch_dependents();
-  const Run run = find_run<kTile, kThreads>(a, MR, blockIdx.x, gridDim.x, 2, &sh.scratch);
+  const Run run = find_run<kTile, kThreads>(a, MR, blockIdx.x, gridDim.x, a.min_run, &sh.scratch);
   if (run.end <= run.begin) {
     if (a.split && tid == 0) a.meta[blockIdx.x].n_runs = 0;
     return;
@@ -186,8 +194,8 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
   if (a.split && tid == 0) {
     RunMeta& mt = a.meta[blockIdx.x];
     mt.begin = run.begin;
-    mt.unit_begin = run.begin - (cur.tile - cur.v.tile_lo);
-    mt.unit_end = mt.unit_begin + cur.v.tiles;
+    mt.unit_begin = run.req_begin + (long long)cur.unit * cur.per;
+    mt.unit_end = mt.unit_begin + cur.per;
     mt.total = run.total;
     mt.n_runs = run.n_runs;
     mt.q0 = cur.v.q0;
@@ -452,6 +460,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
           for (int w = 1; w < 4; ++w) top = fmaxf(top, sh.red_m[w][mt * 16 + r]);
           const float f = m[mt][e] == -INFINITY ? 0.f : ex2_approx(m[mt][e] - top);
           float* row = buf + (warp * 16 + r) * DM;
+          if (mt * 16 + r >= d.rows) continue;
 #pragma unroll
           for (int n = 0; n < NB; ++n) {
             const int c4 = n * 2 + ((lane & 3) >> 1);

@@ -10,7 +10,9 @@ cudaError_t launch_paged_decode_bf16(const PagedArgs& a, cudaStream_t st);
 // registers).
 int decode_rows_per_unit(int D, long long rows) { return rows > 16 && D <= 128 ? 32 : 16; }
 
-// One wave of blocks: two an SM, one where the ring of a block fills it.
+// One wave of blocks: two an SM, one where the ring of a block fills it. More
+// and shorter runs measured slower (64 requests of up to 32769 tokens: 262 us
+// with one wave, 271 with two, 280 with three).
 int decode_ctas(int D, int rows_per_unit) {
   return 148 * ((D > 128 || (D > 64 && rows_per_unit == 32)) ? 1 : 2);
 }

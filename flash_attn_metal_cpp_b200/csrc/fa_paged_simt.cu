@@ -8,7 +8,7 @@
 //
 // One block of 4 warps works through its run of tiles (fa_paged.cuh). In a
 // warp 8 lanes share one key (each holds every 8th 16-byte piece of its row),
-// so 4 keys are in work at once and a dot product needs 3 shuffles; every
+// so 4 keys (8 with two in flight) are in work at once and a dot product needs 3 shuffles; every
 // group of 8 lanes keeps its own m, l and o until the unit ends. A unit has 1
 // row (one query head on a KV head) or 4 rows (2 for head_dim above 128) that
 // use each key row loaded. fp32 decoding is bound by memory latency, so the
@@ -20,7 +20,7 @@
 namespace fa {
 namespace {
 
-constexpr int kTile = 64;
+constexpr int kTile = 32;
 constexpr int kThreads = 128;
 
 // DPL elements of a row: lane `sub` of 8 holds vectors sub, sub + 8, ...
@@ -55,6 +55,7 @@ __device__ __forceinline__ int slice_col(int sub, int i) {
 template <typename T, int DM, int R, bool VEC>
 __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a) {
   constexpr int DPL = DM / 8;
+  constexpr int U = DM <= 128 ? 2 : 1;  // keys a lane group has in flight
   __shared__ RunScratch scratch;
   __shared__ float sm_o[4][R][DM];
   __shared__ float sm_m[4][R], sm_l[4][R];
@@ -64,7 +65,7 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
 
   grid_dep_wait();
   grid_dep_launch_dependents();
-  const Run run = find_run<kTile, kThreads>(a, R, blockIdx.x, gridDim.x, 1, &scratch);
+  const Run run = find_run<kTile, kThreads>(a, R, blockIdx.x, gridDim.x, a.min_run, &scratch);
   if (run.end <= run.begin) {
     if (a.split && tid == 0) a.meta[blockIdx.x].n_runs = 0;
     return;
@@ -86,17 +87,18 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
       continue;
     }
     const int unit = (int)(off / per);
-    const int t0 = v.tile_lo + (a.split ? (int)(off - (long long)unit * per) : 0);
+    const long long unit_begin = req_begin + (long long)unit * per;
     const int t_end = v.tile_lo + v.tiles;
-    const int t1 = a.split ? (int)min((long long)t_end, t0 + (run.end - at)) : t_end;
+    const int t0 = v.tile_lo + (a.split ? tile_at(at - unit_begin) : 0);
+    const int t1 = a.split && run.end < unit_begin + per ? v.tile_lo + tile_at(run.end - unit_begin) : t_end;
     const int hk = unit % a.Hk;
     const int row0 = unit / a.Hk * R;
     const int rows = min(R, v.qlen * a.group - row0);
     if (a.split && at == run.begin && tid == 0) {
       RunMeta& mt = a.meta[blockIdx.x];
       mt.begin = run.begin;
-      mt.unit_begin = req_begin + (long long)unit * per;
-      mt.unit_end = mt.unit_begin + per;
+      mt.unit_begin = unit_begin;
+      mt.unit_end = unit_begin + per;
       mt.total = run.total;
       mt.n_runs = run.n_runs;
       mt.q0 = v.q0;
@@ -122,49 +124,63 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
 #pragma unroll
       for (int i = 0; i < DPL; ++i) o[r][i] = 0.f;
     }
-    const int key_end = min(v.klen, t1 * kTile);
-    for (int base = t0 * kTile + warp * 4; base < key_end; base += 16) {
-      const int key = base + kg;
-      float kx[DPL], vx[DPL];
-      bool on = key < key_end && key >= v.key_lo;
-      if (on) {
-        int2 ps = find_key(a, req, key);
-        ps.x = valid_page(a, ps.x);
-        on = ps.x >= 0;
-        if (on) {
-          load_slice<T, DPL, VEC>(K + (int64_t)ps.x * a.k_sp + (int64_t)ps.y * a.k_ss + (int64_t)hk * a.k_sh, sub, a.D, kx);
-          load_slice<T, DPL, VEC>(V + (int64_t)ps.x * a.v_sp + (int64_t)ps.y * a.v_ss + (int64_t)hk * a.v_sh, sub, a.D, vx);
+    const int key_begin = max(v.key_lo, t0 * kTile), key_end = min(v.klen, t1 * kTile);
+    // Table entries one step ahead of the rows they lead to.
+    int2 next[U];
+    auto fetch = [&](int base) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int key = base + u * 16 + kg;
+        next[u] = key >= key_begin && key < key_end ? find_key(a, req, key) : make_int2(-1, -1);
+      }
+    };
+    const int base0 = t0 * kTile + warp * 4;
+    fetch(base0);
+    for (int base = base0; base < key_end; base += 16 * U) {
+      float kx[U][DPL], vx[U][DPL];
+      bool on[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        on[u] = next[u].y >= 0 && valid_page(a, next[u].x) >= 0;
+        if (on[u]) {
+          const int64_t page = next[u].x, slot = next[u].y;
+          load_slice<T, DPL, VEC>(K + page * a.k_sp + slot * a.k_ss + (int64_t)hk * a.k_sh, sub, a.D, kx[u]);
+          load_slice<T, DPL, VEC>(V + page * a.v_sp + slot * a.v_ss + (int64_t)hk * a.v_sh, sub, a.D, vx[u]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < DPL; ++i) kx[u][i] = vx[u][i] = 0.f;
         }
       }
-      if (!on) {
+      fetch(base + 16 * U);
 #pragma unroll
-        for (int i = 0; i < DPL; ++i) kx[i] = vx[i] = 0.f;
-      }
+      for (int u = 0; u < U; ++u) {
+        const int key = base + u * 16 + kg;
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        float s = 0.f;
+        for (int r = 0; r < R; ++r) {
+          float s = 0.f;
 #pragma unroll
-        for (int i = 0; i < DPL; ++i) s = fmaf(q[r][i], kx[i], s);
-        s += __shfl_xor_sync(0xffffffffu, s, 1);
-        s += __shfl_xor_sync(0xffffffffu, s, 2);
-        s += __shfl_xor_sync(0xffffffffu, s, 4);
-        if (on && key >= vis[r].x && key < vis[r].y) {
-          float x;
-          if (a.softcap > 0.f) x = a.softcap * tanhf(s * a.scale / a.softcap);
-          else x = s * a.scale;
-          x = fmaf(slope[r], (float)(key - qpos[r]), x) * kLog2e;
-          // (a score of -inf, an overflow, leaves the row as it is)
-          if (x > m[r]) {
-            const float f = m[r] == -INFINITY ? 0.f : exp2f(m[r] - x);
-            l[r] *= f;
+          for (int i = 0; i < DPL; ++i) s = fmaf(q[r][i], kx[u][i], s);
+          s += __shfl_xor_sync(0xffffffffu, s, 1);
+          s += __shfl_xor_sync(0xffffffffu, s, 2);
+          s += __shfl_xor_sync(0xffffffffu, s, 4);
+          if (on[u] && key >= vis[r].x && key < vis[r].y) {
+            float x;
+            if (a.softcap > 0.f) x = a.softcap * tanhf(s * a.scale / a.softcap);
+            else x = s * a.scale;
+            x = fmaf(slope[r], (float)(key - qpos[r]), x) * kLog2e;
+            // (a score of -inf, an overflow, leaves the row as it is)
+            if (x > m[r]) {
+              const float f = m[r] == -INFINITY ? 0.f : exp2f(m[r] - x);
+              l[r] *= f;
 #pragma unroll
-            for (int i = 0; i < DPL; ++i) o[r][i] *= f;
-            m[r] = x;
+              for (int i = 0; i < DPL; ++i) o[r][i] *= f;
+              m[r] = x;
+            }
+            const float p = x == -INFINITY ? 0.f : exp2f(x - m[r]);
+            l[r] += p;
+#pragma unroll
+            for (int i = 0; i < DPL; ++i) o[r][i] = fmaf(p, vx[u][i], o[r][i]);
           }
-          const float p = x == -INFINITY ? 0.f : exp2f(x - m[r]);
-          l[r] += p;
-#pragma unroll
-          for (int i = 0; i < DPL; ++i) o[r][i] = fmaf(p, vx[i], o[r][i]);
         }
       }
     }
@@ -216,71 +232,99 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
       }
     }
     __syncthreads();
-    at += a.split ? t1 - t0 : 1;
+    at = unit_begin + per;
   }
 }
 
 // One block joins one row of one unit that was cut between runs: the block of
-// the unit's first cut does it, the others return. The maximum first, then
-// the weighted sums, eight runs at a time (a single long request on one KV
-// head leaves as many partial rows as there are runs); the order is fixed.
+// the unit's first cut does it, the others return. A single long request on
+// one KV head leaves as many partial rows as there are runs, so eight warps
+// share them; the order is fixed.
 constexpr int kJoinWarps = 8;
 __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const PagedArgs a) {
   __shared__ float sm_o[kJoinWarps][256];
-  __shared__ float sm_l[kJoinWarps];
+  __shared__ float sm_m[kJoinWarps], sm_l[kJoinWarps];
   grid_dep_wait();
   grid_dep_launch_dependents();
   const int b = blockIdx.x + 1, r = blockIdx.y;
   const RunMeta mt = a.meta[b];
   if (mt.n_runs == 0 || r >= mt.rows || mt.begin == mt.unit_begin) return;
+  // Run b - 1 begins in the unit's tiles too: its block joins the unit.
   const long long prev = mt.total * (b - 1) / mt.n_runs;
-  if (prev > mt.unit_begin) return;
+  if (prev - mt.unit_begin > kUnitCost) return;
   const int first = b - 1;
-  int last = b;  // one past the last run with tiles of the unit
-  while (last < mt.n_runs && mt.total * last / mt.n_runs < mt.unit_end) ++last;
+  // One past the last run that begins before the unit's end:
+  // floor(total j / n) < e for all j < e n / total.
+  const int last = (int)min((long long)mt.n_runs, (mt.unit_end * mt.n_runs + mt.total - 1) / mt.total);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int sd = (a.D + 3) & ~3;
   auto row_of = [&](int run) {
-    const int slot = run * 2 + ((run == first && prev != mt.unit_begin) ? 1 : 0);
+    const int slot = run * 2 + ((run == first && prev < mt.unit_begin) ? 1 : 0);
     return (int64_t)slot * a.rows_per_unit + r;
   };
-  float top = -INFINITY;
-  for (int j = first + lane; j < last; j += 32) top = fmaxf(top, a.slot_ml[row_of(j)].x);
+  // Each warp joins every eighth run, four of them in flight.
+  float top = -INFINITY, acc[2][4] = {}, l = 0.f;
+  for (int j0 = first + warp; j0 < last; j0 += 4 * kJoinWarps) {
+    float2 ml[4];
+    float4 x[4][2];
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-  float acc[2][4] = {}, l = 0.f;
-#pragma unroll 4
-  for (int j = first + warp; j < last; j += kJoinWarps) {
-    const int64_t sr = row_of(j);
-    const float2 ml = a.slot_ml[sr];
-    const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
-    l = fmaf(f, ml.y, l);
+    for (int i = 0; i < 4; ++i) {
+      const int j = j0 + i * kJoinWarps;
+      ml[i] = make_float2(-INFINITY, 0.f);
+      if (j < last) {
+        const int64_t sr = row_of(j);
+        ml[i] = a.slot_ml[sr];
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int col = c * 128 + lane * 4;
-      if (col < a.D) {
-        const float4 x = *reinterpret_cast<const float4*>(a.slot_o + sr * sd + col);
-        acc[c][0] = fmaf(f, x.x, acc[c][0]);
-        acc[c][1] = fmaf(f, x.y, acc[c][1]);
-        acc[c][2] = fmaf(f, x.z, acc[c][2]);
-        acc[c][3] = fmaf(f, x.w, acc[c][3]);
+        for (int c = 0; c < 2; ++c)
+          if (c * 128 + lane * 4 < a.D) x[i][c] = *reinterpret_cast<const float4*>(a.slot_o + sr * sd + c * 128 + lane * 4);
       }
+    }
+    float nt = top;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) nt = fmaxf(nt, ml[i].x);
+    const float g = top == -INFINITY ? 0.f : exp2f(top - nt);
+    top = nt;
+    l *= g;
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[c][k] *= g;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (ml[i].x == -INFINITY) continue;
+      const float f = exp2f(ml[i].x - top);
+      l = fmaf(f, ml[i].y, l);
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        if (c * 128 + lane * 4 < a.D) {
+          acc[c][0] = fmaf(f, x[i][c].x, acc[c][0]);
+          acc[c][1] = fmaf(f, x[i][c].y, acc[c][1]);
+          acc[c][2] = fmaf(f, x[i][c].z, acc[c][2]);
+          acc[c][3] = fmaf(f, x[i][c].w, acc[c][3]);
+        }
     }
   }
 #pragma unroll
   for (int c = 0; c < 2; ++c)
 #pragma unroll
     for (int i = 0; i < 4; ++i) sm_o[warp][c * 128 + lane * 4 + i] = acc[c][i];
-  if (lane == 0) sm_l[warp] = l;
+  if (lane == 0) {
+    sm_m[warp] = top;
+    sm_l[warp] = l;
+  }
   __syncthreads();
   const int col = threadIdx.x * 4;
   if (col >= a.D) return;
+  top = sm_m[0];
+#pragma unroll
+  for (int w = 1; w < kJoinWarps; ++w) top = fmaxf(top, sm_m[w]);
   float x[4] = {0.f, 0.f, 0.f, 0.f}, ls = 0.f;
 #pragma unroll
   for (int w = 0; w < kJoinWarps; ++w) {
-    ls += sm_l[w];
+    const float f = sm_m[w] == -INFINITY ? 0.f : exp2f(sm_m[w] - top);
+    ls = fmaf(f, sm_l[w], ls);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] += sm_o[w][col + i];
+    for (int i = 0; i < 4; ++i) x[i] = fmaf(f, sm_o[w][col + i], x[i]);
   }
   const int row = mt.row0 + r;
   finish_row4(a, mt.q0 + row / a.group, mt.hk * a.group + row % a.group, col, x, top, ls);
