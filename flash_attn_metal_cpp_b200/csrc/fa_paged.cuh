@@ -55,6 +55,10 @@ struct ReqView {
   __device__ __forceinline__ long long work(const PagedArgs& a) const { return (long long)units * per_unit(a); }
 };
 
+// Lengths and tables are read past L1: PagedArgs::late_wait lets a kernel read
+// them before it has waited for the kernel in front of it.
+__device__ __forceinline__ int ld_index(const int* p) { return __ldcg(p); }
+
 // Lengths outside the table and query ranges outside q are clipped (and noted
 // in the status word): a wrong length gives a wrong row, never a wrong access.
 template <int TN>
@@ -62,7 +66,7 @@ __device__ __forceinline__ ReqView view_request(const PagedArgs& a, int i, int r
   ReqView r;
   bool bad = false;
   if (a.cu_q != nullptr) {
-    int b = a.cu_q[i], e = a.cu_q[i + 1];
+    const int b = ld_index(a.cu_q + i), e = ld_index(a.cu_q + i + 1);
     const int b0 = min(max(b, 0), a.total_q), e0 = min(max(e, b0), a.total_q);
     bad = b0 != b || e0 != e;
     r.q0 = b0;
@@ -71,7 +75,7 @@ __device__ __forceinline__ ReqView view_request(const PagedArgs& a, int i, int r
     r.q0 = i;
     r.qlen = i < a.total_q ? 1 : 0;
   }
-  const int len = a.seq_lens[i];
+  const int len = ld_index(a.seq_lens + i);
   const int cap = (int)min((long long)a.max_pages * a.page_size, (long long)0x3fffffff);
   const int own = min(max(len, 0), cap);
   bad |= own != len;
@@ -93,15 +97,17 @@ struct Run {
   int n_runs;
   int req;                 // request the run begins in
   long long req_begin;     // where that request begins
+  ReqView view;            // of that request
 };
 
 // Sums up the line and finds the block's run. Every thread of the block calls
 // it; `sh` is shared scratch. A run has at least `min_run` of the line:
 // shorter runs cost more in joining than they save.
 struct RunScratch {
-  long long part[32];
+  long long part[8];
   long long req_begin[2], cut[2];
   int req[2];
+  ReqView view;
 };
 template <int TN, int NTHREADS>
 __device__ __forceinline__ Run find_run(const PagedArgs& a, int rows_per_unit, int block, int n_blocks, int min_run,
@@ -111,7 +117,12 @@ __device__ __forceinline__ Run find_run(const PagedArgs& a, int rows_per_unit, i
   const int seg = (a.B + NTHREADS - 1) / NTHREADS;
   const int i0 = min(tid * seg, a.B), i1 = min(i0 + seg, a.B);
   long long sum = 0;
-  for (int i = i0; i < i1; ++i) sum += view_request<TN>(a, i, rows_per_unit).work(a);
+  ReqView mine;  // the first of this thread's requests (mostly its only one)
+  for (int i = i0; i < i1; ++i) {
+    const ReqView v = view_request<TN>(a, i, rows_per_unit);
+    if (i == i0) mine = v;
+    sum += v.work(a);
+  }
   long long inc = sum;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
@@ -139,9 +150,10 @@ __device__ __forceinline__ Run find_run(const PagedArgs& a, int rows_per_unit, i
     if (sum > 0 && cut >= at && cut < at + sum) {
       long long b = at;
       for (int i = i0; i < i1; ++i) {
-        const ReqView v = view_request<TN>(a, i, rows_per_unit);
+        const ReqView v = i == i0 ? mine : view_request<TN>(a, i, rows_per_unit);
         const long long w = v.work(a);
         if (cut < b + w) {
+          if (e == 0) sh->view = v;
           const long long unit_begin = b + (cut - b) / v.per_unit(a) * v.per_unit(a);
           sh->req[e] = i;
           sh->req_begin[e] = b;
@@ -155,6 +167,7 @@ __device__ __forceinline__ Run find_run(const PagedArgs& a, int rows_per_unit, i
   __syncthreads();
   r.req = sh->req[0];
   r.req_begin = sh->req_begin[0];
+  r.view = sh->view;
   r.begin = sh->cut[0];
   r.end = sh->req[1] >= 0 ? sh->cut[1] : total;
   return r;
@@ -171,7 +184,7 @@ __device__ __forceinline__ int2 find_key(const PagedArgs& a, int req, int key) {
   const int p = own / a.page_size;
   const int slot = own - p * a.page_size;
   const int* entry = shared ? a.pre_table + p : a.table + (int64_t)req * a.table_stride + p;
-  return make_int2(*entry, slot);
+  return make_int2(ld_index(entry), slot);
 }
 
 // The page, or -1 (and a note) when the table names none of the cache's.

@@ -103,6 +103,7 @@ struct PagedArgs {
   int own_part;            // part that the few-rows and CUDA-core kernels write (-1: the output)
   float* parts_o;
   float* parts_lse;
+  int late_wait;           // few-rows kernel: wait for the kernel in front only before ending
   // Work that the kernels cut in n_ctas equal runs (split = 1, fa_paged.cuh):
   // per run two partial units of rows_per_unit rows, and where they belong.
   int split;

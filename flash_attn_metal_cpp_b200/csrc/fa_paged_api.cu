@@ -447,6 +447,7 @@ fa_status fa_paged_forward(const fa_paged_params* p, const void* q, const void* 
     a.min_run = h.tensor || a.D <= 64 ? 3 : 4;
     a.split = h.split;
     place_cut(a, h.cut, workspace);
+    a.late_wait = h.shared;
     st = h.tensor ? cuda_status(launch_paged_decode(a, c.dtype, s), "paged attention (few rows)")
                   : cuda_status(launch_paged_simt(a, c.dtype, vec, s), "paged attention (CUDA cores)");
     if (st == FA_OK && a.split) st = cuda_status(launch_paged_join(a, s), "paged attention (join)");

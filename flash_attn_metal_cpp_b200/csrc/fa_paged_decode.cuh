@@ -121,7 +121,7 @@ struct Cursor {
     run_first = true;
     if (run.end <= run.begin) return;
     req = run.req;
-    v = view_request<kTile>(a, req, MR);
+    v = run.view;
     per = v.per_unit(a);
     const long long off = run.begin - run.req_begin;
     unit = (int)(off / per);
@@ -182,11 +182,18 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
   const T* K = reinterpret_cast<const T*>(a.k);
   const T* V = reinterpret_cast<const T*>(a.v);
 
-  grid_dep_wait();
+  // With late_wait the kernel in front is the shared prefix's: this one needs
+  // nothing of it and may run beside it, on the SMs it leaves free. All blocks
+  // of that kernel have waited for everything before it by the time they let
+  // this one start, so lengths, tables and caches are complete (and read from
+  // L2); waiting at the end instead keeps "this kernel is done" meaning "that
+  // one is done too" for the join that follows.
+  if (!a.late_wait) grid_dep_wait();
   grid_dep_launch_dependents();
   const Run run = find_run<kTile, kThreads>(a, MR, blockIdx.x, gridDim.x, a.min_run, &sh.scratch);
   if (run.end <= run.begin) {
     if (a.split && tid == 0) a.meta[blockIdx.x].n_runs = 0;
+    if (a.late_wait) grid_dep_wait();
     return;
   }
   Cursor<MR> cur;
@@ -508,6 +515,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
     st = st == NS - 1 ? 0 : st + 1;
   }
   cp_async_wait<0>();
+  if (a.late_wait) grid_dep_wait();
 }
 
 template <typename T, int DM, int MT>

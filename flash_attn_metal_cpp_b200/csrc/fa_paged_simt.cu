@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
 
   int req = run.req;
   long long req_begin = run.req_begin;
-  ReqView v = view_request<kTile>(a, req, R);
+  ReqView v = run.view;
   long long at = run.begin;
   while (at < run.end) {
     const int per = v.per_unit(a);
@@ -331,57 +331,84 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const Paged
 }
 
 // Join of whole-row partial results: LSE = log sum_p exp(lse_p),
-// o = sum_p exp(lse_p - LSE) o_p. One warp a row; the lanes first take one
-// part's lse each, then 4 columns each of all parts, several parts in flight.
+// o = sum_p exp(lse_p - LSE) o_p. W warps of the block's eight share a row's
+// parts, so that the loads of a row are all in flight however many they are;
+// a lane takes 4 columns (the kernels that write parts have head_dim <= 128).
+template <int W>
 __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedArgs a) {
+  constexpr int R = 8 / W;  // rows a block
+  __shared__ float sm_o[8][128];
+  __shared__ float sm_m[8], sm_l[8];
   grid_dep_wait();
   grid_dep_launch_dependents();
-  const int lane = threadIdx.x & 31;
-  const int64_t row = blockIdx.x * 8ll + (threadIdx.x >> 5);  // token * Hq + head
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t rows = (int64_t)a.total_q * a.Hq;
-  if (row >= rows) return;
+  const int64_t row = blockIdx.x * (int64_t)R + warp / W;  // token * Hq + head
   const int tok = (int)(row / a.Hq), head = (int)(row - (int64_t)tok * a.Hq);
-  const int last = a.cu_q ? min(max(a.cu_q[a.B], 0), a.total_q) : min(a.B, a.total_q);
   const int first = a.cu_q ? min(max(a.cu_q[0], 0), a.total_q) : 0;
-  if (tok < first || tok >= last) return;  // of no sequence
-  float top = -INFINITY;
-  for (int p = lane; p < a.n_parts; p += 32) top = fmaxf(top, a.parts_lse[p * rows + row]);
+  const int last = a.cu_q ? min(max(a.cu_q[a.B], 0), a.total_q) : min(a.B, a.total_q);
+  const bool on = row < rows && tok >= first && tok < last;  // else the row is of no sequence
+  const int col = lane * 4;
+  float x[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f, top = -INFINITY;
+  if (on) {
+    for (int p0 = warp % W; p0 < a.n_parts; p0 += 4 * W) {
+      float lse[4];
+      float4 y[4];
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-  const float sub = top == -INFINITY ? 0.f : top;
-  float x[2][4] = {}, l = 0.f;
-  for (int p0 = 0; p0 < a.n_parts; p0 += 32) {
-    const int n = min(32, a.n_parts - p0);
-    float w = 0.f;
-    if (lane < n) w = expf(a.parts_lse[(p0 + lane) * rows + row] - sub);
-#pragma unroll 4
-    for (int p = 0; p < n; ++p) {
-      const float f = __shfl_sync(0xffffffffu, w, p);
-      l += f;
-      const float* src = a.parts_o + ((p0 + p) * rows + row) * a.D;
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int col = c * 128 + lane * 4;
-        if (col < a.D) {
-          const float4 y = *reinterpret_cast<const float4*>(src + col);
-          x[c][0] = fmaf(f, y.x, x[c][0]);
-          x[c][1] = fmaf(f, y.y, x[c][1]);
-          x[c][2] = fmaf(f, y.z, x[c][2]);
-          x[c][3] = fmaf(f, y.w, x[c][3]);
+      for (int i = 0; i < 4; ++i) {
+        const int p = p0 + i * W;
+        lse[i] = -INFINITY;
+        y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (p < a.n_parts) {
+          lse[i] = a.parts_lse[p * rows + row] * kLog2e;
+          if (col < a.D) y[i] = *reinterpret_cast<const float4*>(a.parts_o + (p * rows + row) * a.D + col);
         }
+      }
+      const float nt = fmaxf(top, fmaxf(fmaxf(lse[0], lse[1]), fmaxf(lse[2], lse[3])));
+      const float sub = nt == -INFINITY ? 0.f : nt;
+      const float g = exp2f(top - sub);
+      top = nt;
+      l *= g;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] *= g;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float f = exp2f(lse[i] - sub);
+        l += f;
+        x[0] = fmaf(f, y[i].x, x[0]);
+        x[1] = fmaf(f, y[i].y, x[1]);
+        x[2] = fmaf(f, y[i].z, x[2]);
+        x[3] = fmaf(f, y[i].w, x[3]);
       }
     }
   }
+  if constexpr (W > 1) {
+    *reinterpret_cast<float4*>(&sm_o[warp][col]) = make_float4(x[0], x[1], x[2], x[3]);
+    if (lane == 0) {
+      sm_m[warp] = top;
+      sm_l[warp] = l;
+    }
+    __syncthreads();
+    if (warp % W != 0) return;
+#pragma unroll
+    for (int w = 1; w < W; ++w) {
+      const float mw = sm_m[warp + w];
+      const float nt = fmaxf(top, mw);
+      const float sub = nt == -INFINITY ? 0.f : nt;
+      const float g = exp2f(top - sub), f = exp2f(mw - sub);
+      top = nt;
+      l = l * g + f * sm_l[warp + w];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] = x[k] * g + f * sm_o[warp + w][col + k];
+    }
+  }
+  if (!on) return;
   const float inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    const int col = c * 128 + lane * 4;
-    if (col >= a.D) continue;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[c][i] *= inv;
-    store_out4(a.o, (int64_t)tok * a.o_st + (int64_t)head * a.o_sh + col, a.out_dtype, x[c], 4);
-  }
-  if (lane == 0 && a.lse != nullptr) a.lse[(int64_t)head * a.total_q + tok] = l > 0.f ? sub + logf(l) : -INFINITY;
+  for (int k = 0; k < 4; ++k) x[k] *= inv;
+  if (col < a.D) store_out4(a.o, (int64_t)tok * a.o_st + (int64_t)head * a.o_sh + col, a.out_dtype, x, 4);
+  if (lane == 0 && a.lse != nullptr)
+    a.lse[(int64_t)head * a.total_q + tok] = l > 0.f ? top * kLn2 + logf(l) : -INFINITY;
 }
 
 template <typename T, int DM, int R, bool VEC>
@@ -426,9 +453,10 @@ cudaError_t launch_paged_simt(const PagedArgs& a, int dtype, bool vec, cudaStrea
 }
 
 cudaError_t launch_paged_merge(const PagedArgs& a, cudaStream_t st) {
-  const long long blocks = ((long long)a.total_q * a.Hq + 7) / 8;
+  const bool wide = a.n_parts > 4;
+  const long long rows = (long long)a.total_q * a.Hq, blocks = wide ? rows : (rows + 7) / 8;
   if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
-  cudaError_t e = launch_pdl(paged_merge_kernel, dim3((unsigned)blocks), dim3(256), 0, st, a);
+  cudaError_t e = launch_pdl(wide ? paged_merge_kernel<8> : paged_merge_kernel<1>, dim3((unsigned)blocks), dim3(256), 0, st, a);
   note_launch();
   return e;
 }

@@ -115,76 +115,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const unsigned long long wlim = a.wait_limit_ns ? a.wait_limit_ns : kWaitLimitNs;
 
-  grid_dep_wait();
-  grid_dep_launch_dependents();
-
-  // ------------------------------------------------------------ work item
-  // Blocks of a request's rows stand in one line over the requests, the last
-  // ones first (under a causal mask they have the most keys); within a block
-  // the KV heads, within a head the parts of the keys.
-  const int split = blockIdx.x % tc.n_split;
-  const int hk = blockIdx.x / tc.n_split % a.Hk;
-  const int bi = blockIdx.x / tc.n_split / a.Hk;
-  Block b;
-  if (tc.shared) {
-    const int last = a.cu_q ? min(max(a.cu_q[a.B], 0), a.total_q) : min(a.B, a.total_q);
-    b.req = -1;
-    b.q0 = 0;
-    b.qlen = last;
-    b.klen = a.pre;
-    b.rows = last * a.group;
-    b.row0 = bi * NT * BM;
-    if (b.row0 >= b.rows) return;
-    if (a.win_left >= 0) {
-      // The window may leave most of the prefix unseen: the earliest query of
-      // the batch says how much.
-      int ahead = 0x7fffffff;
-      for (int i = threadIdx.x; i < a.B; i += kThreads) {
-        const ReqView v = view_request<BN>(a, i, BM);
-        if (v.qlen > 0) ahead = min(ahead, v.klen - v.qlen);
-      }
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1) ahead = min(ahead, __shfl_xor_sync(0xffffffffu, ahead, off));
-      if (lane == 0) bars->part[warp] = ahead;
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        for (int w = 1; w < kThreads / 32; ++w) ahead = min(ahead, bars->part[w]);
-        bars->min_ahead = ahead;
-      }
-    }
-  } else {
-    const int seg = (a.B + kThreads - 1) / kThreads;
-    const int i0 = min((int)threadIdx.x * seg, a.B), i1 = min(i0 + seg, a.B);
-    int n = 0;
-    for (int i = i0; i < i1; ++i)
-      n += (int)(((long long)view_request<BN>(a, i, BM).qlen * a.group + NT * BM - 1) / (NT * BM));
-    if (threadIdx.x == 0) bars->req = -1;
-    int total;
-    int at = scan_block(n, bars->part, &total);
-    const int want = total - 1 - bi;
-    if (want < 0) return;
-    if (want >= at && want < at + n) {
-      for (int i = i0; i < i1; ++i) {
-        const int nb = (int)(((long long)view_request<BN>(a, i, BM).qlen * a.group + NT * BM - 1) / (NT * BM));
-        if (want < at + nb) {
-          bars->req = i;
-          bars->blk = want - at;
-          break;
-        }
-        at += nb;
-      }
-    }
-    __syncthreads();
-    b.req = bars->req;
-    const ReqView v = view_request<BN>(a, b.req, BM);
-    b.q0 = v.q0;
-    b.qlen = v.qlen;
-    b.klen = v.klen;
-    b.rows = v.qlen * a.group;
-    b.row0 = bars->blk * NT * BM;
-  }
-
+  // Set-up that touches no global memory overlaps the end of the kernel in front.
   if (threadIdx.x == kKWarp * 32) {
+    prefetch_tmap(&tm_k);
+    prefetch_tmap(&tm_v);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       mbar_init(smem_addr(&bars->q_full[t]), 4);
@@ -213,6 +147,85 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
   volatile int* abort_flag = &bars->abort_flag;
+  auto leave = [&]() {  // a block without work
+    if (warp == kMmaWarp) tmem_dealloc(tmem, kTmemCols);
+  };
+  grid_dep_wait();
+  grid_dep_launch_dependents();
+
+  // ------------------------------------------------------------ work item
+  // Blocks of a request's rows stand in one line over the requests, the last
+  // ones first (under a causal mask they have the most keys); within a block
+  // the KV heads, within a head the parts of the keys.
+  const int split = blockIdx.x % tc.n_split;
+  const int hk = blockIdx.x / tc.n_split % a.Hk;
+  const int bi = blockIdx.x / tc.n_split / a.Hk;
+  Block b;
+  if (tc.shared) {
+    const int last = a.cu_q ? min(max(a.cu_q[a.B], 0), a.total_q) : min(a.B, a.total_q);
+    b.req = -1;
+    b.q0 = 0;
+    b.qlen = last;
+    b.klen = a.pre;
+    b.rows = last * a.group;
+    b.row0 = bi * NT * BM;
+    if (b.row0 >= b.rows) {
+      leave();
+      return;
+    }
+    if (a.win_left >= 0) {
+      // The window may leave most of the prefix unseen: the earliest query of
+      // the batch says how much.
+      int ahead = 0x7fffffff;
+      for (int i = threadIdx.x; i < a.B; i += kThreads) {
+        const ReqView v = view_request<BN>(a, i, BM);
+        if (v.qlen > 0) ahead = min(ahead, v.klen - v.qlen);
+      }
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) ahead = min(ahead, __shfl_xor_sync(0xffffffffu, ahead, off));
+      if (lane == 0) bars->part[warp] = ahead;
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        for (int w = 1; w < kThreads / 32; ++w) ahead = min(ahead, bars->part[w]);
+        bars->min_ahead = ahead;
+      }
+    }
+  } else {
+    const int seg = (a.B + kThreads - 1) / kThreads;
+    const int i0 = min((int)threadIdx.x * seg, a.B), i1 = min(i0 + seg, a.B);
+    int n = 0;
+    for (int i = i0; i < i1; ++i)
+      n += (int)(((long long)view_request<BN>(a, i, BM).qlen * a.group + NT * BM - 1) / (NT * BM));
+    if (threadIdx.x == 0) bars->req = -1;
+    int total;
+    int at = scan_block(n, bars->part, &total);
+    const int want = total - 1 - bi;
+    if (want < 0) {
+      leave();
+      return;
+    }
+    if (want >= at && want < at + n) {
+      for (int i = i0; i < i1; ++i) {
+        const int nb = (int)(((long long)view_request<BN>(a, i, BM).qlen * a.group + NT * BM - 1) / (NT * BM));
+        if (want < at + nb) {
+          bars->req = i;
+          bars->blk = want - at;
+          break;
+        }
+        at += nb;
+      }
+    }
+    __syncthreads();
+    b.req = bars->req;
+    const ReqView v = view_request<BN>(a, b.req, BM);
+    b.q0 = v.q0;
+    b.qlen = v.qlen;
+    b.klen = v.klen;
+    b.rows = v.qlen * a.group;
+    b.row0 = bars->blk * NT * BM;
+  }
+
+  if (tc.shared && a.win_left >= 0) __syncthreads();  // min_ahead
 
   // Key tiles of each row tile (absolute, in tiles of 128 keys), then the
   // part of them that this split takes. All threads compute the same.
@@ -270,7 +283,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint64_t* full = is_k ? bars->k_full : bars->v_full;
       uint64_t* empty = is_k ? bars->k_empty : bars->v_empty;
       const uint32_t raw = smem_addr(&bars->v_raw);
-      if (lane == 0) prefetch_tmap(tm);
       const int box = tc.box_rows, boxes = BN / box;
       const int* table = tc.shared ? a.pre_table : a.table + (int64_t)b.req * a.table_stride;
       // Page of this lane's box in tile j (-1: nothing to load).
