@@ -43,6 +43,13 @@ __device__ __forceinline__ float cvt_in<__nv_bfloat16>(__nv_bfloat16 x) { return
 // 64 to 32769 tokens: 262 us, 297 us without).
 constexpr int kUnitCost = 2;
 
+// 64-bit quotient of non-negative numbers; a 64-bit division takes some 300
+// cycles, and almost every call's numbers fit 32 bits.
+__device__ __forceinline__ long long div_ll(long long x, long long y) {
+  if (((x | y) >> 32) == 0) return (unsigned)x / (unsigned)y;
+  return x / y;
+}
+
 // One request: its query rows, its keys, and the key tiles any of its rows sees.
 struct ReqView {
   int q0, qlen;      // query tokens
@@ -85,7 +92,7 @@ __device__ __forceinline__ ReqView view_request(const PagedArgs& a, int i, int r
   r.key_lo = min(r.key_lo, r.klen);
   r.tile_lo = r.key_lo / TN;
   r.tiles = max(1, (r.klen + TN - 1) / TN - r.tile_lo);  // a row without keys is still written
-  const int chunks = (int)(((long long)r.qlen * a.group + rows_per_unit - 1) / rows_per_unit);
+  const int chunks = (int)(((unsigned)r.qlen * (unsigned)a.group + rows_per_unit - 1u) / (unsigned)rows_per_unit);
   r.units = chunks * a.Hk;
   return r;
 }
@@ -140,13 +147,13 @@ __device__ __forceinline__ Run find_run(const PagedArgs& a, int rows_per_unit, i
   }
   Run r;
   r.total = total;
-  r.n_runs = (int)min((long long)n_blocks, max(1ll, total / (a.split ? min_run : 1)));
+  r.n_runs = (int)min((long long)n_blocks, max(1ll, div_ll(total, a.split ? min_run : 1)));
   r.begin = r.end = 0;
   if (total == 0 || block >= r.n_runs) return r;
   const long long at = before + inc - sum;
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
-    const long long cut = total * (block + e) / r.n_runs;
+    const long long cut = div_ll(total * (block + e), r.n_runs);
     if (sum > 0 && cut >= at && cut < at + sum) {
       long long b = at;
       for (int i = i0; i < i1; ++i) {
@@ -154,7 +161,7 @@ __device__ __forceinline__ Run find_run(const PagedArgs& a, int rows_per_unit, i
         const long long w = v.work(a);
         if (cut < b + w) {
           if (e == 0) sh->view = v;
-          const long long unit_begin = b + (cut - b) / v.per_unit(a) * v.per_unit(a);
+          const long long unit_begin = b + div_ll(cut - b, v.per_unit(a)) * v.per_unit(a);
           sh->req[e] = i;
           sh->req_begin[e] = b;
           sh->cut[e] = cut - unit_begin <= kUnitCost ? unit_begin : cut;
@@ -181,7 +188,7 @@ __device__ __forceinline__ int tile_at(long long off) { return off <= kUnitCost 
 __device__ __forceinline__ int2 find_key(const PagedArgs& a, int req, int key) {
   const bool shared = key < a.pre;
   const int own = shared ? key : key - a.pre;
-  const int p = own / a.page_size;
+  const int p = (unsigned)own / (unsigned)a.page_size;
   const int slot = own - p * a.page_size;
   const int* entry = shared ? a.pre_table + p : a.table + (int64_t)req * a.table_stride + p;
   return make_int2(ld_index(entry), slot);

@@ -150,6 +150,7 @@ struct PagedTc {
   int box_rows;      // slots of one TMA box
   int partial;       // 1: normalised partial results to part0 + split
   int part0;
+  int out_vec;       // output rows start at 16-byte boundaries
 };
 cudaError_t launch_paged_tc_d64_f16(const PagedArgs&, const PagedTc&, const CUtensorMap&, const CUtensorMap&, cudaStream_t);
 cudaError_t launch_paged_tc_d64_bf16(const PagedArgs&, const PagedTc&, const CUtensorMap&, const CUtensorMap&, cudaStream_t);

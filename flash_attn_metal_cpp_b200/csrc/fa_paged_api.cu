@@ -413,6 +413,8 @@ fa_status fa_paged_forward(const fa_paged_params* p, const void* q, const void* 
   CUtensorMap tk, tv;
   PagedTc t{};
   t.box_rows = h.box;
+  const int64_t om = 16 / (int64_t)elem_size(a.out_dtype);
+  t.out_vec = aligned(o, 16) && a.o_st % om == 0 && a.o_sh % om == 0;
   if (h.shared || h.many) {
     const bool bf = c.dtype == kBF16;
     st = paged_encode(&tk, k_cache, bf, a.D, a.Hk, a.page_size, a.num_pages, a.k_sp, a.k_ss, a.k_sh, h.box);

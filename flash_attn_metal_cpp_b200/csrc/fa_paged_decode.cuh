@@ -124,7 +124,7 @@ struct Cursor {
     v = run.view;
     per = v.per_unit(a);
     const long long off = run.begin - run.req_begin;
-    unit = (int)(off / per);
+    unit = (int)div_ll(off, per);
     const long long in_unit = off - (long long)unit * per;
     left = run.end - run.begin + in_unit;
     hk = unit % a.Hk;

@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
       v = view_request<kTile>(a, ++req, R);
       continue;
     }
-    const int unit = (int)(off / per);
+    const int unit = (int)div_ll(off, per);
     const long long unit_begin = req_begin + (long long)unit * per;
     const int t_end = v.tile_lo + v.tiles;
     const int t0 = v.tile_lo + (a.split ? tile_at(at - unit_begin) : 0);
@@ -250,12 +250,12 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const Paged
   const RunMeta mt = a.meta[b];
   if (mt.n_runs == 0 || r >= mt.rows || mt.begin == mt.unit_begin) return;
   // Run b - 1 begins in the unit's tiles too: its block joins the unit.
-  const long long prev = mt.total * (b - 1) / mt.n_runs;
+  const long long prev = div_ll(mt.total * (b - 1), mt.n_runs);
   if (prev - mt.unit_begin > kUnitCost) return;
   const int first = b - 1;
   // One past the last run that begins before the unit's end:
   // floor(total j / n) < e for all j < e n / total.
-  const int last = (int)min((long long)mt.n_runs, (mt.unit_end * mt.n_runs + mt.total - 1) / mt.total);
+  const int last = (int)min((long long)mt.n_runs, div_ll(mt.unit_end * mt.n_runs + mt.total - 1, mt.total));
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int sd = (a.D + 3) & ~3;
   auto row_of = [&](int run) {

@@ -55,6 +55,13 @@ struct Cfg {
   static constexpr int SMEM_BYTES = OFF_BAR + 1024 + 1024;  // barriers and scratch, alignment slack
 };
 
+// Which rows and keys the block works on.
+struct Block {
+  int q0, qlen, klen;   // query tokens and keys of its request (shared prefix: all tokens, the prefix)
+  int req;
+  int row0, rows;       // packed rows [row0, min(row0 + 256, rows))
+};
+
 struct Bars {
   uint64_t q_full[NT], s_full[NT], p_full[NT][2], o_full[NT];
   uint64_t mma_final, v_raw;
@@ -63,16 +70,10 @@ struct Bars {
   int abort_flag;
   // block search
   int part[kThreads / 32];
-  int req, blk, min_ahead;
+  int min_ahead;
+  Block work;
 };
 static_assert(sizeof(Bars) <= 1024, "barrier space");
-
-// Which rows and keys the block works on.
-struct Block {
-  int q0, qlen, klen;   // query tokens and keys of its request (shared prefix: all tokens, the prefix)
-  int req;
-  int row0, rows;       // packed rows [row0, min(row0 + 256, rows))
-};
 
 template <typename T>
 __device__ __forceinline__ uint32_t pack_p(float lo, float hi) {
@@ -157,9 +158,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   // Blocks of a request's rows stand in one line over the requests, the last
   // ones first (under a causal mask they have the most keys); within a block
   // the KV heads, within a head the parts of the keys.
-  const int split = blockIdx.x % tc.n_split;
-  const int hk = blockIdx.x / tc.n_split % a.Hk;
-  const int bi = blockIdx.x / tc.n_split / a.Hk;
+  const unsigned per_split = blockIdx.x / (unsigned)tc.n_split;
+  const int split = blockIdx.x - per_split * tc.n_split;
+  const int bi = per_split / (unsigned)a.Hk;
+  const int hk = per_split - bi * a.Hk;
   Block b;
   if (tc.shared) {
     const int last = a.cu_q ? min(max(a.cu_q[a.B], 0), a.total_q) : min(a.B, a.total_q);
@@ -193,10 +195,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     const int seg = (a.B + kThreads - 1) / kThreads;
     const int i0 = min((int)threadIdx.x * seg, a.B), i1 = min(i0 + seg, a.B);
+    auto blocks_of = [&](const ReqView& v) { return (v.qlen * a.group + NT * BM - 1) / (NT * BM); };
+    ReqView mine;  // the first of this thread's requests (mostly its only one)
     int n = 0;
-    for (int i = i0; i < i1; ++i)
-      n += (int)(((long long)view_request<BN>(a, i, BM).qlen * a.group + NT * BM - 1) / (NT * BM));
-    if (threadIdx.x == 0) bars->req = -1;
+    for (int i = i0; i < i1; ++i) {
+      const ReqView v = view_request<BN>(a, i, BM);
+      if (i == i0) mine = v;
+      n += blocks_of(v);
+    }
     int total;
     int at = scan_block(n, bars->part, &total);
     const int want = total - 1 - bi;
@@ -206,23 +212,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (want >= at && want < at + n) {
       for (int i = i0; i < i1; ++i) {
-        const int nb = (int)(((long long)view_request<BN>(a, i, BM).qlen * a.group + NT * BM - 1) / (NT * BM));
+        const ReqView v = i == i0 ? mine : view_request<BN>(a, i, BM);
+        const int nb = blocks_of(v);
         if (want < at + nb) {
-          bars->req = i;
-          bars->blk = want - at;
+          bars->work = Block{v.q0, v.qlen, v.klen, i, (want - at) * NT * BM, v.qlen * a.group};
           break;
         }
         at += nb;
       }
     }
     __syncthreads();
-    b.req = bars->req;
-    const ReqView v = view_request<BN>(a, b.req, BM);
-    b.q0 = v.q0;
-    b.qlen = v.qlen;
-    b.klen = v.klen;
-    b.rows = v.qlen * a.group;
-    b.row0 = bars->blk * NT * BM;
+    b = bars->work;
   }
 
   if (tc.shared && a.win_left >= 0) __syncthreads();  // min_ahead
@@ -241,7 +241,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (a.win_left >= 0) lo = (int)max(0ll, (long long)bars->min_ahead - a.win_left);
       } else {
         const int r1 = min(r0 + BM, b.rows) - 1;
-        const int p0 = b.klen - b.qlen + r0 / a.group, p1 = b.klen - b.qlen + r1 / a.group;
+        const int p0 = b.klen - b.qlen + (unsigned)r0 / (unsigned)a.group;
+        const int p1 = b.klen - b.qlen + (unsigned)r1 / (unsigned)a.group;
         lo = visible_keys(a, b.klen, p0).x;
         hi = visible_keys(a, b.klen, p1).y;
       }
@@ -259,8 +260,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     int first = 0, last = 0;
     if (k_hi > k_lo) {
       const int t0 = k_lo / BN, n = (k_hi + BN - 1) / BN - t0;
-      first = t0 + (int)((long long)n * split / tc.n_split);
-      last = t0 + (int)((long long)n * (split + 1) / tc.n_split);
+      // (n < 2^23 tiles, at most 32 parts)
+      first = t0 + (int)((unsigned)(n * split) / (unsigned)tc.n_split);
+      last = t0 + (int)((unsigned)(n * (split + 1)) / (unsigned)tc.n_split);
     }
     j_min = first;
     n_kv = 0;
@@ -283,18 +285,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint64_t* full = is_k ? bars->k_full : bars->v_full;
       uint64_t* empty = is_k ? bars->k_empty : bars->v_empty;
       const uint32_t raw = smem_addr(&bars->v_raw);
-      const int box = tc.box_rows, boxes = BN / box;
+      const int box = tc.box_rows, boxes = BN / (unsigned)box;
       const int* table = tc.shared ? a.pre_table : a.table + (int64_t)b.req * a.table_stride;
-      // Page of this lane's box in tile j (-1: nothing to load).
+      // Table entry and first slot of this lane's box in tile j (slot -1:
+      // nothing to load); the entry is checked when it is used.
       auto look_up = [&](int j) {
         const int key = (j_min + j) * BN + lane * box;
-        if (lane >= boxes || j >= n_kv || key >= k_hi || key + box <= k_lo) return -1;
-        const int page = table[key / a.page_size];
-        if ((unsigned)page < (unsigned)a.num_pages) return page;
-        note_bad_index(a.status);
-        return -1;
+        if (lane >= boxes || j >= n_kv || key >= k_hi || key + box <= k_lo) return make_int2(-1, -1);
+        const int p = (unsigned)key / (unsigned)a.page_size;
+        return make_int2(table[p], key - p * a.page_size);
       };
-      int page = look_up(0), raw_phase = 0, issued = 0;
+      int2 next = look_up(0);
+      int raw_phase = 0, issued = 0;
       for (int j = 0; j < n_kv; ++j) {
         const int st = j % C::NS;
         bool ok = true;
@@ -304,6 +306,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (!__shfl_sync(0xffffffffu, (int)ok, 0)) break;
         const int kv0 = (j_min + j) * BN;
+        const int page = next.y < 0 ? -1 : valid_page(a, next.x), slot = next.y;
         const unsigned on = __ballot_sync(0xffffffffu, page >= 0);
         const uint32_t bytes = (uint32_t)__popc(on) * box * 128 * C::NBOX;
         // Edge tile: some of its rows are not of visible keys.
@@ -317,14 +320,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
         if (page >= 0) {
-          const int slot = (kv0 + lane * box) % a.page_size;
           const uint32_t dst = ring + st * C::TILE_BYTES + lane * box * 128;
 #pragma unroll
           for (int bx = 0; bx < C::NBOX; ++bx)
             tma_load_4d(dst + bx * C::BOX_BYTES, tm, bar, bx * 64, hk, slot, page);
         }
         __syncwarp();
-        page = look_up(j + 1);
+        next = look_up(j + 1);
         if (clean) {
           if (lane == 0) ok = fa_wait(raw, raw_phase, a.status, wlim);
           if (!__shfl_sync(0xffffffffu, (int)ok, 0)) {
@@ -338,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint8_t* tile = smem + C::OFF_V + st * C::TILE_BYTES;
           for (int e = lane; e < BN * 8; e += 32) {
             const int row = e >> 3, key = kv0 + row;
-            if (key >= k_lo && key < k_hi && ((on >> (row / box)) & 1)) continue;
+            if (key >= k_lo && key < k_hi && ((on >> ((unsigned)row / (unsigned)box)) & 1)) continue;
 #pragma unroll
             for (int bx = 0; bx < C::NBOX; ++bx)
               *reinterpret_cast<uint4*>(tile + bx * C::BOX_BYTES + e * 16) = make_uint4(0, 0, 0, 0);
@@ -432,16 +434,36 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool row_ok = pr < b.rows;
     const int my_kv = (t == 0) ? n_kv_t[0] : n_kv_t[1];
     const int my_lo = j_min + ((t == 0) ? s_lo[0] : s_lo[1]);
-    const int tok = row_ok ? b.q0 + pr / a.group : 0;
-    const int head = hk * a.group + pr % a.group;
+    const int pj = (unsigned)pr / (unsigned)a.group;
+    const int tok = row_ok ? b.q0 + pj : 0;
+    const int head = hk * a.group + (pr - pj * a.group);
+    constexpr int CH = D / 8;          // 16-byte pieces of a 16-bit row
+    constexpr int RPI = 32 / CH;       // rows a warp moves with one instruction
+    // Element offset of row `i` of the warp's 32 (a lane's own is `mine`), -1
+    // for a row that does not exist.
+    auto row_at = [&](int64_t mine, int i) {
+      const unsigned lo = __shfl_sync(0xffffffffu, (unsigned)mine, i);
+      const int hi = __shfl_sync(0xffffffffu, (int)(mine >> 32), i);
+      return (int64_t)hi << 32 | lo;
+    };
     if (my_kv > 0) {
-      const T* qrow = reinterpret_cast<const T*>(a.q) + (int64_t)tok * a.q_st + (int64_t)head * a.q_sh;
-      uint8_t* dst = smem + C::OFF_Q + t * C::TILE_BYTES + row * 128;
+      // Whole rows at a time: a lane per row would touch 32 lines with every
+      // load (16 such loads took 2.5 us of a block's 12 us start-up and end).
+      const T* Q = reinterpret_cast<const T*>(a.q);
+      const int64_t q_at = row_ok ? (int64_t)tok * a.q_st + (int64_t)head * a.q_sh : -1;
+      uint8_t* dst = smem + C::OFF_Q + t * C::TILE_BYTES + (warp & 3) * 32 * 128;
+      const int c = lane % CH;
+      uint4 x[CH];
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (row_ok && c * 8 < a.D) x = *reinterpret_cast<const uint4*>(qrow + c * 8);
-        *reinterpret_cast<uint4*>(dst + (c >> 3) * C::BOX_BYTES + (((c & 7) ^ (row & 7)) << 4)) = x;
+      for (int i = 0; i < CH; ++i) {
+        const int64_t at = row_at(q_at, i * RPI + lane / CH);
+        x[i] = make_uint4(0, 0, 0, 0);
+        if (at >= 0 && c * 8 < a.D) x[i] = *reinterpret_cast<const uint4*>(Q + at + c * 8);
+      }
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const int r = i * RPI + lane / CH;
+        *reinterpret_cast<uint4*>(dst + (c >> 3) * C::BOX_BYTES + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x[i];
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -470,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           row_hi = min(see.y, b.klen);
         }
       } else {
-        qpos = b.klen - b.qlen + pr / a.group;
+        qpos = b.klen - b.qlen + pj;
         const int2 see = visible_keys(a, b.klen, qpos);
         row_lo = see.x;
         row_hi = see.y;
@@ -591,45 +613,59 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < D; ++i) ov[i] = 0.f;
       }
+      const int part = tc.part0 + split;
+      const int64_t prow = ((int64_t)part * a.total_q + tok) * a.Hq + head;
       if (row_ok) {
-        if (tc.partial) {
-          const int part = tc.part0 + split;
-          const int64_t prow = ((int64_t)part * a.total_q + tok) * a.Hq + head;
-          float* dst = a.parts_o + prow * a.D;
-          a.parts_lse[prow] = lse;
+        if (tc.partial) a.parts_lse[prow] = lse;
+        else if (a.lse != nullptr) a.lse[(int64_t)head * a.total_q + tok] = lse;
+      }
+      const int64_t o_at = (int64_t)tok * a.o_st + (int64_t)head * a.o_sh;
+      if (tc.partial || tc.out_vec) {
+        // Whole rows at a time here too: each warp turns its 32 rows around in
+        // its part of the row tile's Q space (free: o_full came after the last
+        // S MMA), 16-byte pieces XOR-swizzled by row. A 16-bit row fills its
+        // 2 D bytes at once, a float32 row takes two passes.
+        uint8_t* buf = smem + C::OFF_Q + t * C::TILE_BYTES + (warp & 3) * 32 * (D * 2);
+        const int dt = tc.partial ? (int)kF32 : a.out_dtype;
+        uint8_t* base = tc.partial ? reinterpret_cast<uint8_t*>(a.parts_o) : reinterpret_cast<uint8_t*>(a.o);
+        const int64_t mine = row_ok ? (tc.partial ? prow * a.D : o_at) : -1;
+        const int r = lane, c = lane % CH;
 #pragma unroll
-          for (int c = 0; c < D / 4; ++c)
-            if (c * 4 < a.D)
-              *reinterpret_cast<float4*>(dst + 4 * c) = make_float4(ov[4 * c], ov[4 * c + 1], ov[4 * c + 2], ov[4 * c + 3]);
-        } else {
-          if (a.lse != nullptr) a.lse[(int64_t)head * a.total_q + tok] = lse;
-          const int64_t at = (int64_t)tok * a.o_st + (int64_t)head * a.o_sh;
-          const int elem = a.out_dtype == kF32 ? 4 : 2;
-          uint8_t* dst = reinterpret_cast<uint8_t*>(a.o) + at * elem;
-          if ((reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+        for (int pass = 0; pass < 2; ++pass) {
+          if (pass == 1 && dt != kF32) break;
 #pragma unroll
-            for (int c = 0; c < D / 8; ++c) {
-              if (c * 8 >= a.D) continue;
-              const float* x = ov + c * 8;
-              if (a.out_dtype == kF32) {
-                reinterpret_cast<float4*>(dst)[2 * c] = make_float4(x[0], x[1], x[2], x[3]);
-                reinterpret_cast<float4*>(dst)[2 * c + 1] = make_float4(x[4], x[5], x[6], x[7]);
-              } else if (a.out_dtype == kF16) {
-                reinterpret_cast<uint4*>(dst)[c] = make_uint4(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]),
-                                                              pack_half2(x[4], x[5]), pack_half2(x[6], x[7]));
-              } else {
-                reinterpret_cast<uint4*>(dst)[c] = make_uint4(pack_bf162(x[0], x[1]), pack_bf162(x[2], x[3]),
-                                                              pack_bf162(x[4], x[5]), pack_bf162(x[6], x[7]));
-              }
+          for (int k = 0; k < CH; ++k) {
+            uint4 w;
+            const float* x = ov + k * 8;
+            if (dt == kF32) {
+              const float* y = ov + pass * (D / 2) + k * 4;
+              w = make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
+            } else if (dt == kF16) {
+              w = make_uint4(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]), pack_half2(x[4], x[5]), pack_half2(x[6], x[7]));
+            } else {
+              w = make_uint4(pack_bf162(x[0], x[1]), pack_bf162(x[2], x[3]), pack_bf162(x[4], x[5]), pack_bf162(x[6], x[7]));
             }
-          } else {
-#pragma unroll
-            for (int c = 0; c < D / 4; ++c) {
-              if (c * 4 >= a.D) continue;
-              const float x[4] = {ov[4 * c], ov[4 * c + 1], ov[4 * c + 2], ov[4 * c + 3]};
-              store_out4(a.o, at + 4 * c, a.out_dtype, x, 4);
-            }
+            *reinterpret_cast<uint4*>(buf + r * (D * 2) + ((k ^ (r & 7)) << 4)) = w;
           }
+          __syncwarp();
+          const int col = dt == kF32 ? pass * (D / 2) + c * 4 : c * 8;
+          const int elem = dt == kF32 ? 4 : 2;
+#pragma unroll
+          for (int i = 0; i < CH; ++i) {
+            const int rr = i * RPI + lane / CH;
+            const int64_t at = row_at(mine, rr);
+            if (at >= 0 && col < a.D)
+              *reinterpret_cast<uint4*>(base + (at + col) * elem) =
+                  *reinterpret_cast<const uint4*>(buf + rr * (D * 2) + ((c ^ (rr & 7)) << 4));
+          }
+          __syncwarp();
+        }
+      } else if (row_ok) {
+#pragma unroll
+        for (int k = 0; k < D / 4; ++k) {
+          if (k * 4 >= a.D) continue;
+          const float x[4] = {ov[4 * k], ov[4 * k + 1], ov[4 * k + 2], ov[4 * k + 3]};
+          store_out4(a.o, o_at + 4 * k, a.out_dtype, x, 4);
         }
       }
     }
