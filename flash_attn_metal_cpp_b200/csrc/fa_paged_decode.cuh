@@ -66,9 +66,6 @@ constexpr int smem_bytes() {
   return Cfg<DM, MT>::NS * Cfg<DM, MT>::STAGE + (int)sizeof(Shared<Cfg<DM, MT>::NS, MT>);
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
-}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }

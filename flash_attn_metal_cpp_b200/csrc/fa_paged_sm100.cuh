@@ -451,20 +451,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       // load (16 such loads took 2.5 us of a block's 12 us start-up and end).
       const T* Q = reinterpret_cast<const T*>(a.q);
       const int64_t q_at = row_ok ? (int64_t)tok * a.q_st + (int64_t)head * a.q_sh : -1;
-      uint8_t* dst = smem + C::OFF_Q + t * C::TILE_BYTES + (warp & 3) * 32 * 128;
       const int c = lane % CH;
-      uint4 x[CH];
-#pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        const int64_t at = row_at(q_at, i * RPI + lane / CH);
-        x[i] = make_uint4(0, 0, 0, 0);
-        if (at >= 0 && c * 8 < a.D) x[i] = *reinterpret_cast<const uint4*>(Q + at + c * 8);
-      }
-#pragma unroll
+      const uint32_t dst = sQ + t * C::TILE_BYTES + (warp & 3) * 32 * 128 + (c >> 3) * C::BOX_BYTES;
+      // Rolled, here and where the output leaves: this code runs once a block,
+      // and fetching unrolled instructions took longer than the copies.
+#pragma unroll 1
       for (int i = 0; i < CH; ++i) {
         const int r = i * RPI + lane / CH;
-        *reinterpret_cast<uint4*>(dst + (c >> 3) * C::BOX_BYTES + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x[i];
+        const int64_t at = row_at(q_at, r);
+        const bool on = at >= 0 && c * 8 < a.D;
+        cp_async16(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4), on ? Q + at + c * 8 : Q, on);
       }
+      cp_async_wait_all();
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_addr(&bars->q_full[t]));
@@ -650,7 +648,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
           const int col = dt == kF32 ? pass * (D / 2) + c * 4 : c * 8;
           const int elem = dt == kF32 ? 4 : 2;
-#pragma unroll
+#pragma unroll 4
           for (int i = 0; i < CH; ++i) {
             const int rr = i * RPI + lane / CH;
             const int64_t at = row_at(mine, rr);
