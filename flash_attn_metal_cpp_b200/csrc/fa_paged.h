@@ -68,6 +68,25 @@ struct StoreArgs {
 };
 cudaError_t launch_store_kv(const StoreArgs& a, int dtype, bool vec, cudaStream_t stream);
 
+// Division by a number known on the host, for numerators below 2^31:
+// n / d = (umulhi(n, m) + n) >> s with s = ceil(log2 d) and
+// m = floor(2^32 (2^s - d) / d) + 1 (Granlund and Montgomery 1994). A block of
+// the attention kernels lives for a few microseconds and runs its index
+// arithmetic once: what counts there is the number of instructions.
+struct Div {
+  unsigned m, s;
+  int d;
+  Div() = default;
+  explicit Div(int div) : d(div) {
+    s = 0;
+    while ((1ull << s) < (unsigned long long)div) ++s;
+    m = (unsigned)((1ull << 32) * ((1ull << s) - (unsigned long long)div) / (unsigned long long)div + 1);
+  }
+#ifdef __CUDACC__
+  __device__ __forceinline__ int operator()(int n) const { return (int)((__umulhi((unsigned)n, m) + (unsigned)n) >> s); }
+#endif
+};
+
 // ----------------------------------------------------- attention over pages
 // One call's description for every paged attention kernel. The query tokens
 // of request i are rows [cu_q[i], cu_q[i + 1]) of q (row i alone when cu_q is
@@ -77,6 +96,8 @@ cudaError_t launch_store_kv(const StoreArgs& a, int dtype, bool vec, cudaStream_
 struct PagedArgs {
   int B, total_q, Hq, Hk, D, group;
   int page_size, num_pages, max_pages;
+  int max_len;             // most keys a table row holds (below 2^29)
+  Div by_group, by_page, by_hk;
   const int* table;
   int64_t table_stride;
   const int* seq_lens;
@@ -147,6 +168,7 @@ struct PagedTc {
   int shared;        // 1: the rows of all requests against the prefix
   int n_blocks;      // blocks of 256 packed rows (an upper bound)
   int n_split;       // parts the keys of a block are cut in
+  Div by_split;
   int box_rows;      // slots of one TMA box
   int partial;       // 1: normalised partial results to part0 + split
   int part0;

@@ -63,6 +63,10 @@ fa_status check(const fa_paged_params* p, Checked* c, bool grouped = true) {
   a.max_pages = (int)p->max_pages;
   a.table_stride = p->table_stride ? p->table_stride : (int64_t)p->max_pages;
   a.pre = (int)p->prefix_len;
+  a.max_len = (int)std::min<uint64_t>((uint64_t)p->max_pages * p->page_size, (1u << 29) - 1);
+  a.by_group = Div(std::max(1, a.group));
+  a.by_page = Div(a.page_size);
+  a.by_hk = Div(a.Hk);
   const int64_t row_q = (int64_t)a.Hq * a.D, row_k = (int64_t)a.Hk * a.D;
   auto two = [&](const int64_t in[2], int64_t row, int64_t* s0, int64_t* s1) {
     const bool none = in[0] == 0 && in[1] == 0;
@@ -90,8 +94,8 @@ fa_status check(const fa_paged_params* p, Checked* c, bool grouped = true) {
   a.scale_log2 = (float)((double)p->softmax_scale * 1.4426950408889634);
   a.softcap = p->softcap;
   a.causal = p->is_causal ? 1 : 0;
-  a.win_left = p->window_left < 0 ? -1 : p->window_left;
-  a.win_right = p->window_right < 0 ? -1 : p->window_right;
+  a.win_left = p->window_left < 0 ? -1 : std::min(p->window_left, 1 << 30);
+  a.win_right = p->window_right < 0 ? -1 : std::min(p->window_right, 1 << 30);
   a.alibi = p->alibi_slopes;
   c->dtype = p->dtype;
   const int64_t m = 16 / (int64_t)elem_size(p->dtype);
@@ -426,6 +430,7 @@ fa_status fa_paged_forward(const fa_paged_params* p, const void* q, const void* 
     t.shared = 1;
     t.n_blocks = h.pre_blocks;
     t.n_split = h.pre_split;
+    t.by_split = Div(t.n_split);
     t.partial = 1;
     st = cuda_status(launch_tc(a, t, c.dtype, tk, tv, s), "shared prefix attention");
     if (st != FA_OK) return st;
@@ -436,6 +441,7 @@ fa_status fa_paged_forward(const fa_paged_params* p, const void* q, const void* 
     t.shared = 0;
     t.n_blocks = h.own_blocks;
     t.n_split = h.own_split;
+    t.by_split = Div(t.n_split);
     t.partial = h.n_parts > 0;
     t.part0 = h.pre_split;
     st = cuda_status(launch_tc(a, t, c.dtype, tk, tv, s), "paged attention (many rows)");

@@ -49,7 +49,7 @@ struct TileDesc {
   int rows;       // packed rows of the unit; 0 = no tile
   int row0;
   int q0, qlen, klen, key_lo;
-  int hk, tile;
+  int req, hk, tile;
   int first, last, whole, slot;
 };
 
@@ -124,8 +124,9 @@ struct Cursor {
     unit = (int)div_ll(off, per);
     const long long in_unit = off - (long long)unit * per;
     left = run.end - run.begin + in_unit;
-    hk = unit % a.Hk;
-    row0 = unit / a.Hk * MR;
+    const int chunk = a.by_hk(unit);
+    hk = unit - chunk * a.Hk;
+    row0 = chunk * MR;
     begin_piece(a, a.split ? tile_at(in_unit) : 0);
   }
 
@@ -133,6 +134,7 @@ struct Cursor {
   __device__ __forceinline__ void next(const PagedArgs& a, TileDesc& d) {
     d.rows = 0;
     if (left <= 0) return;
+    d.req = req;
     d.hk = hk;
     d.row0 = row0;
     d.rows = min(MR, v.qlen * a.group - row0);
@@ -211,11 +213,11 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
   // Table entry and slot of key `tid` of a tile (slot -1: no key).
   // put_rows() checks the entry and turns it into row offsets a tile later:
   // the load is in flight until then, and the copies need one addition each.
-  auto look_up = [&](const TileDesc& d, int req) {
+  auto look_up = [&](const TileDesc& d) {
     int2 ps = make_int2(-1, -1);
     if (tid < kTile && d.rows > 0) {
       const int key = d.tile * kTile + tid;
-      if (key >= d.key_lo && key < d.klen) ps = find_key(a, req, key);
+      if (key >= d.key_lo && key < d.klen) ps = find_key(a, d.req, key);
     }
     return ps;
   };
@@ -254,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
           const int e = n * kThreads + tid, r = e / CPR, c = e % CPR;
           const bool on = r < d.rows && c * 8 < a.D;
           const int row = d.row0 + (on ? r : 0);
-          const int j = row / a.group, head = d.hk * a.group + row - j * a.group;
+          const int j = a.by_group(row), head = d.hk * a.group + row - j * a.group;
           const T* qs = on ? Q + (int64_t)(d.q0 + j) * a.q_st + (int64_t)head * a.q_sh + c * 8 : Q;
           cp_async16(sq + r * (DM * 2) + ((c ^ (r & 7)) << 4), qs, on);
         }
@@ -264,23 +266,23 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
   };
 
   {
-    // Prologue: page numbers of the first NS tiles together, then the copies
-    // of NS - 1 of them.
-    int2 ps[NS];
-    int hks[NS];
-#pragma unroll
+    // Prologue: the first NS tiles' page numbers together, then the copies of
+    // NS - 1 of them. The loops stay rolled where they can: this code runs
+    // once, and its instructions come from L2.
+#pragma unroll 1
     for (int i = 0; i < NS; ++i) {
       TileDesc d;
-      const int req = cur.req;
       cur.next(a, d);
       if (tid == 0) sh.desc[i] = d;
-      ps[i] = look_up(d, req);
-      hks[i] = d.hk;
     }
-#pragma unroll
-    for (int i = 0; i < NS; ++i) put_rows(i, ps[i], hks[i]);
     __syncthreads();
+    int2 ps[NS];
 #pragma unroll
+    for (int i = 0; i < NS; ++i) ps[i] = look_up(sh.desc[i]);
+#pragma unroll
+    for (int i = 0; i < NS; ++i) put_rows(i, ps[i], sh.desc[i].hk);
+    __syncthreads();
+#pragma unroll 1
     for (int i = 0; i < NS - 1; ++i) issue(i, i);
   }
 
@@ -302,13 +304,12 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
     const int di_issue = di + NS - 1 > NS ? di - 2 : di + NS - 1;   // (di + NS - 1) mod (NS + 1)
     issue(di_issue, st == 0 ? NS - 1 : st - 1);
     TileDesc dn;
-    const int req_n = cur.req;
     cur.next(a, dn);
-    const int2 pn = look_up(dn, req_n);
+    const int2 pn = look_up(dn);
 
     const uint32_t sk = ring_addr + st * C::STAGE, sv = sk + C::KV_BYTES;
     if (d.first) {
-      const int p0 = d.klen - d.qlen + d.row0 / a.group, p1 = d.klen - d.qlen + (d.row0 + d.rows - 1) / a.group;
+      const int p0 = d.klen - d.qlen + a.by_group(d.row0), p1 = d.klen - d.qlen + a.by_group(d.row0 + d.rows - 1);
       full_hi = plain ? visible_keys(a, d.klen, p0).y : 0;
       full_lo = max(visible_keys(a, d.klen, p1).x, d.key_lo);
       const uint32_t sq = sk + 2 * C::KV_BYTES;
@@ -321,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int row = d.row0 + min(mt * 16 + e * 8 + (lane >> 2), d.rows - 1);
-          const int j = row / a.group;
+          const int j = a.by_group(row);
           qpos[mt][e] = d.klen - d.qlen + j;
           const int2 see = visible_keys(a, d.klen, qpos[mt][e]);
           lo[mt][e] = see.x;
@@ -493,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
             x[3] += y.w;
           }
           if (d.whole) {
-            const int row = d.row0 + rr, j = row / a.group;
+            const int row = d.row0 + rr, j = a.by_group(row);
             finish_row4(a, d.q0 + j, d.hk * a.group + row - j * a.group, col, x, top, ls);
           } else {
             const int64_t sr = ((int64_t)blockIdx.x * 2 + d.slot) * MR + rr;

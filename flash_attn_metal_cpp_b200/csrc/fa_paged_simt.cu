@@ -91,8 +91,9 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
     const int t_end = v.tile_lo + v.tiles;
     const int t0 = v.tile_lo + (a.split ? tile_at(at - unit_begin) : 0);
     const int t1 = a.split && run.end < unit_begin + per ? v.tile_lo + tile_at(run.end - unit_begin) : t_end;
-    const int hk = unit % a.Hk;
-    const int row0 = unit / a.Hk * R;
+    const int chunk = a.by_hk(unit);
+    const int hk = unit - chunk * a.Hk;
+    const int row0 = chunk * R;
     const int rows = min(R, v.qlen * a.group - row0);
     if (a.split && at == run.begin && tid == 0) {
       RunMeta& mt = a.meta[blockIdx.x];
@@ -114,7 +115,7 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int row = row0 + min(r, rows - 1);
-      const int j = row / a.group, head = hk * a.group + row % a.group;
+      const int j = a.by_group(row), head = hk * a.group + row - j * a.group;
       load_slice<T, DPL, VEC>(Q + (int64_t)(v.q0 + j) * a.q_st + (int64_t)head * a.q_sh, sub, a.D, q[r]);
       qpos[r] = v.klen - v.qlen + j;
       vis[r] = visible_keys(a, v.klen, qpos[r]);
@@ -223,8 +224,8 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
         for (int i = 0; i < 4; ++i) x[i] = fmaf(f, sm_o[w][r][col + i], x[i]);
       }
       if (whole) {
-        const int row = row0 + r;
-        finish_row4(a, v.q0 + row / a.group, hk * a.group + row % a.group, col, x, top, ls);
+        const int row = row0 + r, j = a.by_group(row);
+        finish_row4(a, v.q0 + j, hk * a.group + row - j * a.group, col, x, top, ls);
       } else {
         const int64_t sr = (int64_t)slot * a.rows_per_unit + r;
         *reinterpret_cast<float4*>(a.slot_o + sr * sd + col) = make_float4(x[0], x[1], x[2], x[3]);
@@ -326,8 +327,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const Paged
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = fmaf(f, sm_o[w][col + i], x[i]);
   }
-  const int row = mt.row0 + r;
-  finish_row4(a, mt.q0 + row / a.group, mt.hk * a.group + row % a.group, col, x, top, ls);
+  const int row = mt.row0 + r, j = a.by_group(row);
+  finish_row4(a, mt.q0 + j, mt.hk * a.group + row - j * a.group, col, x, top, ls);
 }
 
 // Join of whole-row partial results: LSE = log sum_p exp(lse_p),

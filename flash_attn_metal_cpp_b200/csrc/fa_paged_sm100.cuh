@@ -158,9 +158,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   // Blocks of a request's rows stand in one line over the requests, the last
   // ones first (under a causal mask they have the most keys); within a block
   // the KV heads, within a head the parts of the keys.
-  const unsigned per_split = blockIdx.x / (unsigned)tc.n_split;
+  const int per_split = tc.by_split(blockIdx.x);
   const int split = blockIdx.x - per_split * tc.n_split;
-  const int bi = per_split / (unsigned)a.Hk;
+  const int bi = a.by_hk(per_split);
   const int hk = per_split - bi * a.Hk;
   Block b;
   if (tc.shared) {
@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (a.win_left >= 0) {
       // The window may leave most of the prefix unseen: the earliest query of
       // the batch says how much.
-      int ahead = 0x7fffffff;
+      int ahead = 1 << 30;
       for (int i = threadIdx.x; i < a.B; i += kThreads) {
         const ReqView v = view_request<BN>(a, i, BM);
         if (v.qlen > 0) ahead = min(ahead, v.klen - v.qlen);
@@ -238,11 +238,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (r0 < b.rows) {
       hi = b.klen;
       if (tc.shared) {
-        if (a.win_left >= 0) lo = (int)max(0ll, (long long)bars->min_ahead - a.win_left);
+        if (a.win_left >= 0) lo = max(0, bars->min_ahead - a.win_left);
       } else {
         const int r1 = min(r0 + BM, b.rows) - 1;
-        const int p0 = b.klen - b.qlen + (unsigned)r0 / (unsigned)a.group;
-        const int p1 = b.klen - b.qlen + (unsigned)r1 / (unsigned)a.group;
+        const int p0 = b.klen - b.qlen + a.by_group(r0);
+        const int p1 = b.klen - b.qlen + a.by_group(r1);
         lo = visible_keys(a, b.klen, p0).x;
         hi = visible_keys(a, b.klen, p1).y;
       }
@@ -261,8 +261,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (k_hi > k_lo) {
       const int t0 = k_lo / BN, n = (k_hi + BN - 1) / BN - t0;
       // (n < 2^23 tiles, at most 32 parts)
-      first = t0 + (int)((unsigned)(n * split) / (unsigned)tc.n_split);
-      last = t0 + (int)((unsigned)(n * (split + 1)) / (unsigned)tc.n_split);
+      first = t0 + tc.by_split(n * split);
+      last = t0 + tc.by_split(n * (split + 1));
     }
     j_min = first;
     n_kv = 0;
@@ -285,14 +285,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint64_t* full = is_k ? bars->k_full : bars->v_full;
       uint64_t* empty = is_k ? bars->k_empty : bars->v_empty;
       const uint32_t raw = smem_addr(&bars->v_raw);
-      const int box = tc.box_rows, boxes = BN / (unsigned)box;
+      const int box = tc.box_rows, box_log = 31 - __clz(box), boxes = BN >> box_log;  // (a power of two)
       const int* table = tc.shared ? a.pre_table : a.table + (int64_t)b.req * a.table_stride;
       // Table entry and first slot of this lane's box in tile j (slot -1:
       // nothing to load); the entry is checked when it is used.
       auto look_up = [&](int j) {
         const int key = (j_min + j) * BN + lane * box;
         if (lane >= boxes || j >= n_kv || key >= k_hi || key + box <= k_lo) return make_int2(-1, -1);
-        const int p = (unsigned)key / (unsigned)a.page_size;
+        const int p = a.by_page(key);
         return make_int2(table[p], key - p * a.page_size);
       };
       int2 next = look_up(0);
@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint8_t* tile = smem + C::OFF_V + st * C::TILE_BYTES;
           for (int e = lane; e < BN * 8; e += 32) {
             const int row = e >> 3, key = kv0 + row;
-            if (key >= k_lo && key < k_hi && ((on >> ((unsigned)row / (unsigned)box)) & 1)) continue;
+            if (key >= k_lo && key < k_hi && ((on >> (row >> box_log)) & 1)) continue;
 #pragma unroll
             for (int bx = 0; bx < C::NBOX; ++bx)
               *reinterpret_cast<uint4*>(tile + bx * C::BOX_BYTES + e * 16) = make_uint4(0, 0, 0, 0);
@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool row_ok = pr < b.rows;
     const int my_kv = (t == 0) ? n_kv_t[0] : n_kv_t[1];
     const int my_lo = j_min + ((t == 0) ? s_lo[0] : s_lo[1]);
-    const int pj = (unsigned)pr / (unsigned)a.group;
+    const int pj = a.by_group(pr);
     const int tok = row_ok ? b.q0 + pj : 0;
     const int head = hk * a.group + (pr - pj * a.group);
     constexpr int CH = D / 8;          // 16-byte pieces of a 16-bit row
@@ -601,16 +601,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (ok && b.row0 + t * BM < b.rows) {
       const float inv_l = (l_run > 0.f) ? 1.f / l_run : 0.f;
       const float lse = (l_run > 0.f) ? (m_run + log2f(l_run)) * kLn2 : -INFINITY;
-      float ov[D];
-      if (my_kv > 0) {
-        if constexpr (D == 128) tmem_ld128(tO, ov);
-        else tmem_ld64(tO, ov);
+      // 16 columns of the row's O, divided by the sum.
+      auto take16 = [&](int col, float (&x)[16]) {
+        uint32_t u[16];
+        if (my_kv > 0) tmem_ld16(tO + col, u);
 #pragma unroll
-        for (int i = 0; i < D; ++i) ov[i] *= inv_l;
-      } else {
-#pragma unroll
-        for (int i = 0; i < D; ++i) ov[i] = 0.f;
-      }
+        for (int i = 0; i < 16; ++i) x[i] = my_kv > 0 ? __uint_as_float(u[i]) * inv_l : 0.f;
+      };
       const int part = tc.part0 + split;
       const int64_t prow = ((int64_t)part * a.total_q + tok) * a.Hq + head;
       if (row_ok) {
@@ -625,45 +622,58 @@ __global__ void __launch_bounds__(kThreads, 1)
         // 2 D bytes at once, a float32 row takes two passes.
         uint8_t* buf = smem + C::OFF_Q + t * C::TILE_BYTES + (warp & 3) * 32 * (D * 2);
         const int dt = tc.partial ? (int)kF32 : a.out_dtype;
+        const int elem = dt == kF32 ? 4 : 2;
         uint8_t* base = tc.partial ? reinterpret_cast<uint8_t*>(a.parts_o) : reinterpret_cast<uint8_t*>(a.o);
-        const int64_t mine = row_ok ? (tc.partial ? prow * a.D : o_at) : -1;
+        const int64_t mine = row_ok ? (tc.partial ? prow * a.D : o_at) * elem : -1;
         const int r = lane, c = lane % CH;
-#pragma unroll
-        for (int pass = 0; pass < 2; ++pass) {
-          if (pass == 1 && dt != kF32) break;
-#pragma unroll
-          for (int k = 0; k < CH; ++k) {
-            uint4 w;
-            const float* x = ov + k * 8;
+        const int passes = dt == kF32 ? 2 : 1, cols = D / passes;
+        const int col = c * (16 / elem);  // of this lane's piece, in a pass
+#pragma unroll 1
+        for (int pass = 0; pass < passes; ++pass) {
+#pragma unroll 1
+          for (int k = 0; k < cols; k += 16) {
+            float x[16];
+            take16(pass * cols + k, x);
+            uint8_t* to = buf + r * (D * 2);
+            const int sw = r & 7;
             if (dt == kF32) {
-              const float* y = ov + pass * (D / 2) + k * 4;
-              w = make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
-            } else if (dt == kF16) {
-              w = make_uint4(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]), pack_half2(x[4], x[5]), pack_half2(x[6], x[7]));
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<float4*>(to + (((k / 4 + i) ^ sw) << 4)) =
+                    make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
             } else {
-              w = make_uint4(pack_bf162(x[0], x[1]), pack_bf162(x[2], x[3]), pack_bf162(x[4], x[5]), pack_bf162(x[6], x[7]));
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const float* y = x + 8 * i;
+                *reinterpret_cast<uint4*>(to + (((k / 8 + i) ^ sw) << 4)) =
+                    dt == kF16 ? make_uint4(pack_half2(y[0], y[1]), pack_half2(y[2], y[3]), pack_half2(y[4], y[5]), pack_half2(y[6], y[7]))
+                               : make_uint4(pack_bf162(y[0], y[1]), pack_bf162(y[2], y[3]), pack_bf162(y[4], y[5]), pack_bf162(y[6], y[7]));
+              }
             }
-            *reinterpret_cast<uint4*>(buf + r * (D * 2) + ((k ^ (r & 7)) << 4)) = w;
           }
           __syncwarp();
-          const int col = dt == kF32 ? pass * (D / 2) + c * 4 : c * 8;
-          const int elem = dt == kF32 ? 4 : 2;
+          const bool col_on = pass * cols + col < a.D;
+          uint8_t* dst = base + (int64_t)(pass * cols + col) * elem;
 #pragma unroll 4
           for (int i = 0; i < CH; ++i) {
             const int rr = i * RPI + lane / CH;
             const int64_t at = row_at(mine, rr);
-            if (at >= 0 && col < a.D)
-              *reinterpret_cast<uint4*>(base + (at + col) * elem) =
-                  *reinterpret_cast<const uint4*>(buf + rr * (D * 2) + ((c ^ (rr & 7)) << 4));
+            if (at >= 0 && col_on)
+              *reinterpret_cast<uint4*>(dst + at) = *reinterpret_cast<const uint4*>(buf + rr * (D * 2) + ((c ^ (rr & 7)) << 4));
           }
           __syncwarp();
         }
-      } else if (row_ok) {
+      } else {
+        // Rows that start anywhere: element by element.
+#pragma unroll 1
+        for (int k = 0; k < D; k += 16) {
+          float x[16];
+          take16(k, x);
 #pragma unroll
-        for (int k = 0; k < D / 4; ++k) {
-          if (k * 4 >= a.D) continue;
-          const float x[4] = {ov[4 * k], ov[4 * k + 1], ov[4 * k + 2], ov[4 * k + 3]};
-          store_out4(a.o, o_at + 4 * k, a.out_dtype, x, 4);
+          for (int i = 0; i < 4; ++i) {
+            const float y[4] = {x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
+            if (row_ok && k + 4 * i < a.D) store_out4(a.o, o_at + k + 4 * i, a.out_dtype, y, 4);
+          }
         }
       }
     }
