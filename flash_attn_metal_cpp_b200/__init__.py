@@ -35,10 +35,17 @@ sys.modules.setdefault("_flash_attn_metal", _flash_attn_metal)
 initialize = _flash_attn_metal.initialize
 get_device_info = _flash_attn_metal.get_device_info
 forward = _flash_attn_metal.forward
-plan_pages = _flash_attn_metal.plan_pages
-store_kv = _flash_attn_metal.store_kv
-paged_forward = _flash_attn_metal.paged_forward
-shared_prefix_forward = _flash_attn_metal.shared_prefix_forward
+
+_PAGED = ("plan_pages", "store_kv", "paged_forward", "shared_prefix_forward")
+
+
+def __getattr__(name):
+    """The paged-cache operators, loaded (with torch) on first use."""
+    if name in _PAGED:
+        for n in _PAGED:
+            globals()[n] = getattr(_flash_attn_metal, n)
+        return globals()[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
 def _to_numpy(x):

@@ -3,6 +3,7 @@
 Produces, inside this package directory:
   libfa_b200.so                     C ABI (include/fa_b200.h): kernels + host dispatcher
   _flash_attn_metal.<abi>.so        pybind11 module over that C ABI
+  _flash_attn_paged.<abi>.so        its paged-cache operators (pybind11 and torch)
 
 Every CUDA translation unit is compiled for sm_100a only
 (-gencode arch=compute_100a,code=sm_100a). Objects are compiled in
@@ -24,6 +25,7 @@ INCLUDE = os.path.join(ROOT, "include")
 OBJDIR = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libfa_b200.so")
 EXT = os.path.join(PKG, "_flash_attn_metal" + sysconfig.get_config_var("EXT_SUFFIX"))
+EXT_PAGED = os.path.join(PKG, "_flash_attn_paged" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 CUDA_HOME = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 NVCC = os.path.join(CUDA_HOME, "bin", "nvcc")
@@ -77,8 +79,33 @@ def _compile(src: str, force: bool) -> str:
     return obj
 
 
+def _torch_flags() -> tuple[list[str], list[str]]:
+    """(compile, link) flags of torch's C++ interface."""
+    import torch
+
+    root = os.path.dirname(os.path.abspath(torch.__file__))
+    inc = os.path.join(root, "include")
+    cflags = ["-isystem", inc, "-isystem", os.path.join(inc, "torch", "csrc", "api", "include"),
+              "-isystem", os.path.join(CUDA_HOME, "include"),
+              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    lib = os.path.join(root, "lib")
+    return cflags, ["-L", lib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python", f"-Wl,-rpath,{lib}"]
+
+
+def _extension(path: str, src: str, cflags: list[str], libs: list[str], force: bool) -> None:
+    """One pybind11 extension linked to libfa_b200.so beside it."""
+    import pybind11
+
+    src = os.path.join(CSRC, src)
+    if not force and _mtime(path) >= max(_mtime(src), _mtime(LIB), _mtime(os.path.join(INCLUDE, "fa_b200.h"))):
+        return
+    _run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-I", pybind11.get_include(),
+          "-I", sysconfig.get_paths()["include"], "-I", INCLUDE, *cflags, src, "-o", path, "-L", PKG,
+          "-l:libfa_b200.so", *libs, "-Wl,-rpath,$ORIGIN"])
+
+
 def build(force: bool = False, jobs: int | None = None) -> tuple[str, str]:
-    """Compile the CUDA library and the Python extension; return their paths."""
+    """Compile the CUDA library and the Python extensions; return the library's and the module's path."""
     if not os.path.exists(NVCC):
         raise RuntimeError(f"nvcc not found at {NVCC}")
     os.makedirs(OBJDIR, exist_ok=True)
@@ -88,16 +115,12 @@ def build(force: bool = False, jobs: int | None = None) -> tuple[str, str]:
     if force or _mtime(LIB) < max(_mtime(o) for o in objs):
         _run([NVCC, *ARCH, "-shared", "-Xcompiler", "-fPIC", "-o", LIB, *objs])
 
-    bsrcs = [os.path.join(CSRC, f) for f in ("bindings.cpp", "bindings_paged.cpp")]
-    if force or _mtime(EXT) < max(*map(_mtime, bsrcs), _mtime(LIB), _mtime(os.path.join(INCLUDE, "fa_b200.h"))):
-        import pybind11
-
-        py_inc = sysconfig.get_paths()["include"]
-        _run([
-            "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
-            "-I", pybind11.get_include(), "-I", py_inc, "-I", INCLUDE,
-            *bsrcs, "-o", EXT, "-L", PKG, "-l:libfa_b200.so", "-Wl,-rpath,$ORIGIN",
-        ])
+    # Two extensions over the C ABI, compiled side by side: the module itself
+    # (NumPy and torch, no link to torch) and the paged-cache operators, which
+    # use torch's C++ interface.
+    exts = [(EXT, "bindings.cpp", [], []), (EXT_PAGED, "bindings_paged.cpp", *_torch_flags())]
+    with cf.ThreadPoolExecutor(max_workers=2) as ex:
+        list(ex.map(lambda e: _extension(*e, force), exts))
     return LIB, EXT
 
 

@@ -606,9 +606,32 @@ py::tuple py_pool_stats() {
   return py::make_tuple(h, m, b);
 }
 
-}  // namespace
+// The paged-cache operators are in an extension of their own, built against
+// torch (bindings_paged.cpp): loaded from beside this one, and put into this
+// module, when one of their names is first asked for.
+py::object py_getattr(py::module_ self, const std::string& name) {
+  static const char* const kPaged[] = {"plan_pages", "store_kv", "paged_forward", "shared_prefix_forward"};
+  bool known = false;
+  for (const char* n : kPaged) known |= name == n;
+  if (!known) {
+    const std::string what = "module '_flash_attn_metal' has no attribute '" + name + "'";
+    throw py::attribute_error(what);
+  }
+  py::module_::import("torch");  // its libraries come first
+  py::module_ os = py::module_::import("os");
+  py::module_ machinery = py::module_::import("importlib.machinery");
+  py::module_ util = py::module_::import("importlib.util");
+  py::object dir = os.attr("path").attr("dirname")(os.attr("path").attr("abspath")(self.attr("__file__")));
+  py::object spec = machinery.attr("PathFinder").attr("find_spec")("_flash_attn_paged", py::make_tuple(dir));
+  if (spec.is_none())
+    throw py::import_error("the extension _flash_attn_paged is not built beside _flash_attn_metal");
+  py::object mod = util.attr("module_from_spec")(spec);
+  spec.attr("loader").attr("exec_module")(mod);
+  for (const char* n : kPaged) self.attr(n) = mod.attr(n);
+  return self.attr(name.c_str());
+}
 
-void bind_paged(py::module_& m);  // bindings_paged.cpp
+}  // namespace
 
 PYBIND11_MODULE(_flash_attn_metal, m) {
   m.doc() = "FlashAttention-2 forward for NVIDIA B200 (sm_100a), drop-in for the Metal module";
@@ -668,5 +691,8 @@ PYBIND11_MODULE(_flash_attn_metal, m) {
     fa_status st = fa_ipc_free(reinterpret_cast<void*>(p));
     if (st != FA_OK) throw std::runtime_error(err_text(st));
   }, py::arg("address"));
-  bind_paged(m);
+  const py::handle self = m;  // (the function lives in the module: no reference of its own)
+  m.def("__getattr__", [self](const std::string& name) {
+    return py_getattr(py::reinterpret_borrow<py::module_>(self), name);
+  }, py::arg("name"), "Loads the paged-cache operators on first use");
 }

@@ -1,14 +1,22 @@
-// bindings_paged.cpp - the paged-cache operators of the `_flash_attn_metal`
-// module over the C ABI in fa_b200.h: plan_pages, store_kv, paged_forward and
-// shared_prefix_forward. CUDA torch tensors only; every call runs on the
-// tensors' device and its current stream and returns without synchronising.
+// bindings_paged.cpp - the `_flash_attn_paged` extension: plan_pages,
+// store_kv, paged_forward and shared_prefix_forward over the C ABI in
+// fa_b200.h. CUDA torch tensors only; every call runs on the tensors' device
+// and its current stream and returns without synchronising.
 //
 // A decoding step makes these calls for every layer, each a few microseconds
-// of GPU time, so the tensors are read through a handful of cached attribute
-// names and no Python-level helper.
-#include <pybind11/pybind11.h>
-#include <pybind11/stl.h>
+// of GPU time, so tensors are read and results allocated through torch's C++
+// interface (reading eight tensors and allocating five through Python took
+// 14 us). That is why they live in an extension of their own, which
+// `_flash_attn_metal` loads when one of them is first used: the rest of the
+// module works without torch.
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/python_variable.h>
 
+#include <pybind11/pybind11.h>
+
+#include <optional>
 #include <stdexcept>
 #include <string>
 
@@ -26,53 +34,17 @@ void check_status(fa_status st) {
   paged_error(s.empty() ? "status " + std::to_string((int)st) : s);
 }
 
-// Names and torch objects looked up once; never released (they live as long
-// as the interpreter).
-struct Torch {
-  PyObject *n_ptr, *n_shape, *n_stride, *n_dtype, *n_device, *n_get_device;
-  PyObject *tensor, *empty, *stream, *get_dev, *set_dev;
-  PyObject* dtypes[3];  // fa_dtype order
-  PyObject *i32, *i64, *u8;
-  Torch() {
-    auto name = [](const char* s) { return PyUnicode_InternFromString(s); };
-    n_ptr = name("data_ptr");
-    n_shape = name("shape");
-    n_stride = name("stride");
-    n_dtype = name("dtype");
-    n_device = name("device");
-    n_get_device = name("get_device");
-    py::module_ t = py::module_::import("torch");
-    py::module_ c = py::module_::import("torch._C");
-    auto keep = [](py::object o) { return o.release().ptr(); };
-    tensor = keep(t.attr("Tensor"));
-    empty = keep(t.attr("empty"));
-    stream = keep(c.attr("_cuda_getCurrentRawStream"));
-    get_dev = keep(c.attr("_cuda_getDevice"));
-    set_dev = keep(c.attr("_cuda_setDevice"));
-    dtypes[FA_F16] = keep(t.attr("float16"));
-    dtypes[FA_BF16] = keep(t.attr("bfloat16"));
-    dtypes[FA_F32] = keep(t.attr("float32"));
-    i32 = keep(t.attr("int32"));
-    i64 = keep(t.attr("int64"));
-    u8 = keep(t.attr("uint8"));
-  }
+// Device of the call: the first tensor sets it, the others must be there too.
+struct Device {
+  int index = -1;
 };
-const Torch& torch_names() {
-  static Torch* t = new Torch();
-  return *t;
-}
-
-py::object own(PyObject* p) {
-  if (!p) throw py::error_already_set();
-  return py::reinterpret_steal<py::object>(p);
-}
 
 constexpr int kMaxDims = 4;
 struct View {
   void* ptr = nullptr;
   int nd = 0;
   int64_t size[kMaxDims] = {}, stride[kMaxDims] = {};
-  PyObject* dtype = nullptr;  // borrowed from the tensor's type object
+  at::ScalarType dtype = at::kFloat;
   bool contiguous() const {
     int64_t run = 1;
     for (int i = nd; i-- > 0;) {
@@ -81,114 +53,57 @@ struct View {
     }
     return true;
   }
-  int64_t numel() const {
-    int64_t n = 1;
-    for (int i = 0; i < nd; ++i) n *= size[i];
-    return n;
-  }
 };
 
-// Device of the call: the first tensor sets it, the others must be there too.
-struct Device {
-  int index = -1;
-  py::object device;
-};
-
-View view(const py::object& o, const char* what, int nd, Device& dev) {
-  const Torch& t = torch_names();
-  if (PyObject_IsInstance(o.ptr(), t.tensor) != 1) paged_error(std::string(what) + " must be a CUDA torch tensor");
-  py::object d = own(PyObject_CallMethodNoArgs(o.ptr(), t.n_get_device));
-  const long index = PyLong_AsLong(d.ptr());
-  if (index < 0) {
-    PyErr_Clear();
-    paged_error(std::string(what) + " must be a CUDA torch tensor");
-  }
-  if (dev.index < 0) {
-    dev.index = (int)index;
-    dev.device = own(PyObject_GetAttr(o.ptr(), t.n_device));
-  } else if (dev.index != (int)index) {
-    paged_error(std::string(what) + " is on another device than the other tensors");
-  }
+View view(py::handle o, const char* what, int nd, Device& dev) {
+  if (!THPVariable_Check(o.ptr())) paged_error(std::string(what) + " must be a CUDA torch tensor");
+  const at::Tensor& t = THPVariable_Unpack(o.ptr());
+  if (!t.is_cuda()) paged_error(std::string(what) + " must be a CUDA torch tensor");
+  const int index = t.get_device();
+  if (dev.index < 0) dev.index = index;
+  else if (dev.index != index) paged_error(std::string(what) + " is on another device than the other tensors");
+  if (t.dim() != nd) paged_error(std::string(what) + " must have " + std::to_string(nd) + " dimensions");
   View v;
-  py::object shape = own(PyObject_GetAttr(o.ptr(), t.n_shape));
-  v.nd = (int)PyTuple_GET_SIZE(shape.ptr());
-  if (v.nd != nd) paged_error(std::string(what) + " must have " + std::to_string(nd) + " dimensions");
-  py::object stride = own(PyObject_CallMethodNoArgs(o.ptr(), t.n_stride));
+  v.nd = nd;
   for (int i = 0; i < nd; ++i) {
-    v.size[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(shape.ptr(), i));
-    v.stride[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(stride.ptr(), i));
+    v.size[i] = t.size(i);
+    v.stride[i] = t.stride(i);
   }
-  py::object p = own(PyObject_CallMethodNoArgs(o.ptr(), t.n_ptr));
-  v.ptr = PyLong_AsVoidPtr(p.ptr());
-  v.dtype = own(PyObject_GetAttr(o.ptr(), t.n_dtype)).ptr();  // dtype objects are never freed
+  v.ptr = t.data_ptr();
+  v.dtype = t.scalar_type();
   return v;
 }
 
 int float_code(const View& v, const char* what) {
-  const Torch& t = torch_names();
-  for (int i = 0; i < 3; ++i)
-    if (v.dtype == t.dtypes[i]) return i;
-  paged_error(std::string(what) + " must be float16, bfloat16 or float32");
+  switch (v.dtype) {
+    case at::kHalf: return FA_F16;
+    case at::kBFloat16: return FA_BF16;
+    case at::kFloat: return FA_F32;
+    default: paged_error(std::string(what) + " must be float16, bfloat16 or float32");
+  }
 }
+at::ScalarType type_of(int code) { return code == FA_F16 ? at::kHalf : code == FA_BF16 ? at::kBFloat16 : at::kFloat; }
 
 // int32 vector of n values (any n when n < 0), contiguous.
-View int_vector(const py::object& o, const char* what, int64_t n, Device& dev) {
+View int_vector(py::handle o, const char* what, int64_t n, Device& dev) {
   View v = view(o, what, 1, dev);
-  if (v.dtype != torch_names().i32) paged_error(std::string(what) + " must be int32");
+  if (v.dtype != at::kInt) paged_error(std::string(what) + " must be int32");
   if (!v.contiguous()) paged_error(std::string(what) + " must be contiguous");
-  if (n >= 0 && v.size[0] != n)
-    paged_error(std::string(what) + " must have " + std::to_string(n) + " entries");
+  if (n >= 0 && v.size[0] != n) paged_error(std::string(what) + " must have " + std::to_string(n) + " entries");
   return v;
 }
 
-py::object empty(std::initializer_list<int64_t> shape, PyObject* dtype, const Device& dev) {
-  static PyObject* kw = [] {
-    PyObject* k = PyTuple_New(2);
-    PyTuple_SET_ITEM(k, 0, PyUnicode_InternFromString("dtype"));
-    PyTuple_SET_ITEM(k, 1, PyUnicode_InternFromString("device"));
-    return k;
-  }();
-  py::object sz = own(PyTuple_New((Py_ssize_t)shape.size()));
-  Py_ssize_t i = 0;
-  for (int64_t s : shape) PyTuple_SET_ITEM(sz.ptr(), i++, PyLong_FromLongLong(s));
-  PyObject* args[3] = {sz.ptr(), dtype, dev.device.ptr()};
-  return own(PyObject_Vectorcall(torch_names().empty, args, 1, kw));
+at::Tensor empty(at::IntArrayRef shape, at::ScalarType dtype, const Device& dev) {
+  return at::empty(shape, at::TensorOptions().dtype(dtype).device(at::Device(at::kCUDA, (c10::DeviceIndex)dev.index)));
 }
 
-void* ptr_of(const py::object& o) {
-  return PyLong_AsVoidPtr(own(PyObject_CallMethodNoArgs(o.ptr(), torch_names().n_ptr)).ptr());
-}
+py::object wrap(const at::Tensor& t) { return py::reinterpret_steal<py::object>(THPVariable_Wrap(t)); }
 
-void* stream_of(const Device& dev) {
-  py::object i = own(PyLong_FromLong(dev.index));
-  py::object s = own(PyObject_CallOneArg(torch_names().stream, i.ptr()));
-  return PyLong_AsVoidPtr(s.ptr());
-}
+void* stream_of(const Device& dev) { return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev.index).stream(); }
 
 // Makes the tensors' device current for the call and puts the caller's back.
-class OnDevice {
- public:
-  explicit OnDevice(const Device& dev) {
-    const Torch& t = torch_names();
-    prev_ = own(PyObject_CallNoArgs(t.get_dev));
-    if (PyLong_AsLong(prev_.ptr()) == dev.index) {
-      prev_ = py::object();
-      return;
-    }
-    py::object i = own(PyLong_FromLong(dev.index));
-    own(PyObject_CallOneArg(t.set_dev, i.ptr()));
-  }
-  ~OnDevice() {
-    if (!prev_) return;
-    py::error_scope keep;  // an exception of the call may be on its way
-    PyObject* r = PyObject_CallOneArg(torch_names().set_dev, prev_.ptr());
-    if (r) Py_DECREF(r);
-    else PyErr_Clear();
-  }
-
- private:
-  py::object prev_;
-};
+using OnDevice = c10::cuda::CUDAGuard;
+OnDevice on_device(const Device& dev) { return OnDevice((c10::DeviceIndex)dev.index); }
 
 // Strides (in elements) of the `n` leading dimensions. Dimensions of one entry
 // get their row's length, so that the C ABI's "all zero = contiguous" is never
@@ -245,12 +160,11 @@ void unit_inner(const View& v, const char* what) {
 // ------------------------------------------------------------------ planning
 py::tuple plan_pages(py::object cached_lens, py::object new_lens, py::object block_table, py::object free_pages,
                      int64_t page_size, int64_t total_new, py::object free_begin) {
-  const Torch& t = torch_names();
   Device dev;
   const View c = int_vector(cached_lens, "cached_lens", -1, dev);
   const View n = int_vector(new_lens, "new_lens", c.size[0], dev);
   const View tb = view(block_table, "block_table", 2, dev);
-  if (tb.dtype != t.i32) paged_error("block_table must be int32");
+  if (tb.dtype != at::kInt) paged_error("block_table must be int32");
   if (tb.size[0] != c.size[0]) paged_error("block_table must have one row per request");
   if (tb.size[1] > 1 && tb.stride[1] != 1) paged_error("block_table needs a unit innermost stride");
   if (tb.size[0] > 1 && tb.stride[0] < tb.size[1]) paged_error("block_table rows must not overlap");
@@ -259,25 +173,25 @@ py::tuple plan_pages(py::object cached_lens, py::object new_lens, py::object blo
   if (total_new < 0) paged_error("total_new must not be negative");
   const int32_t* begin = nullptr;
   if (!free_begin.is_none()) begin = static_cast<const int32_t*>(int_vector(free_begin, "free_begin", 1, dev).ptr);
-  OnDevice guard(dev);
+  const OnDevice guard = on_device(dev);
   const int64_t b = c.size[0];
-  py::object lens = empty({b}, t.i32, dev), cu = empty({b + 1}, t.i32, dev), slots = empty({total_new}, t.i64, dev),
-             pos = empty({total_new}, t.i32, dev), end = empty({1}, t.i32, dev);
+  const at::Tensor lens = empty({b}, at::kInt, dev), cu = empty({b + 1}, at::kInt, dev),
+                   slots = empty({total_new}, at::kLong, dev), pos = empty({total_new}, at::kInt, dev),
+                   end = empty({1}, at::kInt, dev);
   check_status(fa_plan_pages(u32(b, "batch"), u32(page_size, "page_size"), u32(tb.size[1], "max_pages"),
                              u32(f.size[0], "free_pages"), u32(total_new, "total_new"),
                              static_cast<const int32_t*>(c.ptr), static_cast<const int32_t*>(n.ptr),
                              static_cast<const int32_t*>(f.ptr), begin, static_cast<int32_t*>(tb.ptr),
-                             tb.size[0] > 1 ? tb.stride[0] : tb.size[1], static_cast<int32_t*>(ptr_of(lens)),
-                             static_cast<int32_t*>(ptr_of(cu)), static_cast<int64_t*>(ptr_of(slots)),
-                             static_cast<int32_t*>(ptr_of(pos)), static_cast<int32_t*>(ptr_of(end)), stream_of(dev)));
-  return py::make_tuple(lens, cu, slots, pos, end);
+                             tb.size[0] > 1 ? tb.stride[0] : tb.size[1], static_cast<int32_t*>(lens.data_ptr()),
+                             static_cast<int32_t*>(cu.data_ptr()), static_cast<int64_t*>(slots.data_ptr()),
+                             static_cast<int32_t*>(pos.data_ptr()), static_cast<int32_t*>(end.data_ptr()), stream_of(dev)));
+  return py::make_tuple(wrap(lens), wrap(cu), wrap(slots), wrap(pos), wrap(end));
 }
 
 // -------------------------------------------------------------- cache append
 py::object store_kv(py::object k, py::object v, py::object k_cache, py::object v_cache, py::object slots, py::object q,
                     py::object positions, py::object cos, py::object sin, py::object rope_theta,
                     py::object max_position) {
-  const Torch& t = torch_names();
   Device dev;
   const View kn = view(k, "k", 3, dev), vn = view(v, "v", 3, dev);
   const View kc = view(k_cache, "k_cache", 4, dev), vc = view(v_cache, "v_cache", 4, dev);
@@ -299,7 +213,7 @@ py::object store_kv(py::object k, py::object v, py::object k_cache, py::object v
   no_overlap(kc, "k_cache");
   no_overlap(vc, "v_cache");
   const View sl = view(slots, "slots", 1, dev);
-  if (sl.dtype != t.i64 || !sl.contiguous() || sl.size[0] != tokens)
+  if (sl.dtype != at::kLong || !sl.contiguous() || sl.size[0] != tokens)
     paged_error("slots must be a contiguous int64 vector with one entry per token");
   const int32_t* pos = nullptr;
   if (!positions.is_none()) pos = static_cast<const int32_t*>(int_vector(positions, "positions", tokens, dev).ptr);
@@ -321,7 +235,7 @@ py::object store_kv(py::object k, py::object v, py::object k_cache, py::object v
     const View cv = view(cos, "cos", 2, dev), sv = view(sin, "sin", 2, dev);
     const int64_t half = kc.size[3] / 2;
     for (const View* x : {&cv, &sv})
-      if (x->dtype != t.dtypes[FA_F32] || !x->contiguous() || x->size[1] != half || x->size[0] != cv.size[0])
+      if (x->dtype != at::kFloat || !x->contiguous() || x->size[1] != half || x->size[0] != cv.size[0])
         paged_error("cos and sin must be contiguous float32 [positions, head_dim / 2] tensors");
     if (!rope_theta.is_none()) paged_error("give cos and sin or rope_theta, not both");
     cp = static_cast<const float*>(cv.ptr);
@@ -334,19 +248,19 @@ py::object store_kv(py::object k, py::object v, py::object k_cache, py::object v
     if (max_position.is_none()) paged_error("rope_theta needs max_position, one past the largest position");
     rows = max_position.cast<int64_t>();
   }
-  OnDevice guard(dev);
-  py::object out = py::none();
+  const OnDevice guard = on_device(dev);
+  at::Tensor out;
   void *qp = nullptr, *qo = nullptr;
   if (has_q) {
     out = empty({tokens, qv.size[1], qv.size[2]}, kc.dtype, dev);
     if (tokens > 0 && qv.size[1] > 0) {
       qp = qv.ptr;
-      qo = ptr_of(out);
+      qo = out.data_ptr();
     }
   }
   check_status(fa_store_kv(&p, kn.ptr, vn.ptr, kc.ptr, vc.ptr, static_cast<const int64_t*>(sl.ptr), pos, cp, sp,
                            u32(rows, "max_position"), theta, qp, qo, stream_of(dev)));
-  return out;
+  return has_q ? wrap(out) : py::none();
 }
 
 // ----------------------------------------------------- attention over pages
@@ -355,7 +269,6 @@ py::object attention(py::object q, py::object k_cache, py::object v_cache, const
                      bool is_causal, py::object cu_seqlens_q, py::object max_seqlen_q, float softcap,
                      py::object window_size, py::object alibi_slopes, py::object out_dtype, bool return_lse,
                      py::object out) {
-  const Torch& t = torch_names();
   Device dev;
   const View qv = view(q, "q", 3, dev);
   const View kc = view(k_cache, "k_cache", 4, dev), vc = view(v_cache, "v_cache", 4, dev);
@@ -369,7 +282,7 @@ py::object attention(py::object q, py::object k_cache, py::object v_cache, const
   const View lens = int_vector(seq_lens, "seq_lens", -1, dev);
   const int64_t b = lens.size[0];
   const View tb = view(block_table, "block_table", 2, dev);
-  if (tb.dtype != t.i32) paged_error("block_table must be int32");
+  if (tb.dtype != at::kInt) paged_error("block_table must be int32");
   if (tb.size[0] != b) paged_error("block_table must have one row per request");
   if (tb.size[1] > 1 && tb.stride[1] != 1) paged_error("block_table needs a unit innermost stride");
   p.batch_size = u32(b, "batch");
@@ -389,7 +302,7 @@ py::object attention(py::object q, py::object k_cache, py::object v_cache, const
   }
   if (!alibi_slopes.is_none()) {
     const View al = view(alibi_slopes, "alibi_slopes", 1, dev);
-    if (al.dtype != t.dtypes[FA_F32] || !al.contiguous() || al.size[0] != qv.size[1])
+    if (al.dtype != at::kFloat || !al.contiguous() || al.size[0] != qv.size[1])
       paged_error("alibi_slopes must hold one float32 slope per query head");
     p.alibi_slopes = static_cast<const float*>(al.ptr);
   }
@@ -422,35 +335,35 @@ py::object attention(py::object q, py::object k_cache, py::object v_cache, const
     if (oc < 0) paged_error("out_dtype must be float16, bfloat16 or float32");
   }
   p.out_dtype = oc;
-  OnDevice guard(dev);
+  const OnDevice guard = on_device(dev);
   void* op;
   if (out.is_none()) {
-    out = empty({qv.size[0], qv.size[1], qv.size[2]}, t.dtypes[oc], dev);
-    op = ptr_of(out);
+    out = wrap(empty({qv.size[0], qv.size[1], qv.size[2]}, type_of(oc), dev));
+    op = THPVariable_Unpack(out.ptr()).data_ptr();
   } else {
     const View ov = view(out, "out", 3, dev);
     if (ov.size[0] != qv.size[0] || ov.size[1] != qv.size[1] || ov.size[2] != qv.size[2])
       paged_error("out has the wrong shape");
-    if (ov.dtype != t.dtypes[oc]) paged_error("out has the wrong dtype");
+    if (ov.dtype != type_of(oc)) paged_error("out has the wrong dtype");
     unit_inner(ov, "out");
     no_overlap(ov, "out");
     copy_strides(ov, 2, p.o_stride, "out");
     op = ov.ptr;
   }
-  py::object lse = py::none();
+  at::Tensor lse;
   float* lp = nullptr;
   if (return_lse) {
-    lse = empty({qv.size[1], qv.size[0]}, t.dtypes[FA_F32], dev);
-    lp = static_cast<float*>(ptr_of(lse));
+    lse = empty({qv.size[1], qv.size[0]}, at::kFloat, dev);
+    lp = static_cast<float*>(lse.data_ptr());
   }
   // The scratch is the call's own: torch hands it out on the current stream
   // (and, while a graph is captured, from that graph's memory).
   const size_t bytes = fa_paged_workspace_size(&p);
-  py::object ws = empty({(int64_t)bytes}, t.u8, dev);
+  const at::Tensor ws = empty({(int64_t)bytes}, at::kByte, dev);
   check_status(fa_paged_forward(&p, qv.ptr, kc.ptr, vc.ptr, static_cast<const int32_t*>(tb.ptr),
-                                static_cast<const int32_t*>(lens.ptr), cu, pre, op, lp, ptr_of(ws), bytes,
+                                static_cast<const int32_t*>(lens.ptr), cu, pre, op, lp, ws.data_ptr(), bytes,
                                 stream_of(dev)));
-  if (return_lse) return py::make_tuple(out, lse);
+  if (return_lse) return py::make_tuple(out, wrap(lse));
   return out;
 }
 
@@ -473,7 +386,8 @@ py::object shared_prefix_forward(py::object q, py::object k_cache, py::object v_
 
 }  // namespace
 
-void bind_paged(py::module_& m) {
+PYBIND11_MODULE(_flash_attn_paged, m) {
+  m.doc() = "Paged KV cache: planning, append, attention over pages (CUDA torch tensors)";
   m.def("plan_pages", &plan_pages, py::arg("cached_lens"), py::arg("new_lens"), py::arg("block_table"),
         py::arg("free_pages"), py::arg("page_size"), py::arg("total_new"), py::kw_only(),
         py::arg("free_begin") = py::none(),

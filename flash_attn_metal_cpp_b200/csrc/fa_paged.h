@@ -3,6 +3,7 @@
 // side (fa_paged_api.cu).
 #pragma once
 
+#include <atomic>
 #include <cstdint>
 #include <string>
 
@@ -67,6 +68,19 @@ struct StoreArgs {
   unsigned* status;
 };
 cudaError_t launch_store_kv(const StoreArgs& a, int dtype, bool vec, cudaStream_t stream);
+
+// Lets a kernel use `bytes` of dynamic shared memory on the current device:
+// asked of the driver once a device (`done`: one bit each).
+inline cudaError_t allow_smem(const void* kernel, int bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
 
 // Division by a number known on the host, for numerators below 2^31:
 // n / d = (umulhi(n, m) + n) >> s with s = ceil(log2 d) and

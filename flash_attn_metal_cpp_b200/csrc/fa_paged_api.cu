@@ -237,6 +237,18 @@ Choice choose(const fa_paged_params* p, const Checked& c, bool vec, bool one) {
   return h;
 }
 
+// Every choice the tensors' base addresses (bit 0: 16-byte aligned) and
+// cu_seqlens_q (bit 1: none) can lead to; returns the scratch of the largest.
+size_t choose_all(const fa_paged_params* p, const Checked& c, Choice (&all)[4]) {
+  size_t bytes = 0;
+  for (int i = 0; i < 4; ++i) {
+    if ((i & 1) && !c.vec) continue;
+    all[i] = choose(p, c, (i & 1) != 0, (i & 2) != 0);
+    bytes = std::max(bytes, all[i].bytes);
+  }
+  return bytes;
+}
+
 cudaError_t launch_tc(const PagedArgs& a, const PagedTc& t, int dtype, const CUtensorMap& tk, const CUtensorMap& tv,
                       cudaStream_t s) {
   if (a.D <= 64)
@@ -368,14 +380,8 @@ fa_status fa_store_kv(const fa_paged_params* p, const void* k, const void* v, vo
 size_t fa_paged_workspace_size(const fa_paged_params* p) {
   Checked c;
   if (check(p, &c) != FA_OK) return 0;
-  const PagedArgs& a = c.a;
-  // Whatever the tensors' base addresses and cu_seqlens_q turn out to be.
-  size_t ws = 0;
-  for (int i = 0; i < 4; ++i) {
-    if ((i & 1) && !c.vec) continue;
-    ws = std::max(ws, choose(p, c, (i & 1) != 0, (i & 2) != 0).bytes);
-  }
-  return ws;
+  Choice all[4];
+  return choose_all(p, c, all);
 }
 
 fa_status fa_paged_forward(const fa_paged_params* p, const void* q, const void* k_cache, const void* v_cache,
@@ -390,7 +396,8 @@ fa_status fa_paged_forward(const fa_paged_params* p, const void* q, const void* 
   if (!q || !o || !seq_lens || (a.max_pages && !block_table) || (a.pre && !prefix_table) ||
       (a.num_pages && (!k_cache || !v_cache)))
     return paged_fail(FA_ERR_INVALID_ARG, "NULL tensor pointer");
-  const size_t need = fa_paged_workspace_size(p);
+  Choice all[4];
+  const size_t need = choose_all(p, c, all);
   if (!workspace || workspace_bytes < need)
     return paged_fail(FA_ERR_INVALID_ARG, "workspace smaller than fa_paged_workspace_size()");
   if (!aligned(workspace, 256)) return paged_fail(FA_ERR_INVALID_ARG, "workspace must be 256-byte aligned");
@@ -408,7 +415,7 @@ fa_status fa_paged_forward(const fa_paged_params* p, const void* q, const void* 
   a.lse = lse;
   a.wait_limit_ns = paged_wait_limit_ns();
   const bool vec = c.vec && aligned(q, 16) && aligned(k_cache, 16) && aligned(v_cache, 16);
-  const Choice h = choose(p, c, vec, cu_seqlens_q == nullptr);
+  const Choice& h = all[(vec ? 1 : 0) + (cu_seqlens_q == nullptr ? 2 : 0)];
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   a.n_parts = h.n_parts;
   a.own_part = h.n_parts > 0 && !h.many ? h.pre_split : -1;

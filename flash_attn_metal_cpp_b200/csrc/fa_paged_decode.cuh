@@ -521,7 +521,8 @@ cudaError_t launch(const PagedArgs& a, cudaStream_t st) {
   constexpr int smem = smem_bytes<DM, MT>();
   static_assert(smem <= 227 * 1024 && Cfg<DM, MT>::BLOCKS * (smem + 1024) <= 228 * 1024, "shared memory");
   auto kern = paged_decode_kernel<T, DM, MT>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<unsigned long long> done{0};
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), smem, done);
   if (e != cudaSuccess) return e;
   e = launch_pdl(kern, dim3((unsigned)a.n_ctas), dim3(kThreads), smem, st, a);
   note_launch();

@@ -692,7 +692,8 @@ template <int D, typename T, int XF>
 cudaError_t launch_xf(const PagedArgs& a, const PagedTc& tc, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t st) {
   auto kern = paged_attn_sm100<D, T, XF>;
   constexpr int smem = Cfg<D>::SMEM_BYTES;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<unsigned long long> done{0};
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), smem, done);
   if (e != cudaSuccess) return e;
   const long long blocks = (long long)tc.n_blocks * a.Hk * tc.n_split;
   if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
