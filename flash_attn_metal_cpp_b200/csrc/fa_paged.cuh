@@ -43,13 +43,6 @@ __device__ __forceinline__ float cvt_in<__nv_bfloat16>(__nv_bfloat16 x) { return
 // 64 to 32769 tokens: 262 us, 297 us without).
 constexpr int kUnitCost = 2;
 
-// 64-bit quotient of non-negative numbers; a 64-bit division takes some 300
-// cycles, and almost every call's numbers fit 32 bits.
-__device__ __forceinline__ long long div_ll(long long x, long long y) {
-  if (((x | y) >> 32) == 0) return (unsigned)x / (unsigned)y;
-  return x / y;
-}
-
 // One request: its query rows, its keys, and the key tiles any of its rows sees.
 struct ReqView {
   int q0, qlen;      // query tokens
@@ -59,7 +52,7 @@ struct ReqView {
   int units;         // chunks * Hk
   // What a unit and the request add to the line (uncut work counts units).
   __device__ __forceinline__ int per_unit(const PagedArgs& a) const { return a.split ? tiles + kUnitCost : 1; }
-  __device__ __forceinline__ long long work(const PagedArgs& a) const { return (long long)units * per_unit(a); }
+  __device__ __forceinline__ int work(const PagedArgs& a) const { return units * per_unit(a); }
 };
 
 // Lengths and tables. Read past L1 by a kernel that has not waited for the one
@@ -96,71 +89,102 @@ __device__ __forceinline__ ReqView view_request(const PagedArgs& a, int i, int r
   return r;
 }
 
+// Equal runs of a line of `total`: the first total % n are one longer. (The
+// host cuts work only while the line is shorter than 2^31.)
+struct Cuts {
+  int quot, rest, n;
+  __device__ __forceinline__ Cuts(int total, int runs) : n(runs) {
+    quot = (unsigned)total / (unsigned)runs;
+    rest = total - quot * runs;
+  }
+  __device__ __forceinline__ int begin(int run) const { return quot * run + min(run, rest); }
+  // First run that begins at or behind `at`.
+  __device__ __forceinline__ int first_from(int at) const {
+    const int longer = rest * (quot + 1);
+    if (at <= longer) return (unsigned)(at + quot) / (unsigned)(quot + 1);
+    return rest + (unsigned)(at - longer + quot - 1) / (unsigned)quot;
+  }
+};
+
 // The run of one block: [begin, end) of the line. A cut that falls on a unit's
 // own cost, not on its tiles, is moved to the unit's beginning.
 struct Run {
-  long long begin, end, total;
+  int begin, end, total;
   int n_runs;
   int req;                 // request the run begins in
-  long long req_begin;     // where that request begins
+  int req_begin;           // where that request begins
   ReqView view;            // of that request
 };
 
 // Sums up the line and finds the block's run. Every thread of the block calls
-// it; `sh` is shared scratch. A run has at least `min_run` of the line:
-// shorter runs cost more in joining than they save.
+// it; `sh` is shared scratch. A run has at least PagedArgs::min_run of the
+// line: shorter runs cost more in joining than they save.
 struct RunScratch {
-  long long part[8];
-  long long req_begin[2], cut[2];
-  int req[2];
+  int part[8];
+  int req_begin[2], cut[2], req[2];
   ReqView view;
 };
 template <int TN, int NTHREADS>
-__device__ __forceinline__ Run find_run(const PagedArgs& a, int rows_per_unit, int block, int n_blocks, int min_run,
-                                        RunScratch* sh) {
+__device__ __forceinline__ Run find_run(const PagedArgs& a, int rows_per_unit, RunScratch* sh) {
   constexpr int NW = NTHREADS / 32;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int seg = (a.B + NTHREADS - 1) / NTHREADS;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, block = blockIdx.x;
+  Run r;
+  if (a.units_per_req > 0) {
+    // Uncut units, as many in every request: no sum is needed.
+    r.n_runs = gridDim.x;
+    r.total = r.n_runs;
+    r.req = a.by_units(block);
+    r.req_begin = r.req * a.units_per_req;
+    r.view = view_request<TN>(a, r.req, rows_per_unit);
+    r.begin = block;
+    r.end = r.view.units > 0 ? block + 1 : block;  // (q may have fewer rows than requests)
+    return r;
+  }
+  const int seg = a.B <= NTHREADS ? 1 : (unsigned)(a.B + NTHREADS - 1) / NTHREADS;
   const int i0 = min(tid * seg, a.B), i1 = min(i0 + seg, a.B);
-  long long sum = 0;
   ReqView mine;  // the first of this thread's requests (mostly its only one)
+  int sum = 0;
+#pragma unroll 1
   for (int i = i0; i < i1; ++i) {
     const ReqView v = view_request<TN>(a, i, rows_per_unit);
     if (i == i0) mine = v;
     sum += v.work(a);
   }
-  long long inc = sum;
+  int inc = sum;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, inc, off);
+    const int v = __shfl_up_sync(0xffffffffu, inc, off);
     if (lane >= off) inc += v;
   }
   if (lane == 31) sh->part[warp] = inc;
   if (tid < 2) sh->req[tid] = -1;
   __syncthreads();
-  long long before = 0, total = 0;
+  int before = 0, total = 0;
 #pragma unroll
   for (int w = 0; w < NW; ++w) {
     if (w < warp) before += sh->part[w];
     total += sh->part[w];
   }
-  Run r;
   r.total = total;
-  r.n_runs = (int)min((long long)n_blocks, max(1ll, div_ll(total, a.split ? min_run : 1)));
+  r.n_runs = min((int)gridDim.x, max(1, a.split ? a.by_min_run(total) : total));
   r.begin = r.end = 0;
   if (total == 0 || block >= r.n_runs) return r;
-  const long long at = before + inc - sum;
-#pragma unroll
+  const int at = before + inc - sum;
+  const Cuts cuts(total, r.n_runs);
+#pragma unroll 1
   for (int e = 0; e < 2; ++e) {
-    const long long cut = div_ll(total * (block + e), r.n_runs);
-    if (sum > 0 && cut >= at && cut < at + sum) {
-      long long b = at;
+    const int cut = cuts.begin(block + e);
+    if (cut >= at && cut < at + sum) {
+      int b = at;
+      ReqView v = mine;
+#pragma unroll 1
       for (int i = i0; i < i1; ++i) {
-        const ReqView v = i == i0 ? mine : view_request<TN>(a, i, rows_per_unit);
-        const long long w = v.work(a);
+        if (i > i0) v = view_request<TN>(a, i, rows_per_unit);
+        const int w = v.work(a);
         if (cut < b + w) {
           if (e == 0) sh->view = v;
-          const long long unit_begin = b + div_ll(cut - b, v.per_unit(a)) * v.per_unit(a);
+          const int per = v.per_unit(a);
+          const int unit_begin = b + (int)((unsigned)(cut - b) / (unsigned)per) * per;
           sh->req[e] = i;
           sh->req_begin[e] = b;
           sh->cut[e] = cut - unit_begin <= kUnitCost ? unit_begin : cut;
@@ -172,6 +196,7 @@ __device__ __forceinline__ Run find_run(const PagedArgs& a, int rows_per_unit, i
   }
   __syncthreads();
   r.req = sh->req[0];
+  if (r.req < 0) return r;  // (offsets that overlap can make a sum no request holds)
   r.req_begin = sh->req_begin[0];
   r.view = sh->view;
   r.begin = sh->cut[0];
@@ -180,7 +205,7 @@ __device__ __forceinline__ Run find_run(const PagedArgs& a, int rows_per_unit, i
 }
 
 // First tile (counted from the unit's first) at `off` of a unit's stretch.
-__device__ __forceinline__ int tile_at(long long off) { return off <= kUnitCost ? 0 : (int)(off - kUnitCost); }
+__device__ __forceinline__ int tile_at(int off) { return off <= kUnitCost ? 0 : off - kUnitCost; }
 
 // Table entry of key `key` of a request and its slot in the page. The entry
 // is not checked here, so that the load can stay in flight: valid_page does.

@@ -143,7 +143,9 @@ struct PagedArgs {
   // per run two partial units of rows_per_unit rows, and where they belong.
   int split;
   int n_ctas;
-  int min_run;             // least length of a run
+  Div by_min_run;          // least length of a run
+  int units_per_req;       // uncut work, one block a unit (0: the kernel sums up the requests)
+  Div by_units;
   int rows_per_unit;
   int join_rows;           // most rows a unit can have here (for the join's grid)
   float* slot_o;           // [n_ctas, 2, rows_per_unit, D] unnormalised
@@ -156,10 +158,10 @@ struct PagedArgs {
 // Where one run of the cut work begins (written by the attention kernel, read
 // by the join).
 struct RunMeta {
-  long long begin;         // of the run, in the call's line of work
-  long long unit_begin;    // of the unit it begins in
-  long long unit_end;
-  long long total;         // length of the line
+  int begin;               // of the run, in the call's line of work
+  int unit_begin;          // of the unit it begins in
+  int unit_end;
+  int total;               // length of the line
   int n_runs;              // runs in use (0: run not in use)
   int q0;                  // first query row of the unit's request
   int row0;                // first packed row of the unit (row = token * group + head of the group)

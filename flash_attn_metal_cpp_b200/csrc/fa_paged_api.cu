@@ -140,6 +140,7 @@ struct Choice {
   int own_split, pre_split;        // parts the keys are cut in
   int own_blocks, pre_blocks;      // blocks of 256 packed rows
   int rows_per_unit, n_ctas, join_rows, split;
+  int units_per_req;
   int n_parts;                     // whole-row partial results to join (0: none)
   CutLayout cut;
   size_t parts_lse, parts_o, bytes;  // offsets of the partial results
@@ -217,14 +218,17 @@ Choice choose(const fa_paged_params* p, const Checked& c, bool vec, bool one) {
     // times as many keys. (One request of 400 keys, 8 KV heads, D = 128: 14.0
     // us uncut; of 1000 keys, cut: 12.8 us; 4 requests of 512, 16 heads, D =
     // 64: 10.6 us uncut, 12.0 us cut.)
-    const long long chunks = one ? (long long)a.B * ((a.group + h.rows_per_unit - 1) / h.rows_per_unit)
-                                 : all_rows / h.rows_per_unit + a.B;
+    const long long per_req = (a.group + h.rows_per_unit - 1) / h.rows_per_unit * a.Hk;
+    const long long units = one ? a.B * per_req : (all_rows / h.rows_per_unit + a.B) * a.Hk;
     const long long few = h.tensor ? 32768 : 16384;
-    h.split = keys * a.D > (chunks * a.Hk >= h.n_ctas ? 4 * few : few);
+    h.split = keys * a.D > (units >= h.n_ctas ? 4 * few : few);
+    // The line the kernels cut is counted in 32 bits.
+    if (units * (keys / 32 + 4) >= (1ll << 31)) h.split = 0;
     if (!h.split) {
-      h.n_ctas = (int)std::min<long long>(chunks * a.Hk, 148 * 16);
+      h.n_ctas = (int)std::min<long long>(units, one ? 1 << 30 : 148 * 16);
+      h.units_per_req = one && units <= (1 << 30) ? (int)per_req : 0;
     }
-    h.cut = cut_layout(h.n_ctas, h.rows_per_unit, a.D);
+    h.cut = cut_layout(h.split ? h.n_ctas : 0, h.rows_per_unit, a.D);
     h.bytes = h.cut.bytes;
   }
   // Whole-row partial results: the prefix's, then the own keys' (the few-rows
@@ -240,7 +244,7 @@ Choice choose(const fa_paged_params* p, const Checked& c, bool vec, bool one) {
 // Every choice the tensors' base addresses (bit 0: 16-byte aligned) and
 // cu_seqlens_q (bit 1: none) can lead to; returns the scratch of the largest.
 size_t choose_all(const fa_paged_params* p, const Checked& c, Choice (&all)[4]) {
-  size_t bytes = 0;
+  size_t bytes = 256;  // (0 means invalid parameters)
   for (int i = 0; i < 4; ++i) {
     if ((i & 1) && !c.vec) continue;
     all[i] = choose(p, c, (i & 1) != 0, (i & 2) != 0);
@@ -459,7 +463,9 @@ fa_status fa_paged_forward(const fa_paged_params* p, const void* q, const void* 
     // Shortest run (kUnitCost + 1 at least): one request of 1000 keys, 8 KV
     // heads, D = 128: 12.8 us with 3, 13.7 us with 4; CUDA cores, 32 units of
     // 600 keys and D = 128: 29 us with 3, 23.5 us with 4.
-    a.min_run = h.tensor || a.D <= 64 ? 3 : 4;
+    a.by_min_run = Div(h.tensor || a.D <= 64 ? 3 : 4);
+    a.units_per_req = h.units_per_req;
+    a.by_units = Div(std::max(1, h.units_per_req));
     a.split = h.split;
     place_cut(a, h.cut, workspace);
     a.late_wait = h.shared;

@@ -99,7 +99,7 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 // Steps through the tiles of a run: request, unit (chunk of rows, KV head), tile.
 template <int MR>
 struct Cursor {
-  long long left;        // of the line, from the unit's beginning on
+  int left;              // of the line, from the unit's beginning on
   int req, unit, per;    // per: a unit's stretch of the line
   int hk, row0;          // of the unit
   int tile, tile_end;    // of the current piece, from the unit's first tile
@@ -120,9 +120,9 @@ struct Cursor {
     req = run.req;
     v = run.view;
     per = v.per_unit(a);
-    const long long off = run.begin - run.req_begin;
-    unit = (int)div_ll(off, per);
-    const long long in_unit = off - (long long)unit * per;
+    const int off = run.begin - run.req_begin;
+    unit = (unsigned)off / (unsigned)per;
+    const int in_unit = off - unit * per;
     left = run.end - run.begin + in_unit;
     const int chunk = a.by_hk(unit);
     hk = unit - chunk * a.Hk;
@@ -159,7 +159,11 @@ struct Cursor {
         if (++unit == v.units) {
           unit = hk = row0 = 0;
           do {
-            v = view_request<kTile>(a, ++req, MR);
+            if (++req >= a.B) {
+              left = 0;
+              return;
+            }
+            v = view_request<kTile>(a, req, MR);
           } while (v.units == 0);
           per = v.per_unit(a);
         }
@@ -189,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
   // one is done too" for the join that follows.
   if (!a.late_wait) grid_dep_wait();
   grid_dep_launch_dependents();
-  const Run run = find_run<kTile, kThreads>(a, MR, blockIdx.x, gridDim.x, a.min_run, &sh.scratch);
+  const Run run = find_run<kTile, kThreads>(a, MR, &sh.scratch);
   if (run.end <= run.begin) {
     if (a.split && tid == 0) a.meta[blockIdx.x].n_runs = 0;
     if (a.late_wait) grid_dep_wait();
@@ -200,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
   if (a.split && tid == 0) {
     RunMeta& mt = a.meta[blockIdx.x];
     mt.begin = run.begin;
-    mt.unit_begin = run.req_begin + (long long)cur.unit * cur.per;
+    mt.unit_begin = run.req_begin + cur.unit * cur.per;
     mt.unit_end = mt.unit_begin + cur.per;
     mt.total = run.total;
     mt.n_runs = run.n_runs;
@@ -266,9 +270,9 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
   };
 
   {
-    // Prologue: the first NS tiles' page numbers together, then the copies of
-    // NS - 1 of them. The loops stay rolled where they can: this code runs
-    // once, and its instructions come from L2.
+    // The first NS tiles' page numbers together. Loops stay rolled here, and
+    // the first copies are issued by the main loop's code: what runs once a
+    // block waits for its instructions from L2 longer than for anything else.
 #pragma unroll 1
     for (int i = 0; i < NS; ++i) {
       TileDesc d;
@@ -282,8 +286,6 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
 #pragma unroll
     for (int i = 0; i < NS; ++i) put_rows(i, ps[i], sh.desc[i].hk);
     __syncthreads();
-#pragma unroll 1
-    for (int i = 0; i < NS - 1; ++i) issue(i, i);
   }
 
   uint32_t qf[MT][KK][4];
@@ -295,14 +297,23 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
   const float cap_in = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
   const float cap_log2 = a.softcap * kLog2e;
 
-  int di = 0, st = 0;  // slots of the current tile
+  int di = 0, st = 0;          // slot and stage of the current tile
+  int di_in = 0, st_in = 0;    // of the next tile to be copied
+  int ahead = NS - 1;          // copies to issue before the first tile is awaited
   while (true) {
-    cp_async_wait<NS - 2>();
-    __syncthreads();
+    if (ahead == 0) {
+      cp_async_wait<NS - 2>();
+      __syncthreads();
+      if (sh.desc[di].rows == 0) break;
+    }
+    issue(di_in, st_in);
+    di_in = di_in == NS ? 0 : di_in + 1;
+    st_in = st_in == NS - 1 ? 0 : st_in + 1;
+    if (ahead > 0) {
+      --ahead;
+      continue;
+    }
     const TileDesc& d = sh.desc[di];
-    if (d.rows == 0) break;
-    const int di_issue = di + NS - 1 > NS ? di - 2 : di + NS - 1;   // (di + NS - 1) mod (NS + 1)
-    issue(di_issue, st == 0 ? NS - 1 : st - 1);
     TileDesc dn;
     cur.next(a, dn);
     const int2 pn = look_up(dn);

@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
 
   grid_dep_wait();
   grid_dep_launch_dependents();
-  const Run run = find_run<kTile, kThreads>(a, R, blockIdx.x, gridDim.x, a.min_run, &scratch);
+  const Run run = find_run<kTile, kThreads>(a, R, &scratch);
   if (run.end <= run.begin) {
     if (a.split && tid == 0) a.meta[blockIdx.x].n_runs = 0;
     return;
@@ -75,19 +75,20 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
   const T* V = reinterpret_cast<const T*>(a.v);
 
   int req = run.req;
-  long long req_begin = run.req_begin;
+  int req_begin = run.req_begin;
   ReqView v = run.view;
-  long long at = run.begin;
+  int at = run.begin;
   while (at < run.end) {
     const int per = v.per_unit(a);
-    const long long off = at - req_begin;
-    if (off >= (long long)v.units * per) {
-      req_begin += (long long)v.units * per;
-      v = view_request<kTile>(a, ++req, R);
+    const int off = at - req_begin;
+    if (off >= v.units * per) {
+      req_begin += v.units * per;
+      if (++req >= a.B) break;
+      v = view_request<kTile>(a, req, R);
       continue;
     }
-    const int unit = (int)div_ll(off, per);
-    const long long unit_begin = req_begin + (long long)unit * per;
+    const int unit = (unsigned)off / (unsigned)per;
+    const int unit_begin = req_begin + unit * per;
     const int t_end = v.tile_lo + v.tiles;
     const int t0 = v.tile_lo + (a.split ? tile_at(at - unit_begin) : 0);
     const int t1 = a.split && run.end < unit_begin + per ? v.tile_lo + tile_at(run.end - unit_begin) : t_end;
@@ -251,12 +252,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const Paged
   const RunMeta mt = a.meta[b];
   if (mt.n_runs == 0 || r >= mt.rows || mt.begin == mt.unit_begin) return;
   // Run b - 1 begins in the unit's tiles too: its block joins the unit.
-  const long long prev = div_ll(mt.total * (b - 1), mt.n_runs);
+  const Cuts cuts(mt.total, mt.n_runs);
+  const int prev = cuts.begin(b - 1);
   if (prev - mt.unit_begin > kUnitCost) return;
-  const int first = b - 1;
-  // One past the last run that begins before the unit's end:
-  // floor(total j / n) < e for all j < e n / total.
-  const int last = (int)min((long long)mt.n_runs, div_ll(mt.unit_end * mt.n_runs + mt.total - 1, mt.total));
+  const int first = b - 1, last = min(mt.n_runs, cuts.first_from(mt.unit_end));
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int sd = (a.D + 3) & ~3;
   auto row_of = [&](int run) {

@@ -203,6 +203,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (i == i0) mine = v;
       n += blocks_of(v);
     }
+    if (threadIdx.x == 0) bars->work.req = -1;
     int total;
     int at = scan_block(n, bars->part, &total);
     const int want = total - 1 - bi;
@@ -223,6 +224,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncthreads();
     b = bars->work;
+    if (b.req < 0) {  // (offsets that overlap can make a sum no request holds)
+      leave();
+      return;
+    }
   }
 
   if (tc.shared && a.win_left >= 0) __syncthreads();  // min_ahead
