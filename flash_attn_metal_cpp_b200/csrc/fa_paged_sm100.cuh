@@ -41,6 +41,7 @@ constexpr uint32_t kRegsLaunch = 168, kRegsSoftmax = 216, kRegsOther = 72;
 static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsOther <= kThreads * kRegsLaunch, "register split exceeds launch");
 constexpr uint32_t kTmemCols = 512, kColS = 0, kColO = 256;
 constexpr float kRescaleThreshold = 8.0f;
+constexpr float kFastCap = 256.f;
 
 template <int D>
 struct Cfg {
@@ -103,7 +104,17 @@ __device__ __forceinline__ int scan_block(int x, int* part, int* total) {
 }
 
 // XF: what a score goes through before the softmax. 0: scale alone (positive);
-// 1: any scale, ALiBi; 2: the tanh cap, any scale, ALiBi.
+// 1: any scale, ALiBi; 2: the tanh cap with a positive scale, caps up to
+// kFastCap; 3: the tanh cap, any size and scale, ALiBi.
+//
+// XF 2 uses cap tanh(y) = cap (1 - 2 r), r = 1 / (1 + e^(2y)), which is
+// monotone in the score: the row maximum is taken of the raw scores, and the
+// weight is exp2(cap' - m - 2 cap' r) with cap' = cap log2(e). Two scores share
+// one reciprocal (r1 = d2 R, r2 = d1 R, R = 1 / (d1 d2); e^(2y) is held below
+// 2^40, where r is below 2^-40 anyway, so the product stays finite): 2.5
+// special-function operations a score instead of 3, and 5 others. r is off by
+// at most 2^-22.5, the score by 2^-21 cap; caps beyond kFastCap take XF 3,
+// whose tanh is exact in the relative sense.
 template <int D, typename T, int XF>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_attn_sm100(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -477,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (row_ok) {
       if (tc.shared) {
         row_hi = b.klen;
-        if (a.causal || a.win_left >= 0 || a.win_right >= 0 || XF != 0) {
+        if (a.causal || a.win_left >= 0 || a.win_right >= 0 || (XF & 1) != 0) {
           int i = tok;
           if (a.cu_q != nullptr) {
             int lo = 0, hi = a.B;  // the last request that begins at or before the token
@@ -501,8 +512,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         row_hi = see.y;
       }
     }
-    const float slope = (XF != 0 && a.alibi != nullptr) ? a.alibi[head] * kLog2e : 0.f;
-    const float cap_in = XF == 2 ? a.scale / a.softcap : 0.f, cap_log2 = a.softcap * kLog2e;
+    const float slope = ((XF & 1) != 0 && a.alibi != nullptr) ? a.alibi[head] * kLog2e : 0.f;
+    const float cap_in = XF >= 2 ? a.scale / a.softcap : 0.f, cap_log2 = a.softcap * kLog2e;
     const float sl2 = XF == 0 ? a.scale_log2 : 1.f;
     const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t tS = lane_base + kColS + t * 128;
@@ -527,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int c = 0; c < BN; ++c) s[c] = fmaf(s[c], a.scale_log2, slope * (base + (float)c));
       }
-      if constexpr (XF == 2) {
+      if constexpr (XF == 3) {
         const float base = (float)(kv0 - qpos);
 #pragma unroll
         for (int c = 0; c < BN; ++c) s[c] = fmaf(cap_log2, cap_tanh(s[c] * cap_in), slope * (base + (float)c));
@@ -540,7 +551,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int c = 0; c < BN; ++c) ext = fmaxf(ext, (c < key_lim && c >= key_beg) ? s[c] : -INFINITY);
       }
-      const float m_new = fmaxf(m_run, ext * sl2);
+      // (XF 2: e^(2y) and the score of the row maximum)
+      const float cap_k = cap_in * (2.f * kLog2e);
+      float m_cand = ext * sl2;
+      if constexpr (XF == 2)
+        m_cand = ext == -INFINITY ? -INFINITY
+                                  : cap_log2 * (1.f - __fdividef(2.f, 1.f + ex2_approx(fminf(ext * cap_k, 40.f))));
+      const float m_new = fmaxf(m_run, m_cand);
       const bool grow = m_new > m_run + kRescaleThreshold;
       const bool any_grow = __any_sync(0xffffffffu, grow);
       const float m_use = any_grow ? m_new : m_run;
@@ -557,7 +574,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
-      const float2 sc2 = make_float2(sl2, sl2), nm2 = make_float2(-m_sub, -m_sub);
+      // The exponent of a weight is u * sc2 + nm2: u the score, XF 2: r.
+      const float sc = XF == 2 ? -2.f * cap_log2 : sl2, nm = XF == 2 ? cap_log2 - m_sub : -m_sub;
+      const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(nm, nm);
+      auto exponents = [&](float s0, float s1) {
+        float2 u = make_float2(s0, s1);
+        if constexpr (XF == 2) {
+          const float2 d = __fadd2_rn(make_float2(ex2_approx(fminf(s0 * cap_k, 40.f)), ex2_approx(fminf(s1 * cap_k, 40.f))),
+                                      make_float2(1.f, 1.f));
+          const float inv = __fdividef(1.f, d.x * d.y);
+          u = make_float2(d.y * inv, d.x * inv);
+        }
+        return __ffma2_rn(u, sc2, nm2);
+      };
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t p[32];
@@ -565,8 +594,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             const int c = h * 64 + 2 * i;
-            const float p0 = (c < key_lim && c >= key_beg) ? ex2_approx(fmaf(s[c], sl2, -m_sub)) : 0.f;
-            const float p1 = (c + 1 < key_lim && c + 1 >= key_beg) ? ex2_approx(fmaf(s[c + 1], sl2, -m_sub)) : 0.f;
+            // (a masked score may be NaN and shares its reciprocal: it goes first)
+            const bool on0 = c < key_lim && c >= key_beg, on1 = c + 1 < key_lim && c + 1 >= key_beg;
+            const float2 x = exponents(on0 ? s[c] : 0.f, on1 ? s[c + 1] : 0.f);
+            const float p0 = on0 ? ex2_approx(x.x) : 0.f, p1 = on1 ? ex2_approx(x.y) : 0.f;
             acc0 = __fadd2_rn(acc0, make_float2(p0, p1));
             p[i] = pack_p<T>(p0, p1);
           }
@@ -574,7 +605,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             const int c = h * 64 + 2 * i;
-            const float2 x = __ffma2_rn(make_float2(s[c], s[c + 1]), sc2, nm2);
+            const float2 x = exponents(s[c], s[c + 1]);
             const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
             if (i & 1) acc1 = __fadd2_rn(acc1, e);
             else acc0 = __fadd2_rn(acc0, e);
@@ -709,7 +740,9 @@ cudaError_t launch_xf(const PagedArgs& a, const PagedTc& tc, const CUtensorMap& 
 
 template <int D, typename T>
 cudaError_t launch_dt(const PagedArgs& a, const PagedTc& tc, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t st) {
-  if (a.softcap > 0.f) return launch_xf<D, T, 2>(a, tc, tk, tv, st);
+  if (a.softcap > 0.f && a.softcap <= kFastCap && a.scale > 0.f && a.alibi == nullptr)
+    return launch_xf<D, T, 2>(a, tc, tk, tv, st);
+  if (a.softcap > 0.f) return launch_xf<D, T, 3>(a, tc, tk, tv, st);
   if (a.alibi != nullptr || !(a.scale > 0.f)) return launch_xf<D, T, 1>(a, tc, tk, tv, st);
   return launch_xf<D, T, 0>(a, tc, tk, tv, st);
 }
