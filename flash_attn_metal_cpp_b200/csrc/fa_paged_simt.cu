@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const Paged
 template <int W>
 __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedArgs a) {
   constexpr int R = 8 / W;  // rows a block
-  __shared__ float sm_o[8][128];
+  __shared__ __align__(16) float sm_o[8][128];
   __shared__ float sm_m[8], sm_l[8];
   grid_dep_wait();
   grid_dep_launch_dependents();
