@@ -130,6 +130,7 @@ struct PagedArgs {
   float* lse;              // [Hq, total_q] natural log (NULL = not written)
   float scale, scale_log2;
   float softcap;           // > 0: x = softcap * tanh(scale * q.k / softcap)
+  float cap_in;            // scale / softcap
   int causal, win_left, win_right;
   const float* alibi;      // [Hq] (NULL = none)
   // Partial results of whole rows, joined by a last kernel: normalised o

@@ -93,6 +93,8 @@ fa_status check(const fa_paged_params* p, Checked* c, bool grouped = true) {
   a.scale = p->softmax_scale;
   a.scale_log2 = (float)((double)p->softmax_scale * 1.4426950408889634);
   a.softcap = p->softcap;
+  // (finite for the smallest caps: 0 * cap_in stays 0)
+  if (a.softcap > 0.f) a.cap_in = std::max(-1e37f, std::min(1e37f, a.scale / a.softcap));
   a.causal = p->is_causal ? 1 : 0;
   a.win_left = p->window_left < 0 ? -1 : std::min(p->window_left, 1 << 30);
   a.win_right = p->window_right < 0 ? -1 : std::min(p->window_right, 1 << 30);
@@ -183,7 +185,7 @@ Choice choose(const fa_paged_params* p, const Checked& c, bool vec, bool one) {
   Choice h{};
   const long long rows = max_rows(p, a, one);
   const long long all_rows = (long long)a.total_q * a.group;
-  const long long own_keys = (long long)a.max_pages * a.page_size;
+  const long long own_keys = a.max_len;
   // 16-bit rows of whole 16-byte pieces go to the tensor cores; fp32 and
   // everything that cannot be copied in such pieces to the CUDA cores.
   h.tensor = c.dtype != kF32 && vec && a.num_pages > 0;

@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
   int lo[MT][2], hi[MT][2], qpos[MT][2];
   int full_lo = 0, full_hi = 0;  // keys that every row of the unit sees
   const bool plain = a.softcap == 0.f && a.alibi == nullptr && a.scale > 0.f;
-  const float cap_in = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
+  const float cap_in = a.cap_in;
   const float cap_log2 = a.softcap * kLog2e;
 
   int di = 0, st = 0;          // slot and stage of the current tile
@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
           const int2 see = visible_keys(a, d.klen, qpos[mt][e]);
           lo[mt][e] = see.x;
           hi[mt][e] = see.y;
-          slope[mt][e] = a.alibi ? a.alibi[d.hk * a.group + row - j * a.group] * kLog2e : 0.f;
+          slope[mt][e] = a.alibi ? __ldcg(a.alibi + d.hk * a.group + row - j * a.group) * kLog2e : 0.f;
           m[mt][e] = -INFINITY;
           l[mt][e] = 0.f;
         }

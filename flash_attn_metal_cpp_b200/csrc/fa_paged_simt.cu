@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
           s += __shfl_xor_sync(0xffffffffu, s, 4);
           if (on[u] && key >= vis[r].x && key < vis[r].y) {
             float x;
-            if (a.softcap > 0.f) x = a.softcap * tanhf(s * a.scale / a.softcap);
+            if (a.softcap > 0.f) x = a.softcap * tanhf(s * a.cap_in);
             else x = s * a.scale;
             x = fmaf(slope[r], (float)(key - qpos[r]), x) * kLog2e;
             // (a score of -inf, an overflow, leaves the row as it is)

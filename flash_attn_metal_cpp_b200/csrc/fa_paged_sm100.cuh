@@ -520,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     const float slope = ((XF & 1) != 0 && a.alibi != nullptr) ? a.alibi[head] * kLog2e : 0.f;
-    const float cap_in = XF >= 2 ? a.scale / a.softcap : 0.f, cap_log2 = a.softcap * kLog2e;
+    const float cap_in = a.cap_in, cap_log2 = a.softcap * kLog2e;
     const float sl2 = XF == 0 ? a.scale_log2 : 1.f;
     const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t tS = lane_base + kColS + t * 128;

@@ -262,6 +262,83 @@ def test_bad_pages_and_lengths_are_reported(fa, cuda_device):
                     ref.assert_attention(o[s], w[s], tol[s], what)
 
 
+@pytest.mark.parametrize("d", [8, 16, 40, 56, 64, 72, 88, 104, 120, 128])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_head_dims_of_prompt_chunks(fa, cuda_device, d, dtype):
+    b = Batch(cuda_device, [300, 129, 40], qlens=[200, 129, 33], d=d, hq=4, hk=2, dtype=dtype)
+    b.check(fa, f"d {d}", causal=True)
+    b.check(fa, f"d {d} capped", causal=True, cap=20.0)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("cap", [1e-30, 1e-3, 300.0, 1e4, 1e30])
+@pytest.mark.parametrize("qlens", [None, [100, 60]])
+def test_caps_of_any_size(fa, cuda_device, dtype, cap, qlens):
+    """A cap far above the scores changes nothing, one far below makes the weights equal."""
+    b = Batch(cuda_device, [150, 70], qlens=qlens, d=64, dtype=dtype)
+    o = b.run(fa, softcap=cap, out_dtype="float32")
+    torch.cuda.synchronize()
+    exact_cap = 0.0 if cap > 1e6 else cap
+    w, _, tol, _ = b.want(out_dtype=FP, cap=exact_cap)
+    if 256 < cap <= 1e6:  # 2^-20 cap is the reference's allowance; beyond 256 the kernels are relatively exact
+        w0, _, tol0, _ = b.want(out_dtype=FP)
+        ref.assert_attention(o, w, tol0 + (w - w0).abs() * 2.0 ** -10, "cap")
+    else:
+        ref.assert_attention(o, w, tol, "cap")
+
+
+@pytest.mark.parametrize("hint", [1, 3, 1000])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_max_seqlen_is_only_a_hint(fa, cuda_device, hint, dtype):
+    b = Batch(cuda_device, [300, 90, 200], qlens=[150, 1, 70], d=64, dtype=dtype)
+    o = fa.paged_forward(b.q, b.k_cache, b.v_cache, b.table, b.seq, b.scale, True, cu_seqlens_q=b.cu, max_seqlen_q=hint)
+    p = fa.paged_forward(b.q, b.k_cache, b.v_cache, b.table, b.seq, b.scale, True, cu_seqlens_q=b.cu)
+    torch.cuda.synchronize()
+    fa.check_status()
+    w, _, tol, _ = b.want(True)
+    ref.assert_attention(o, w, tol, "hint")
+    ref.assert_attention(p, w, tol, "no hint")
+
+
+def test_offsets_out_of_order_are_reported(fa, cuda_device):
+    """Offsets that fall, overlap or leave q give unspecified rows, no access outside q and a report."""
+    for dtype in (BF, FP):
+        for n in (1, 60):
+            b = Batch(cuda_device, [100, 90, 300], qlens=[n, n, n], d=64, dtype=dtype, width=64)
+            for cu in ([0, 3 * n, 0, 3 * n], [0, n, 5 * n, 3 * n], [-7, n, 2 * n, 1 << 30], [2 * n, n, 0, 3 * n]):
+                fa.paged_forward(b.q, b.k_cache, b.v_cache, b.table, b.seq, b.scale, True, max_seqlen_q=n,
+                                 cu_seqlens_q=torch.tensor(cu, dtype=torch.int32, device=cuda_device))
+                torch.cuda.synchronize()
+                with pytest.raises(RuntimeError, match="outside its cache"):
+                    fa.check_status()
+            b.check(fa, "after", causal=True, use_cu=True)
+
+
+def test_broadcast_heads_and_unaligned_rows(fa, cuda_device):
+    for qlens in ([1, 1], [70, 50]):
+        b = Batch(cuda_device, [300, 90], qlens=qlens, hq=4, hk=1, d=64, dtype=BF)
+        b.k_cache, b.v_cache = (c.expand(-1, -1, 2, -1) for c in (b.k_cache, b.v_cache))  # one row for two KV heads
+        b.check(fa, "broadcast heads", causal=True)
+        b = Batch(cuda_device, [300, 90], qlens=qlens, hq=4, hk=2, d=64, dtype=BF)
+        flat = torch.zeros(b.q.numel() + 1, dtype=BF, device=cuda_device)
+        flat[1:] = b.q.flatten()
+        b.q = flat[1:].view(b.q.shape)
+        b.check(fa, "unaligned q", causal=True)
+        out = torch.zeros(b.q.numel() + 1, dtype=BF, device=cuda_device)[1:].view(b.q.shape)
+        b.q = b.q.clone()
+        b.run(fa, True, out=out)
+        w, _, tol, _ = b.want(True)
+        ref.assert_attention(out, w, tol, "unaligned out")
+
+
+def test_wide_tables(fa, cuda_device):
+    """A table with room for a million tokens a request, as a graph for any length has."""
+    for dtype in (BF, FP):
+        for qlens in (None, [40, 100, 64]):
+            b = Batch(cuda_device, [50, 300, 64], qlens=qlens, d=64, dtype=dtype, width=65536)
+            b.check(fa, "wide", causal=True)
+
+
 # -------------------------------------------------------------- shared prefix
 @pytest.mark.parametrize("dtype", [BF, HF, FP])
 @pytest.mark.parametrize("prefix", [1, 16, 100, 128, 1037])
@@ -288,6 +365,22 @@ def test_shared_prefix_odd_sizes(fa, cuda_device, d, page):
     for dtype in (BF, FP):
         b = Batch(cuda_device, [1, 30, 77], hq=12, hk=3, d=d, dtype=dtype, prefix=401, page=page)
         b.check(fa, "odd")
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("d", [40, 64, 128])
+@pytest.mark.parametrize("opts", [{}, dict(cap=25.0), dict(cap=400.0), dict(window=(2500, -1)), dict(window=(50, -1)),
+                                  dict(window=(-1, 3)), "alibi", dict(scale=-0.1)])
+@pytest.mark.parametrize("qlens", [None, [1, 3, 2, 0, 4, 1]])
+def test_prefix_shared_beside_single_tokens(fa, cuda_device, dtype, d, opts, qlens):
+    """Prefixes long enough to be computed once for the batch while its own keys take the few-rows kernel."""
+    n = 40 if qlens is None else 6
+    prefix = 16e6 / (n * 2 * d * 4) // 1 + 3
+    lens = [max((i * 29) % 90, 4) for i in range(n)]
+    b = Batch(cuda_device, lens, qlens=qlens, hq=6, hk=2, d=d, dtype=dtype, prefix=int(prefix), page=48)
+    if opts == "alibi":
+        opts = dict(slopes=torch.tensor([2.0 ** -(i + 3) for i in range(6)], device=cuda_device))
+    b.check(fa, str(opts), causal=qlens is not None, **opts)
 
 
 def test_shared_prefix_large_batch(fa, cuda_device):
@@ -321,7 +414,7 @@ def _plan_case(dev, cached, new, page, rows, width, n_free, begin, seed=0):
     ([0], [1], 16, 1), ([15, 16, 17, 0, 31], [1, 1, 1, 1, 1], 16, 5), ([0, 0, 5], [0, 0, 0], 4, 3),
     ([3, 0, 100, 7], [50, 1, 0, 9], 8, 70), (list(range(300)), [1] * 300, 16, 300),
     ([i % 40 for i in range(1500)], [(i * 7) % 5 for i in range(1500)], 3, 3100), ([5000, 12], [2500, 4000], 64, 6500),
-    ([1, 2], [3, 4], 1, 7)])
+    ([1, 2], [3, 4], 1, 7), ([i % 90 for i in range(8192)], [1] * 8192, 32, 8200)])
 @pytest.mark.parametrize("begin", [None, 3])
 def test_plan_pages(fa, cuda_device, cached, new, page, rows, begin):
     width = max(-(-(c + n) // page) for c, n in zip(cached, new)) + 2

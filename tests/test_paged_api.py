@@ -7,6 +7,7 @@ import math
 import os
 import shutil
 import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -166,3 +167,14 @@ def test_plan_reference():
     table, lens, cu, slots, pos, end = ref.plan([3, 4], [2, 1], [[9, -1, -1], [7, -1, -1]], [1, 2, 3], 4, 5)
     assert table == [[9, 1, -1], [7, 2, -1]] and lens == [5, 5] and cu == [0, 2, 3] and end == 2
     assert slots == [39, 4, 8, -1, -1] and pos == [3, 4, 4, 0, 0]
+
+
+def test_module_loads_the_operators_on_first_use():
+    """The module and the package import without torch; the first paged name loads its extension and torch."""
+    code = ("import sys, flash_attn_metal_cpp_b200 as p, _flash_attn_metal as m\n"
+            "assert 'torch' not in sys.modules\n"
+            "assert not hasattr(m, 'no_such_name') and not hasattr(p, 'no_such_name')\n"
+            "assert m.store_kv is p.store_kv and m.plan_pages is p.plan_pages and 'torch' in sys.modules\n"
+            "from flash_attn_metal_cpp_b200 import paged_forward, shared_prefix_forward\n"
+            "assert paged_forward.__module__ == '_flash_attn_paged'\n")
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=ROOT)
