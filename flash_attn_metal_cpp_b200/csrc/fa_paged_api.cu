@@ -149,19 +149,26 @@ struct Choice {
 };
 
 // Parts that the keys of `blocks` blocks (256 rows, up to `tiles` tiles of
-// 128 keys) are cut in. A wave of 148 blocks takes one tile in about 2.1 us
-// (D = 128), a block about 2 tiles more to begin and end; every part writes
-// and reads its partial rows once (about 5 TB/s). One part needs no join.
-int choose_parts(long long blocks, long long tiles, int D, double row_bytes, bool join_anyway) {
-  const double tile = D <= 64 ? 1.3e-6 : 2.1e-6;
-  const int top = (int)std::max(1ll, std::min(32ll, tiles / 2));
+// 128 keys) are cut in. A wave of 148 blocks takes one tile in 2.15 us (D =
+// 128; 1.8 at 64) and about 14 us more to begin and end (64 blocks of 256
+// tiles: 568 us in 1 part, 315 in 2 = one wave, 368 in 4 = two waves, 375 in 9
+// = four); every part writes
+// and reads its partial rows once (about 5 TB/s). One part needs no join. With
+// the few-rows kernel running `beside`, a single wave leaves it a quarter of
+// the SMs, or costs its time (some 10 us) on top. (24 requests of 4 tokens, 8
+// heads on one KV head, a prefix of 50001 keys: 74 us with 16 parts, 52 with
+// 31, 56 with 49.)
+int choose_parts(long long blocks, long long tiles, int D, double row_bytes, bool join_anyway, bool beside) {
+  const double tile = D <= 64 ? 1.8e-6 : 2.15e-6;
+  const int top = (int)std::max(1ll, std::min(64ll, tiles / 2));
   int best = 1;
   double best_cost = 0;
   for (int n = 1; n <= top; ++n) {
     const double waves = (double)((blocks * n + 147) / 148);
-    double cost = waves * (double)((tiles + n - 1) / n + 2) * tile;
+    double cost = waves * ((double)((tiles + n - 1) / n) * tile + 14e-6);
     if (n > 1 || join_anyway) cost += 2.0 * n * row_bytes / 5e12;
     if (n > 1 && !join_anyway) cost += 3e-6;  // the join's own launch
+    if (beside && blocks * n > 112 && blocks * n <= 148) cost += 10e-6;
     if (n == 1 || cost < best_cost) {
       best = n;
       best_cost = cost;
@@ -198,11 +205,11 @@ Choice choose(const fa_paged_params* p, const Checked& c, bool vec, bool one) {
   const double row_bytes = (double)a.total_q * a.Hq * a.D * 4;
   if (h.shared) {
     h.pre_blocks = (int)((all_rows + 255) / 256);
-    h.pre_split = choose_parts((long long)h.pre_blocks * a.Hk, (a.pre + 127) / 128, a.D, row_bytes, true);
+    h.pre_split = choose_parts((long long)h.pre_blocks * a.Hk, (a.pre + 127) / 128, a.D, row_bytes, true, !h.many);
   }
   if (h.many) {
     h.own_blocks = (int)(one ? (long long)a.B * ((a.group + 255) / 256) : (all_rows + 255) / 256 + a.B);
-    h.own_split = choose_parts((long long)h.own_blocks * a.Hk, (own_keys + 127) / 128, a.D, row_bytes, h.shared);
+    h.own_split = choose_parts((long long)h.own_blocks * a.Hk, (own_keys + 127) / 128, a.D, row_bytes, h.shared, false);
   }
   if (!h.many) {
     if (h.tensor) {

@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int first = 0, last = 0;
     if (k_hi > k_lo) {
       const int t0 = k_lo / BN, n = (k_hi + BN - 1) / BN - t0;
-      // (n < 2^23 tiles, at most 32 parts)
+      // (n < 2^23 tiles, at most 64 parts)
       first = t0 + tc.by_split(n * split);
       last = t0 + tc.by_split(n * (split + 1));
     }
