@@ -87,8 +87,9 @@ __device__ __forceinline__ uint32_t pack_p(float lo, float hi) {
   else return pack_bf162(lo, hi);
 }
 
-// Sum of one int per thread before the calling thread (and the total).
-__device__ __forceinline__ int scan_block(int x, int* part, int* total) {
+// Sum of one int per thread before the calling thread (and the total); only
+// the first `warps` warps have any.
+__device__ __forceinline__ int scan_block(int x, int warps, int* part, int* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int inc = x;
 #pragma unroll
@@ -99,8 +100,8 @@ __device__ __forceinline__ int scan_block(int x, int* part, int* total) {
   if (lane == 31) part[warp] = inc;
   __syncthreads();
   int before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) {
+#pragma unroll 1
+  for (int w = 0; w < warps; ++w) {
     if (w < warp) before += part[w];
     all += part[w];
   }
@@ -223,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (threadIdx.x == 0) bars->work.req = -1;
     int total;
-    int at = scan_block(n, bars->part, &total);
+    int at = scan_block(n, a.B >= kThreads ? kThreads / 32 : (a.B + 31) / 32, bars->part, &total);
     const int want = total - 1 - bi;
     if (want < 0) {
       leave();
@@ -476,9 +477,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t q_at = row_ok ? (int64_t)tok * a.q_st + (int64_t)head * a.q_sh : -1;
       const int c = lane % CH;
       const uint32_t dst = sQ + t * C::TILE_BYTES + (warp & 3) * 32 * 128 + (c >> 3) * C::BOX_BYTES;
-      // Rolled, here and where the output leaves: this code runs once a block,
-      // and fetching unrolled instructions took longer than the copies.
-#pragma unroll 1
+      // Hardly unrolled, here and where the output leaves: this code runs once
+      // a block, and fetching its instructions takes longer than the copies.
+#pragma unroll 4
       for (int i = 0; i < CH; ++i) {
         const int r = i * RPI + lane / CH;
         const int64_t at = row_at(q_at, r);
@@ -646,12 +647,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (ok && b.row0 + t * BM < b.rows) {
       const float inv_l = (l_run > 0.f) ? 1.f / l_run : 0.f;
       const float lse = (l_run > 0.f) ? (m_run + log2f(l_run)) * kLn2 : -INFINITY;
-      // 16 columns of the row's O, divided by the sum.
-      auto take16 = [&](int col, float (&x)[16]) {
-        uint32_t u[16];
-        if (my_kv > 0) tmem_ld16(tO + col, u);
+      // 32 columns of the row's O, divided by the sum.
+      auto take32 = [&](int col, float (&x)[32]) {
+        uint32_t u[32];
+        if (my_kv > 0) tmem_ld32(tO + col, u);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = my_kv > 0 ? __uint_as_float(u[i]) * inv_l : 0.f;
+        for (int i = 0; i < 32; ++i) x[i] = my_kv > 0 ? __uint_as_float(u[i]) * inv_l : 0.f;
       };
       const int part = tc.part0 + split;
       const int64_t prow = ((int64_t)part * a.total_q + tok) * a.Hq + head;
@@ -676,19 +677,19 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
         for (int pass = 0; pass < passes; ++pass) {
 #pragma unroll 1
-          for (int k = 0; k < cols; k += 16) {
-            float x[16];
-            take16(pass * cols + k, x);
+          for (int k = 0; k < cols; k += 32) {
+            float x[32];
+            take32(pass * cols + k, x);
             uint8_t* to = buf + r * (D * 2);
             const int sw = r & 7;
             if (dt == kF32) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
+              for (int i = 0; i < 8; ++i)
                 *reinterpret_cast<float4*>(to + (((k / 4 + i) ^ sw) << 4)) =
                     make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
             } else {
 #pragma unroll
-              for (int i = 0; i < 2; ++i) {
+              for (int i = 0; i < 4; ++i) {
                 const float* y = x + 8 * i;
                 *reinterpret_cast<uint4*>(to + (((k / 8 + i) ^ sw) << 4)) =
                     dt == kF16 ? make_uint4(pack_half2(y[0], y[1]), pack_half2(y[2], y[3]), pack_half2(y[4], y[5]), pack_half2(y[6], y[7]))
@@ -711,11 +712,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       } else {
         // Rows that start anywhere: element by element.
 #pragma unroll 1
-        for (int k = 0; k < D; k += 16) {
-          float x[16];
-          take16(k, x);
+        for (int k = 0; k < D; k += 32) {
+          float x[32];
+          take32(k, x);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < 8; ++i) {
             const float y[4] = {x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
             if (row_ok && k + 4 * i < a.D) store_out4(a.o, o_at + k + 4 * i, a.out_dtype, y, 4);
           }
