@@ -89,7 +89,7 @@ def _torch_flags() -> tuple[list[str], list[str]]:
               "-isystem", os.path.join(CUDA_HOME, "include"),
               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
     lib = os.path.join(root, "lib")
-    return cflags, ["-L", lib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python", f"-Wl,-rpath,{lib}"]
+    return cflags, ["-L", lib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python", f"-Wl,-rpath,{lib}"]
 
 
 def _extension(path: str, src: str, cflags: list[str], libs: list[str], force: bool) -> None:

@@ -10,6 +10,7 @@
 // `_flash_attn_metal` loads when one of them is first used: the rest of the
 // module works without torch.
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -94,7 +95,8 @@ View int_vector(py::handle o, const char* what, int64_t n, Device& dev) {
 }
 
 at::Tensor empty(at::IntArrayRef shape, at::ScalarType dtype, const Device& dev) {
-  return at::empty(shape, at::TensorOptions().dtype(dtype).device(at::Device(at::kCUDA, (c10::DeviceIndex)dev.index)));
+  // (what at::empty ends in, without the dispatcher on the way)
+  return at::detail::empty_cuda(shape, dtype, at::Device(at::kCUDA, (c10::DeviceIndex)dev.index), std::nullopt);
 }
 
 py::object wrap(const at::Tensor& t) { return py::reinterpret_steal<py::object>(THPVariable_Wrap(t)); }
