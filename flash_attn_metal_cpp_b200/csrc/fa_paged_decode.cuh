@@ -189,14 +189,15 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
   // nothing of it and may run beside it, on the SMs it leaves free. All blocks
   // of that kernel have waited for everything before it by the time they let
   // this one start, so lengths, tables and caches are complete (and read from
-  // L2); waiting at the end instead keeps "this kernel is done" meaning "that
-  // one is done too" for the join that follows.
+  // L2). One block waits at its end instead, so that "this kernel is done"
+  // still means "that one is done too" for the join that follows; the others
+  // make room for the next block when their run is finished.
   if (!a.late_wait) grid_dep_wait();
   grid_dep_launch_dependents();
   const Run run = find_run<kTile, kThreads>(a, MR, &sh.scratch);
   if (run.end <= run.begin) {
     if (a.split && tid == 0) a.meta[blockIdx.x].n_runs = 0;
-    if (a.late_wait) grid_dep_wait();
+    if (a.late_wait && blockIdx.x == 0) grid_dep_wait();
     return;
   }
   Cursor<MR> cur;
@@ -524,7 +525,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
     st = st == NS - 1 ? 0 : st + 1;
   }
   cp_async_wait<0>();
-  if (a.late_wait) grid_dep_wait();
+  if (a.late_wait && blockIdx.x == 0) grid_dep_wait();
 }
 
 template <typename T, int DM, int MT>
