@@ -692,7 +692,9 @@ fa_status paged_rope(float theta, int D, int rows, cudaStream_t stream, const fl
     *sn = it->second.sn;
     return FA_OK;
   }
-  return rope_from_theta(ds, theta, D, rows, stream, cs, sn);
+  st = rope_from_theta(ds, theta, D, rows, stream, cs, sn);
+  if (st != FA_OK) cudaGetLastError();  // (tables too large) reported here, not by the next call
+  return st;
 }
 
 fa_status paged_encode(CUtensorMap* m, const void* base, bool bf16, int D, int H, int slots, int pages, int64_t sp,

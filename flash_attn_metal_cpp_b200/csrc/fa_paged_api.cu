@@ -18,7 +18,9 @@ size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 fa_status cuda_status(cudaError_t e, const char* what) {
-  return e == cudaSuccess ? FA_OK : paged_fail(FA_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+  if (e == cudaSuccess) return FA_OK;
+  cudaGetLastError();  // reported here, not by the next call
+  return paged_fail(FA_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
 }
 
 struct Checked {

@@ -30,6 +30,10 @@ class Batch:
             base = torch.randn((n_pages, page, hk, d), generator=g, device=dev).to(dtype)
             if layout == "NHPD":
                 base = base.transpose(1, 2).contiguous().transpose(1, 2)
+            elif layout == "paired":  # K and V pages side by side in one tensor
+                both = torch.zeros((n_pages, 2, page, hk, d), dtype=dtype, device=dev)
+                both[:, 1] = base
+                base = both[:, 1]
             elif layout == "odd":  # rows at element strides that no vector load can take
                 wide = torch.zeros((n_pages, page, hk, d + 1), dtype=dtype, device=dev)
                 wide[..., :d] = base
@@ -121,7 +125,7 @@ def test_head_dims(fa, cuda_device, dtype, d):
     b.check(fa, f"d {d}", causal=True)
 
 
-@pytest.mark.parametrize("layout", ["NHPD", "odd"])
+@pytest.mark.parametrize("layout", ["NHPD", "paired", "odd"])
 @pytest.mark.parametrize("dtype", [BF, FP])
 @pytest.mark.parametrize("qlens", [[1, 1, 1], [90, 1, 200]])
 def test_cache_strides(fa, cuda_device, layout, dtype, qlens):
@@ -153,6 +157,17 @@ def test_scores_and_masks(fa, cuda_device, dtype, qlens, opts):
     elif opts == "all":
         opts = dict(slopes=slopes, cap=15.0, window=(200, -1))
     b.check(fa, str(opts), causal=True, **opts)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("qlens", [[5, 3, 1], [70, 40, 90]])
+def test_more_tokens_than_keys(fa, cuda_device, dtype, qlens):
+    """Rows whose position lies before the first key see nothing under a causal mask."""
+    for prefix in (0, 20):
+        b = Batch(cuda_device, [2, 0, 30], qlens=qlens, d=64, dtype=dtype, prefix=prefix)
+        b.check(fa, "short", causal=True)
+        b.check(fa, "short", causal=True, window=(3, -1))
+        b.check(fa, "short full")
 
 
 def test_large_scores(fa, cuda_device):
@@ -630,6 +645,71 @@ def test_captured_step_follows_the_lengths(fa, cuda_device, dtype, prefix):
         w, _, tol, _ = x.want()
         ref.assert_attention(o, w, tol, "two streams")
     del keep
+
+
+def test_captured_serving_step(fa, cuda_device):
+    """Planning, append and attention of a decoding step in one graph; each replay is the next step."""
+    n, page, hq, hk, d, dev = 4, 16, 8, 2, 64, cuda_device
+    kc, vc = (torch.full((40, page, hk, d), math.nan, dtype=HF, device=dev) for _ in range(2))
+    table = torch.full((n, 8), -1, dtype=torch.int32, device=dev)
+    free = torch.randperm(40, device=dev).to(torch.int32)
+    cached, new = torch.zeros(n, dtype=torch.int32, device=dev), torch.ones(n, dtype=torch.int32, device=dev)
+    begin = torch.zeros(1, dtype=torch.int32, device=dev)
+    q, k, v = (torch.empty((n, h, d), dtype=HF, device=dev) for h in (hq, hk, hk))
+
+    def step():
+        lens, _, slots, pos, end = fa.plan_pages(cached, new, table, free, page, n, free_begin=begin)
+        qr = fa.store_kv(k, v, kc, vc, slots, q=q, positions=pos, rope_theta=1e4, max_position=256)
+        o = fa.paged_forward(qr, kc, vc, table, lens, d ** -0.5)
+        cached.copy_(lens)
+        begin.copy_(end)
+        return qr, o
+
+    def reset():
+        cached.copy_(torch.tensor([0, 15, 16, 31], dtype=torch.int32))
+        begin.zero_()
+        table.fill_(-1)
+        for t in (kc, vc):
+            t.fill_(math.nan)
+        # what the requests hold already
+        zero = torch.zeros(n, dtype=torch.int32, device=dev)
+        _, _, slots, _, end = fa.plan_pages(zero, cached, table, free, page, 62, free_begin=begin)
+        x = torch.randn((62, hk, d), device=dev).half()
+        fa.store_kv(x, x, kc, vc, slots)
+        begin.copy_(end)
+
+    for t in (q, k, v):
+        t.normal_()
+    reset()
+    step()
+    torch.cuda.synchronize()
+    reset()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        qr, o = step()
+    reset()
+    for i in range(20):
+        for t in (q, k, v):
+            t.normal_()
+        g.replay()
+        torch.cuda.synchronize()
+        fa.check_status()
+        lens = cached.tolist()
+        assert lens == [x + i + 1 for x in (0, 15, 16, 31)]
+        w, _, tol, _ = ref.attention(qr, kc, vc, table, lens, d ** -0.5)
+        ref.assert_attention(o, w, tol, f"step {i}")
+
+
+def test_an_error_does_not_reach_the_next_call(fa, cuda_device):
+    x = torch.ones((1, 1, 256), dtype=FP, device=cuda_device)
+    kc = torch.zeros((1, 16, 1, 256), dtype=FP, device=cuda_device)
+    slots, pos = (torch.zeros(1, dtype=t, device=cuda_device) for t in (torch.int64, torch.int32))
+    with pytest.raises(RuntimeError, match="cudaMalloc"):  # tables of 2^30 positions
+        fa.store_kv(x, x, kc, kc.clone(), slots, positions=pos, rope_theta=77.0, max_position=1 << 30)
+    q = torch.randn((1, 32, 2, 160), device=cuda_device)  # CUDA-core forward
+    fa.forward(q, q, q, 0.1)
+    fa.store_kv(x, x, kc, kc.clone(), slots)
+    torch.cuda.synchronize()
 
 
 def test_two_streams_eager(fa, cuda_device):
