@@ -223,16 +223,16 @@ Choice choose(const fa_paged_params* p, const Checked& c, bool vec, bool one) {
     }
     h.join_rows = (int)std::min<long long>(h.rows_per_unit, one ? (long long)a.group : all_rows);
     const long long keys = own_keys + (h.shared ? 0 : a.pre);
-    // A unit of few keys is not worth cutting: its block takes about 1 us a
-    // tile of 64 keys at D = 128 (0.8 us at 64, CUDA cores more), the join 4 to
-    // 5 us. With more units than blocks cutting balances little up to four
-    // times as many keys. (One request of 400 keys, 8 KV heads, D = 128: 14.0
-    // us uncut; of 1000 keys, cut: 12.8 us; 4 requests of 512, 16 heads, D =
-    // 64: 10.6 us uncut, 12.0 us cut.)
+    // A unit of few keys is not worth cutting: its block takes 0.6 to 1.2 us a
+    // tile of 64 keys, the join 4 us. One request on 8 KV heads, D = 128, uncut
+    // and cut: 250 keys 8.6 and 11.4 us, 380 keys 11.1 and 11.4, 500 keys 13.4
+    // and 12.5; 4 requests on 16 heads, D = 64: 250 keys 8.2 and 11.0, 500 keys
+    // 12.0 and 11.3; 40 requests on 8 heads, D = 128: 250 keys 18.2 and 17.4, 500
+    // keys 29 and 24. CUDA cores, 8 requests on 8 heads, D = 64: 120 keys 7.4 and
+    // 9.8, 250 keys 12.0 and 10.0.
     const long long per_req = (a.group + h.rows_per_unit - 1) / h.rows_per_unit * a.Hk;
     const long long units = one ? a.B * per_req : (all_rows / h.rows_per_unit + a.B) * a.Hk;
-    const long long few = h.tensor ? 32768 : 16384;
-    h.split = keys * a.D > (units >= h.n_ctas ? 4 * few : few);
+    h.split = keys > (h.tensor ? 384 : 160);
     // The line the kernels cut is counted in 32 bits.
     if (units * (keys / 32 + 4) >= (1ll << 31)) h.split = 0;
     if (!h.split) {
@@ -471,10 +471,9 @@ fa_status fa_paged_forward(const fa_paged_params* p, const void* q, const void* 
     a.rows_per_unit = h.rows_per_unit;
     a.n_ctas = h.n_ctas;
     a.join_rows = h.join_rows;
-    // Shortest run (kUnitCost + 1 at least): one request of 1000 keys, 8 KV
-    // heads, D = 128: 12.8 us with 3, 13.7 us with 4; CUDA cores, 32 units of
-    // 600 keys and D = 128: 29 us with 3, 23.5 us with 4.
-    a.by_min_run = Div(h.tensor || a.D <= 64 ? 3 : 4);
+    // Shortest run, kUnitCost + 1 (one request of 1000 keys, 8 KV heads, D =
+    // 128: 11.6 us, with 4 instead of 3 12.7 us).
+    a.by_min_run = Div(3);
     a.units_per_req = h.units_per_req;
     a.by_units = Div(std::max(1, h.units_per_req));
     a.split = h.split;

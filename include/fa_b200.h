@@ -344,7 +344,8 @@ fa_status fa_noalloc_check_status(void);
  * skipped, never followed, the rows that needed it are unspecified, and
  * fa_check_device_status then reports FA_ERR_BAD_INDEX. All entry points
  * enqueue on `stream` and return without synchronising; none allocates
- * (except the first use of a rope_theta, see fa_store_kv). */
+ * (except the first use of a rope_theta, see fa_store_kv). Limits: 2^29 - 1
+ * keys a request, total_q * num_heads_q <= 2^30, head_dim <= 256. */
 
 /* One step's pages, from the requests' lengths. For request i with cached[i]
  * tokens in the cache and fresh[i] tokens to append:
@@ -409,7 +410,8 @@ void fa_paged_params_init(fa_paged_params* p);
  * in fa_forward) or, when they are NULL, from the library's tables of
  * rope_theta with table_rows rows: the first call with a new theta or more
  * rows builds them (allocating and synchronising, so it is refused while the
- * stream is being captured). A position without a table row leaves its row
+ * stream is being captured; fa_pool_clear frees them, also under captured
+ * graphs that use them). A position without a table row leaves its row
  * unrotated and sets the status word. Rotation is computed in float32 and
  * rounded once. */
 fa_status fa_store_kv(const fa_paged_params* p, const void* k, const void* v, void* k_cache, void* v_cache,
