@@ -20,6 +20,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 namespace fa {
 
 // Bit of the bad-index status word.
@@ -266,6 +268,14 @@ __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wai
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.69314718055994531f;
+
+// The running maximum of the tensor-core kernels is held this much (log2 units)
+// below the true one, so weights reach 2^7 (2^15 where the many-rows kernel lets
+// its maximum lag by 2^8) and fp16 holds them with full precision down to 2^-21
+// of the largest, instead of 2^-14: thousands of small weights beside a large
+// one would otherwise be rounded off, or away. bf16 has the range anyway.
+template <typename T>
+__device__ constexpr float weight_bias() { return std::is_same<T, __half>::value ? 7.f : 0.f; }
 
 // tanh for the score cap of the tensor-core kernels: the odd series up to y^9
 // below 1/4 (its next term is under 2^-26 of the value there), else

@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
       for (int e = 0; e < 2; ++e) {
         top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
         top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
-        const float nm = fmaxf(m[mt][e], top[e] * mul);
+        const float nm = fmaxf(m[mt][e], top[e] * mul - weight_bias<T>());
         grow |= nm > m[mt][e];
         sub[e] = nm == -INFINITY ? 0.f : nm;
         f[e] = ex2_approx(m[mt][e] - sub[e]);  // 0 for the first keys of a row

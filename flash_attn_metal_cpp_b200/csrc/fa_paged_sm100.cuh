@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if constexpr (XF == 2)
         m_cand = ext == -INFINITY ? -INFINITY
                                   : cap_log2 * (1.f - __fdividef(2.f, 1.f + ex2_approx(fminf(ext * cap_k, 40.f))));
-      const float m_new = fmaxf(m_run, m_cand);
+      const float m_new = fmaxf(m_run, m_cand - weight_bias<T>());
       const bool grow = m_new > m_run + kRescaleThreshold;
       const bool any_grow = __any_sync(0xffffffffu, grow);
       const float m_use = any_grow ? m_new : m_run;

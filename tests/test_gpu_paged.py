@@ -178,6 +178,23 @@ def test_large_scores(fa, cuda_device):
         b.check(fa, "large capped", cap=5.0)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("far", [9.0, 13.0, 17.0])
+@pytest.mark.parametrize("qlens", [[1], [64]])
+def test_many_small_weights(fa, cuda_device, dtype, far, qlens):
+    """One key far above the others, whose value is 0: the output is what thousands of small weights add up to."""
+    for prefix in (0, 4000):
+        b = Batch(cuda_device, [20000], qlens=qlens, hq=8, hk=1, d=64, dtype=dtype, prefix=prefix, page=64)
+        b.k_cache.zero_()
+        b.v_cache.fill_(1.0)
+        b.q.zero_()
+        b.q[..., 0] = 8.0
+        page, slot = int(b.table[0, 3]), 11
+        b.k_cache[page, slot, :, 0] = far
+        b.v_cache[page, slot] = 0.0
+        b.check(fa, f"far {far}")
+
+
 @pytest.mark.parametrize("dtype", [BF, FP])
 @pytest.mark.parametrize("hk", [1, 8])
 def test_one_long_request(fa, cuda_device, dtype, hk):
