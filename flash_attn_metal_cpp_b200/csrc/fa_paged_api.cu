@@ -201,9 +201,16 @@ Choice choose(const fa_paged_params* p, const Checked& c, bool vec, bool one) {
   h.box = gcd(a.page_size, 128);
   const bool tma = h.tensor && a.D <= 128 && h.box >= 8 && a.k_sp > 0 && a.k_ss > 0 && a.k_sh > 0 && a.v_sp > 0 &&
                    a.v_ss > 0 && a.v_sh > 0;
+  // Above 32 rows the few-rows kernel reads the keys more than once. (16
+  // requests of 8000 keys, 32 heads on 8 KV heads: 16 rows 97 us and 119 in the
+  // many-rows kernel, 32 rows 103 and 119, 48 rows 245 and 119.)
   h.many = tma && rows > 32;
+  // A prefix is computed apart when each request's reading it (from L2) would
+  // cost more than a kernel and a join. (In this place and apart, D = 128, 8 KV
+  // heads: 8 requests of 500 keys, 16 MB, 13.6 and 16.2 us; of 1000 keys 16.3
+  // and 16.5; of 2000 keys 20.8 and 17.1; 64 requests of 600 keys 41 and 21.)
   h.shared = tma && a.pre > 0 &&
-             (h.many || (a.pre >= 256 && (double)a.B * a.pre * a.Hk * a.D * 4 >= 16e6));
+             (h.many || (a.B > 1 && a.pre >= 128 && (double)a.B * a.pre * a.Hk * a.D * 4 >= 32e6));
   const double row_bytes = (double)a.total_q * a.Hq * a.D * 4;
   if (h.shared) {
     h.pre_blocks = (int)((all_rows + 255) / 256);

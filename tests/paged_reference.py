@@ -3,7 +3,8 @@
 `attention` also returns, for every output element, how far a correct kernel may be off. With P the
 normalised weights and u the rounding of a probability that is fed to the tensor cores in the input
 type (half a step, relative: finfo.eps / 2; 0 for float32 inputs):
-  |dO| <= (u + 2 ds) (P |V|) + u_out |O|
+  |dO| <= (u + 2 ds) (P |V|) + u_out |O| + half the smallest step of the output type
+(float16 values below 2^-14 stand 2^-24 apart whatever their size, so their rounding is off by up to 2^-25)
 where ds bounds the error of a score (and so the relative error of an exponential, in numerator and
 denominator alike): products and sums of D terms in float32, (D + 8) 2^-24 scale sum |q_d k_d|, the
 cap's tanh 2^-20 cap, the bias 2^-22 |slope rel|, and 2^-18 for exponentials, running sums and joins.
@@ -15,6 +16,7 @@ import math
 import torch
 
 U = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
+STEP = {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134, torch.float32: 2.0 ** -150}
 
 
 def rows_of(cache, pages, n):
@@ -36,7 +38,7 @@ def attention(q, k_cache, v_cache, table, lens, scale, causal=False, starts=None
     lse = torch.full((hq, rows), math.nan, dtype=torch.float64, device=dev)
     lse_tol = torch.zeros_like(lse)
     u_p = 0.0 if q.dtype == torch.float32 else U[q.dtype]
-    u_out = U[out_dtype or q.dtype]
+    u_out, step = U[out_dtype or q.dtype], STEP[out_dtype or q.dtype]
     for i, n in enumerate(lens):
         a, b = starts[i], starts[i + 1]
         if a == b:
@@ -78,7 +80,7 @@ def attention(q, k_cache, v_cache, table, lens, scale, causal=False, starts=None
             o = p @ vh
             off = (u_p + 2 * torch.where(see, ds, torch.zeros_like(ds)).amax(1) if x.shape[1] else x.new_zeros(b - a))
             out[a:b, h] = o
-            tol[a:b, h] = off[:, None] * (p @ vh.abs()) + u_out * o.abs() + 1e-30
+            tol[a:b, h] = off[:, None] * (p @ vh.abs()) + u_out * o.abs() + step + 1e-30
             lse[h, a:b] = torch.where(empty, torch.full_like(m, -math.inf), m + torch.log(s))
             lse_tol[h, a:b] = off - u_p + 2.0 ** -22 * (m.abs() + 1)
     return out, lse, tol, lse_tol

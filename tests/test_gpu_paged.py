@@ -407,7 +407,7 @@ def test_shared_prefix_odd_sizes(fa, cuda_device, d, page):
 def test_prefix_shared_beside_single_tokens(fa, cuda_device, dtype, d, opts, qlens):
     """Prefixes long enough to be computed once for the batch while its own keys take the few-rows kernel."""
     n = 40 if qlens is None else 6
-    prefix = 16e6 / (n * 2 * d * 4) // 1 + 3
+    prefix = 32e6 / (n * 2 * d * 4) // 1 + 3
     lens = [max((i * 29) % 90, 4) for i in range(n)]
     b = Batch(cuda_device, lens, qlens=qlens, hq=6, hk=2, d=d, dtype=dtype, prefix=int(prefix), page=48)
     if opts == "alibi":
