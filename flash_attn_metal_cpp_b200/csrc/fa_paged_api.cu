@@ -46,6 +46,8 @@ fa_status check(const fa_paged_params* p, Checked* c, bool grouped = true) {
     return paged_fail(FA_ERR_INVALID_ARG, "tensor dimensions out of range");
   if (grouped && (uint64_t)p->total_q * p->num_heads_q > lim)
     return paged_fail(FA_ERR_INVALID_ARG, "total_q * num_heads_q must not exceed 2^30");
+  if (grouped && (uint64_t)p->batch_size * p->num_heads_q > lim)
+    return paged_fail(FA_ERR_INVALID_ARG, "batch_size * num_heads_q must not exceed 2^30");
   if (p->prefix_len > lim / 2 || (uint64_t)p->prefix_len > (uint64_t)p->prefix_pages * p->page_size)
     return paged_fail(FA_ERR_INVALID_ARG, "prefix_len is beyond the pages of the prefix table");
   if (!std::isfinite(p->softmax_scale)) return paged_fail(FA_ERR_INVALID_ARG, "softmax_scale must be finite");
@@ -154,12 +156,11 @@ struct Choice {
 // 128 keys) are cut in. A wave of 148 blocks takes one tile in 2.15 us (D =
 // 128; 1.8 at 64) and about 14 us more to begin and end (64 blocks of 256
 // tiles: 568 us in 1 part, 315 in 2 = one wave, 368 in 4 = two waves, 375 in 9
-// = four); every part writes
-// and reads its partial rows once (about 5 TB/s). One part needs no join. With
-// the few-rows kernel running `beside`, a single wave leaves it a quarter of
-// the SMs, or costs its time (some 10 us) on top. (24 requests of 4 tokens, 8
-// heads on one KV head, a prefix of 50001 keys: 74 us with 16 parts, 52 with
-// 31, 56 with 49.)
+// = four); every part writes and reads its partial rows once (about 5 TB/s).
+// One part needs no join. With the few-rows kernel running `beside`, a single
+// wave leaves it a quarter of the SMs, or costs its time (some 10 us) on top.
+// (24 requests of 4 tokens, 8 heads on one KV head, a prefix of 50001 keys: 74
+// us with 16 parts, 52 with 31, 56 with 49.)
 int choose_parts(long long blocks, long long tiles, int D, double row_bytes, bool join_anyway, bool beside) {
   const double tile = D <= 64 ? 1.8e-6 : 2.15e-6;
   const int top = (int)std::max(1ll, std::min(64ll, tiles / 2));
