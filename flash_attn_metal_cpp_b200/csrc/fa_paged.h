@@ -173,7 +173,7 @@ struct RunMeta {
 // CUDA-core kernel: fp32 inputs, and 16-bit inputs the tensor cores' copies
 // cannot take (any head_dim <= 256, any strides and alignment).
 int simt_rows_per_unit(int dtype, bool vec, int D, long long rows);
-int simt_ctas(int D);
+int simt_ctas(int D, int rows_per_unit);
 cudaError_t launch_paged_simt(const PagedArgs& a, int dtype, bool vec, cudaStream_t stream);
 // Tensor-core kernel for few rows (16-bit, rows of 16-byte pieces).
 int decode_rows_per_unit(int D, long long rows);

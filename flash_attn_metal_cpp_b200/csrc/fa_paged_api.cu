@@ -227,7 +227,7 @@ Choice choose(const fa_paged_params* p, const Checked& c, bool vec, bool one) {
       h.n_ctas = decode_ctas(a.D, h.rows_per_unit);
     } else {
       h.rows_per_unit = simt_rows_per_unit(c.dtype, vec, a.D, rows);
-      h.n_ctas = simt_ctas(a.D);
+      h.n_ctas = simt_ctas(a.D, h.rows_per_unit);
     }
     h.join_rows = (int)std::min<long long>(h.rows_per_unit, one ? (long long)a.group : all_rows);
     const long long keys = own_keys + (h.shared ? 0 : a.pre);
@@ -236,11 +236,11 @@ Choice choose(const fa_paged_params* p, const Checked& c, bool vec, bool one) {
     // and cut: 250 keys 8.6 and 11.4 us, 380 keys 11.1 and 11.4, 500 keys 13.4
     // and 12.5; 4 requests on 16 heads, D = 64: 250 keys 8.2 and 11.0, 500 keys
     // 12.0 and 11.3; 40 requests on 8 heads, D = 128: 250 keys 18.2 and 17.4, 500
-    // keys 29 and 24. CUDA cores, 8 requests on 8 heads, D = 64: 120 keys 7.4 and
-    // 9.8, 250 keys 12.0 and 10.0.
+    // keys 29 and 24. CUDA cores, 8 requests on 8 heads, D = 64: 160 keys 8.9 and
+    // 10.1, 200 keys 10.5 and 10.2, 250 keys 12.3 and 10.4.
     const long long per_req = (a.group + h.rows_per_unit - 1) / h.rows_per_unit * a.Hk;
     const long long units = one ? a.B * per_req : (all_rows / h.rows_per_unit + a.B) * a.Hk;
-    h.split = keys > (h.tensor ? 384 : 160);
+    h.split = keys > (h.tensor ? 384 : 192);
     // The line the kernels cut is counted in 32 bits.
     if (units * (keys / 32 + 4) >= (1ll << 31)) h.split = 0;
     if (!h.split) {

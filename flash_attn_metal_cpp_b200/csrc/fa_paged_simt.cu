@@ -8,13 +8,20 @@
 //
 // One block of 4 warps works through its run of tiles (fa_paged.cuh). In a
 // warp 8 lanes share one key (each holds every 8th 16-byte piece of its row),
-// so 4 keys (8 with two in flight) are in work at once and a dot product needs
-// 3 shuffles; every group of 8 lanes keeps its own m, l and o until the unit
-// ends. A unit has 1 row (one query head on a KV head) or 4 rows (2 for
-// head_dim above 128) that use each key row loaded. fp32 decoding is bound by
-// memory latency, so the grid asks for several blocks an SM: 8 requests of 200
-// to 1025 tokens, 8 heads of 64, take 10.1 us with the join (1.4 TB/s), of
-// 8000 tokens 74 us (3.6 TB/s).
+// so 4 keys are in work at once and a dot product needs 3 shuffles; every group
+// of 8 lanes keeps its own m, l and o until the unit ends. A unit has 1 row (one
+// query head on a KV head) or 4 rows (2 for head_dim above 128) that use each
+// key row loaded.
+//
+// Bound by memory latency: with one row the warps an SM holds cover it better
+// than a second key a lane group has in flight (D = 64, 64 requests of 8000
+// tokens on 8 heads: 363 us, 5.8 TB/s, with 24 warps, 457 with 16 warps and two
+// keys); with 4 rows the registers decide the warps, and two keys give the
+// scheduler 8 independent dot products (32 heads on 8 KV heads: 739 and 770 us).
+// 16 or 32 lanes a key, for fewer registers at D = 128 and 256, double the
+// shuffles and the softmax work: 1525 us instead of 1190. 8 requests of 200 to
+// 1025 tokens, 8 heads of 64, take 10.8 us with the join, of 8000 tokens 55 us
+// (4.8 TB/s).
 #include "fa_paged.cuh"
 
 #include <algorithm>
@@ -57,7 +64,7 @@ __device__ __forceinline__ int slice_col(int sub, int i) {
 template <typename T, int DM, int R, bool VEC>
 __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a) {
   constexpr int DPL = DM / 8;
-  constexpr int U = DM <= 128 ? 2 : 1;  // keys a lane group has in flight
+  constexpr int U = R > 1 && DM <= 128 ? 2 : 1;  // keys a lane group has in flight
   __shared__ RunScratch scratch;
   __shared__ float sm_o[4][R][DM];
   __shared__ float sm_m[4][R], sm_l[4][R];
@@ -156,31 +163,58 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
         }
       }
       fetch(base + 16 * U);
+      // Every score of the step before any of its branches, so that the dot
+      // products and their shuffles overlap.
+      float x[U][R];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int key = base + u * 16 + kg;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          float s = 0.f;
+          x[u][r] = 0.f;
 #pragma unroll
-          for (int i = 0; i < DPL; ++i) s = fmaf(q[r][i], kx[u][i], s);
-          s += __shfl_xor_sync(0xffffffffu, s, 1);
-          s += __shfl_xor_sync(0xffffffffu, s, 2);
-          s += __shfl_xor_sync(0xffffffffu, s, 4);
-          if (on[u] && key >= vis[r].x && key < vis[r].y) {
-            float x;
-            if (a.softcap > 0.f) x = a.softcap * tanhf(s * a.cap_in);
-            else x = s * a.scale;
-            x = fmaf(slope[r], (float)(key - qpos[r]), x) * kLog2e;
-            // (a score of -inf, an overflow, leaves the row as it is)
-            if (x > m[r]) {
-              const float f = m[r] == -INFINITY ? 0.f : exp2f(m[r] - x);
-              l[r] *= f;
+          for (int i = 0; i < DPL; ++i) x[u][r] = fmaf(q[r][i], kx[u][i], x[u][r]);
+        }
+      }
 #pragma unroll
-              for (int i = 0; i < DPL; ++i) o[r][i] *= f;
-              m[r] = x;
-            }
-            const float p = x == -INFINITY ? 0.f : exp2f(x - m[r]);
+      for (int d = 1; d < 8; d *= 2) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int r = 0; r < R; ++r) x[u][r] += __shfl_xor_sync(0xffffffffu, x[u][r], d);
+      }
+      if (a.softcap > 0.f) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int r = 0; r < R; ++r) x[u][r] = a.softcap * tanhf(x[u][r] * a.cap_in);
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int r = 0; r < R; ++r) x[u][r] *= a.scale;
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float top = m[r];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int key = base + u * 16 + kg;
+          x[u][r] = fmaf(slope[r], (float)(key - qpos[r]), x[u][r]) * kLog2e;
+          if (!on[u] || key < vis[r].x || key >= vis[r].y) x[u][r] = -INFINITY;
+          top = fmaxf(top, x[u][r]);
+        }
+        if (top > m[r]) {
+          const float f = m[r] == -INFINITY ? 0.f : exp2f(m[r] - top);
+          l[r] *= f;
+#pragma unroll
+          for (int i = 0; i < DPL; ++i) o[r][i] *= f;
+          m[r] = top;
+        }
+        // (a score of -inf, hidden or an overflow, leaves the row as it is)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (x[u][r] != -INFINITY) {
+            const float p = exp2f(x[u][r] - m[r]);
             l[r] += p;
 #pragma unroll
             for (int i = 0; i < DPL; ++i) o[r][i] = fmaf(p, vx[u][i], o[r][i]);
@@ -444,7 +478,11 @@ int simt_rows_per_unit(int dtype, bool vec, int D, long long rows) {
   return D <= 128 ? 4 : 2;
 }
 
-int simt_ctas(int D) { return 148 * (D <= 64 ? 8 : 4); }
+// One wave: what the registers let an SM hold. (D = 64, one row, 8000 tokens: 6
+// blocks an SM 363 us, 8 blocks 500, 5 blocks 414.)
+int simt_ctas(int D, int rows_per_unit) {
+  return 148 * (rows_per_unit == 1 ? (D <= 64 ? 6 : D <= 128 ? 4 : 2) : (D <= 64 ? 3 : 2));
+}
 
 cudaError_t launch_paged_simt(const PagedArgs& a, int dtype, bool vec, cudaStream_t st) {
   switch (dtype) {
