@@ -147,6 +147,7 @@ struct PagedArgs {
   Div by_min_run;          // least length of a run
   int units_per_req;       // uncut work, one block a unit (0: the kernel sums up the requests)
   Div by_units;
+  int cluster_shift;       // > 0: a cluster of 1 << cluster_shift blocks shares an uncut unit's tiles
   int rows_per_unit;
   int join_rows;           // most rows a unit can have here (for the join's grid)
   float* slot_o;           // [n_ctas, 2, rows_per_unit, D] unnormalised
@@ -155,6 +156,27 @@ struct PagedArgs {
   unsigned* status;        // [0] timeouts, [1] bad index
   unsigned long long wait_limit_ns;
 };
+
+// launch_pdl with the grid in clusters of `cluster` blocks.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_pdl_cluster(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                               unsigned cluster, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+}
 
 // Where one run of the cut work begins (written by the attention kernel, read
 // by the join).

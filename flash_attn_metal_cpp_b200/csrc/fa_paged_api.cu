@@ -146,7 +146,7 @@ struct Choice {
   int own_split, pre_split;        // parts the keys are cut in
   int own_blocks, pre_blocks;      // blocks of 256 packed rows
   int rows_per_unit, n_ctas, join_rows, split;
-  int units_per_req;
+  int units_per_req, cluster_shift;
   int n_parts;                     // whole-row partial results to join (0: none)
   CutLayout cut;
   size_t parts_lse, parts_o, bytes;  // offsets of the partial results
@@ -229,6 +229,7 @@ Choice choose(const fa_paged_params* p, const Checked& c, bool vec, bool one) {
       h.rows_per_unit = simt_rows_per_unit(c.dtype, vec, a.D, rows);
       h.n_ctas = simt_ctas(a.D, h.rows_per_unit);
     }
+    const int wave = h.n_ctas;
     h.join_rows = (int)std::min<long long>(h.rows_per_unit, one ? (long long)a.group : all_rows);
     const long long keys = own_keys + (h.shared ? 0 : a.pre);
     // A unit of few keys is not worth cutting: its block takes 0.6 to 1.2 us a
@@ -246,6 +247,29 @@ Choice choose(const fa_paged_params* p, const Checked& c, bool vec, bool one) {
     if (!h.split) {
       h.n_ctas = (int)std::min<long long>(units, one ? 1 << 30 : 148 * 16);
       h.units_per_req = one && units <= (1 << 30) ? (int)per_req : 0;
+    }
+    // Units of few tiles are cut between the blocks of a cluster instead, which
+    // saves the join's launch but balances nothing, so a block's share by the
+    // table's width is at most 128 KB of K and V. (One request on 8 KV heads, D =
+    // 128, cut in runs and in clusters: 500 keys 13.1 and 7.9 us, 2000 keys, 4
+    // tiles a share, 13.6 and 11.4, 4000 keys 13.3 and 15.9; 16 requests of 1 to
+    // 1000 keys, 8 tiles a share, 13.0 and 15.8. Uncut and in clusters: 200 keys
+    // 9.2 and 7.1, D = 64 8.7 and 7.5, 160 keys 7.7 and 8.0; fp32, 90 keys 9.4
+    // and 8.5, 250 keys 14.9 and 7.9.) Blocks that fill an SM go in fours: eights
+    // took 17.9 us where fours take 15.9. Beside the prefix's kernel more
+    // blocks find no SM free (16 requests of up to 200 keys 19.1 us, uncut 17.8).
+    const bool can = h.tensor ? h.rows_per_unit == 16 : vec;
+    if (one && can && !h.shared && keys > (h.tensor ? 224 : 96)) {
+      const int tile = h.tensor ? 64 : 32, most = h.tensor && a.D > 128 ? 2 : 3;
+      const long long tiles = (keys + tile - 1) / tile;
+      int shift = 0;
+      while (shift < most && (units << (shift + 1)) <= wave && (2ll << shift) <= tiles) ++shift;
+      if (shift > 0 && (tiles >> shift) * a.D <= 512) {
+        h.cluster_shift = shift;
+        h.split = 0;
+        h.n_ctas = (int)units << shift;
+        h.units_per_req = (int)per_req;
+      }
     }
     h.cut = cut_layout(h.split ? h.n_ctas : 0, h.rows_per_unit, a.D);
     h.bytes = h.cut.bytes;
@@ -485,6 +509,7 @@ fa_status fa_paged_forward(const fa_paged_params* p, const void* q, const void* 
     a.units_per_req = h.units_per_req;
     a.by_units = Div(std::max(1, h.units_per_req));
     a.split = h.split;
+    a.cluster_shift = h.cluster_shift;
     place_cut(a, h.cut, workspace);
     a.late_wait = h.shared;
     st = h.tensor ? cuda_status(launch_paged_decode(a, c.dtype, s), "paged attention (few rows)")

@@ -99,7 +99,7 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 }
 
 // Steps through the tiles of a run: request, unit (chunk of rows, KV head), tile.
-template <int MR>
+template <int MR, bool CL>
 struct Cursor {
   int left;              // of the line, from the unit's beginning on
   int req, unit, per;    // per: a unit's stretch of the line
@@ -111,7 +111,7 @@ struct Cursor {
 
   __device__ __forceinline__ void begin_piece(const PagedArgs& a, int first) {
     tile = first;
-    tile_end = a.split && left < per ? tile_at(left) : v.tiles;
+    tile_end = !CL && a.split && left < per ? tile_at(left) : v.tiles;
     whole = first == 0 && tile_end == v.tiles;
     new_piece = true;
   }
@@ -129,7 +129,14 @@ struct Cursor {
     const int chunk = a.by_hk(unit);
     hk = unit - chunk * a.Hk;
     row0 = chunk * MR;
-    begin_piece(a, a.split ? tile_at(in_unit) : 0);
+    begin_piece(a, !CL && a.split ? tile_at(in_unit) : 0);
+    if constexpr (CL) {
+      const int rank = blockIdx.x & ((1 << a.cluster_shift) - 1);
+      tile = share_begin(a, v.tiles, rank);
+      tile_end = share_begin(a, v.tiles, rank + 1);
+      whole = false;
+      if (tile == tile_end) left = 0;
+    }
   }
 
   // Describes the current tile and moves on.
@@ -153,7 +160,7 @@ struct Cursor {
     if (d.last) {
       run_first = false;
       left -= per;
-      if (left > 0) {
+      if (!CL && left > 0) {
         if (++hk == a.Hk) {
           hk = 0;
           row0 += MR;
@@ -175,7 +182,8 @@ struct Cursor {
   }
 };
 
-template <typename T, int DM, int MT>
+// CL: clusters of blocks share uncut units (PagedArgs::cluster_shift).
+template <typename T, int DM, int MT, bool CL>
 __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_kernel(const PagedArgs a) {
   using C = Cfg<DM, MT>;
   constexpr int NS = C::NS, MR = MT * 16, CPR = DM / 8, NB = DM / 8, KK = DM / 16;
@@ -194,17 +202,17 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
   // L2). One block waits at its end instead, so that "this kernel is done"
   // still means "that one is done too" for the join that follows; the others
   // make room for the next block when their run is finished.
-  if (!a.late_wait) grid_dep_wait();
+  if (CL || !a.late_wait) grid_dep_wait();
   grid_dep_launch_dependents();
   const Run run = find_run<kTile, kThreads>(a, MR, &sh.scratch);
   if (run.end <= run.begin) {
-    if (a.split && tid == 0) a.meta[blockIdx.x].n_runs = 0;
-    if (a.late_wait && blockIdx.x == 0) grid_dep_wait();
+    if (!CL && a.split && tid == 0) a.meta[blockIdx.x].n_runs = 0;
+    if (!CL && a.late_wait && blockIdx.x == 0) grid_dep_wait();
     return;
   }
-  Cursor<MR> cur;
+  Cursor<MR, CL> cur;
   cur.start(a, run);
-  if (a.split && tid == 0) {
+  if (!CL && a.split && tid == 0) {
     RunMeta& mt = a.meta[blockIdx.x];
     mt.begin = run.begin;
     mt.unit_begin = run.req_begin + cur.unit * cur.per;
@@ -507,9 +515,13 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
             x[2] += y.z;
             x[3] += y.w;
           }
-          if (d.whole) {
+          if (!CL && d.whole) {
             const int row = d.row0 + rr, j = a.by_group(row);
             finish_row4(a, d.q0 + j, d.hk * a.group + row - j * a.group, col, x, top, ls);
+          } else if (CL) {
+            float* part = reinterpret_cast<float*>(ring + (st == 0 ? 1 : 0) * C::STAGE);
+            *reinterpret_cast<float4*>(part + rr * DM + col) = make_float4(x[0], x[1], x[2], x[3]);
+            if (col == 0) reinterpret_cast<float2*>(part + MR * DM)[rr] = make_float2(top, ls);
           } else {
             const int64_t sr = ((int64_t)blockIdx.x * 2 + d.slot) * MR + rr;
             *reinterpret_cast<float4*>(a.slot_o + sr * a.D + col) = make_float4(x[0], x[1], x[2], x[3]);
@@ -527,18 +539,28 @@ __global__ void __launch_bounds__(kThreads, (Cfg<DM, MT>::BLOCKS)) paged_decode_
     st = st == NS - 1 ? 0 : st + 1;
   }
   cp_async_wait<0>();
-  if (a.late_wait && blockIdx.x == 0) grid_dep_wait();
+  if constexpr (CL) {
+    // A block's part is in stage 1 if its last tile was in stage 0, else in
+    // stage 0 (and nowhere when it had no tile).
+    const int rows = min(MR, cur.v.qlen * a.group - cur.row0);
+    join_cluster<MR, DM, kThreads>(a, cur.v, cur.row0, rows, cur.hk, [&](int tiles) {
+      return ring_addr + ((unsigned)(tiles - 1) % NS == 0 ? C::STAGE : 0);
+    });
+  }
+  if (!CL && a.late_wait && blockIdx.x == 0) grid_dep_wait();
 }
 
-template <typename T, int DM, int MT>
+template <typename T, int DM, int MT, bool CL = false>
 cudaError_t launch(const PagedArgs& a, cudaStream_t st) {
   constexpr int smem = smem_bytes<DM, MT>();
   static_assert(smem <= 227 * 1024 && Cfg<DM, MT>::BLOCKS * (smem + 1024) <= 228 * 1024, "shared memory");
-  auto kern = paged_decode_kernel<T, DM, MT>;
+  auto kern = paged_decode_kernel<T, DM, MT, CL>;
   static std::atomic<unsigned long long> done{0};
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), smem, done);
   if (e != cudaSuccess) return e;
-  e = launch_pdl(kern, dim3((unsigned)a.n_ctas), dim3(kThreads), smem, st, a);
+  const dim3 grid((unsigned)a.n_ctas), block(kThreads);
+  e = CL ? launch_pdl_cluster(kern, grid, block, smem, st, 1u << a.cluster_shift, a)
+         : launch_pdl(kern, grid, block, smem, st, a);
   note_launch();
   return e;
 }
@@ -546,6 +568,10 @@ cudaError_t launch(const PagedArgs& a, cudaStream_t st) {
 template <typename T>
 cudaError_t launch_t(const PagedArgs& a, cudaStream_t st) {
   const bool two = a.rows_per_unit == 32;
+  if (a.cluster_shift > 0) {  // (one MMA tile of rows only)
+    if (a.D <= 64) return launch<T, 64, 1, true>(a, st);
+    return a.D <= 128 ? launch<T, 128, 1, true>(a, st) : launch<T, 256, 1, true>(a, st);
+  }
   if (a.D <= 64) return two ? launch<T, 64, 2>(a, st) : launch<T, 64, 1>(a, st);
   if (a.D <= 128) return two ? launch<T, 128, 2>(a, st) : launch<T, 128, 1>(a, st);
   return launch<T, 256, 1>(a, st);

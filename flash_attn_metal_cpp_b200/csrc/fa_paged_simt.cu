@@ -61,13 +61,15 @@ __device__ __forceinline__ int slice_col(int sub, int i) {
   return VEC ? ((i / 4) * 8 + sub) * 4 + (i & 3) : i * 8 + sub;
 }
 
-template <typename T, int DM, int R, bool VEC>
+// CL: clusters of blocks share uncut units (PagedArgs::cluster_shift).
+template <typename T, int DM, int R, bool VEC, bool CL>
 __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a) {
   constexpr int DPL = DM / 8;
   constexpr int U = R > 1 && DM <= 128 ? 2 : 1;  // keys a lane group has in flight
   __shared__ RunScratch scratch;
   __shared__ float sm_o[4][R][DM];
   __shared__ float sm_m[4][R], sm_l[4][R];
+  __shared__ __align__(16) float sm_part[CL ? R * DM + 2 * R : 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int sub = lane & 7, kg = lane >> 3;
   const int sd = (a.D + 3) & ~3;
@@ -76,7 +78,7 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
   grid_dep_launch_dependents();
   const Run run = find_run<kTile, kThreads>(a, R, &scratch);
   if (run.end <= run.begin) {
-    if (a.split && tid == 0) a.meta[blockIdx.x].n_runs = 0;
+    if (!CL && a.split && tid == 0) a.meta[blockIdx.x].n_runs = 0;
     return;
   }
   const T* Q = reinterpret_cast<const T*>(a.q);
@@ -99,13 +101,20 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
     const int unit = (unsigned)off / (unsigned)per;
     const int unit_begin = req_begin + unit * per;
     const int t_end = v.tile_lo + v.tiles;
-    const int t0 = v.tile_lo + (a.split ? tile_at(at - unit_begin) : 0);
-    const int t1 = a.split && run.end < unit_begin + per ? v.tile_lo + tile_at(run.end - unit_begin) : t_end;
+    int t0 = v.tile_lo, t1 = t_end;
+    if constexpr (CL) {
+      const int rank = blockIdx.x & ((1 << a.cluster_shift) - 1);
+      t1 = t0 + share_begin(a, v.tiles, rank + 1);
+      t0 += share_begin(a, v.tiles, rank);
+    } else if (a.split) {
+      t0 += tile_at(at - unit_begin);
+      if (run.end < unit_begin + per) t1 = v.tile_lo + tile_at(run.end - unit_begin);
+    }
     const int chunk = a.by_hk(unit);
     const int hk = unit - chunk * a.Hk;
     const int row0 = chunk * R;
     const int rows = min(R, v.qlen * a.group - row0);
-    if (a.split && at == run.begin && tid == 0) {
+    if (!CL && a.split && at == run.begin && tid == 0) {
       RunMeta& mt = a.meta[blockIdx.x];
       mt.begin = run.begin;
       mt.unit_begin = unit_begin;
@@ -260,7 +269,10 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[i] = fmaf(f, sm_o[w][r][col + i], x[i]);
       }
-      if (whole) {
+      if constexpr (CL) {
+        *reinterpret_cast<float4*>(sm_part + r * DM + col) = make_float4(x[0], x[1], x[2], x[3]);
+        if (col == 0) *reinterpret_cast<float2*>(sm_part + R * DM + 2 * r) = make_float2(top, ls);
+      } else if (whole) {
         const int row = row0 + r, j = a.by_group(row);
         finish_row4(a, v.q0 + j, hk * a.group + row - j * a.group, col, x, top, ls);
       } else {
@@ -268,6 +280,11 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a)
         *reinterpret_cast<float4*>(a.slot_o + sr * sd + col) = make_float4(x[0], x[1], x[2], x[3]);
         if (col == 0) a.slot_ml[sr] = make_float2(top, ls);
       }
+    }
+    if constexpr (CL) {
+      const uint32_t part = smem_addr(sm_part);
+      join_cluster<R, DM, kThreads>(a, v, row0, rows, hk, [part](int) { return part; });
+      return;
     }
     __syncthreads();
     at = unit_begin + per;
@@ -449,7 +466,12 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedArgs a) {
 
 template <typename T, int DM, int R, bool VEC>
 cudaError_t launch_one(const PagedArgs& a, cudaStream_t st) {
-  cudaError_t e = launch_pdl(paged_simt_kernel<T, DM, R, VEC>, dim3((unsigned)a.n_ctas), dim3(kThreads), 0, st, a);
+  const dim3 grid((unsigned)a.n_ctas), block(kThreads);
+  cudaError_t e;
+  if (VEC && a.cluster_shift > 0)
+    e = launch_pdl_cluster(paged_simt_kernel<T, DM, R, VEC, VEC>, grid, block, 0, st, 1u << a.cluster_shift, a);
+  else
+    e = launch_pdl(paged_simt_kernel<T, DM, R, VEC, false>, grid, block, 0, st, a);
   note_launch();
   return e;
 }

@@ -210,6 +210,34 @@ def test_many_short_requests(fa, cuda_device):
         b.check(fa, "short")
 
 
+# Tables narrow enough that a cluster of 2, 4 or 8 blocks shares a unit's tiles (many requests, heads and
+# columns leave fewer blocks a unit): requests of no key, of one, of fewer tiles than blocks.
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("heads", [(16, 16), (8, 2), (15, 1), (3, 3)])
+@pytest.mark.parametrize("d", [40, 64, 128, 160, 256])
+@pytest.mark.parametrize("copies", [1, 3])
+def test_narrow_tables(fa, cuda_device, dtype, heads, d, copies):
+    lens = [1, 0, 33, 64, 65, 130, 300, 449] * copies
+    b = Batch(cuda_device, lens, hq=heads[0], hk=heads[1], d=d, dtype=dtype)
+    b.check(fa, f"{dtype} {heads} d{d}")
+    slopes = torch.linspace(0.02, 0.5, heads[0], dtype=torch.float32, device=cuda_device)
+    b.check(fa, "window, slopes", window=(70, 0), slopes=slopes)
+    b.check(fa, "cap", cap=15.0, out_dtype=dtype)
+
+
+@pytest.mark.parametrize("dtype", [HF, FP])
+@pytest.mark.parametrize("lens", [[512], [225], [0], [1, 2, 640, 3]])
+def test_narrow_tables_few_requests(fa, cuda_device, dtype, lens):
+    for width in (None, 60):
+        b = Batch(cuda_device, lens, hq=8, hk=8, d=64, dtype=dtype, spare_rows=2, width=width)
+        b.check(fa, f"{lens} width {width}")
+        c = Batch(cuda_device, lens, hq=8, hk=2, d=128, dtype=dtype, prefix=130, width=width)
+        c.check(fa, f"{lens} width {width}, short prefix")
+        first = c.run(fa, return_lse=True)
+        again = c.run(fa, return_lse=True)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
 def test_window_leaves_old_pages_unread(fa, cuda_device):
     """Pages wholly before the window may have been given away: their entries and slots hold anything."""
     for qlens in ([1, 1], [5, 2], [100, 40]):
