@@ -11,7 +11,8 @@
 // ends go to the block's two partial slots and a second kernel joins them in
 // the order of the blocks, so results do not depend on timing. Calls whose
 // keys are few by the table's width are not cut (PagedArgs::split): the line
-// then counts units and nothing is joined.
+// then counts units and nothing is joined, or a cluster of blocks takes each
+// unit and joins it in shared memory (join_cluster).
 #pragma once
 
 #include "fa_paged.h"
@@ -315,13 +316,14 @@ __device__ __forceinline__ void finish_row4(const PagedArgs& a, int token, int h
 // cluster, and joined through its shared memory instead of by a second kernel:
 // a launch and its wait less. (On 8 KV heads, D = 128, one request of 500 keys
 // 13.1 -> 7.7 us, 16 requests 17.0 -> 11.6 us.)
+
 // First of a unit's tiles that block `rank` of its cluster takes.
 __device__ __forceinline__ int share_begin(const PagedArgs& a, int tiles, int rank) {
   return (int)(((long long)tiles * rank) >> a.cluster_shift);
 }
 
 __device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 // Address of a shared variable of this block in block `rank` of its cluster.
 __device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, int rank) {

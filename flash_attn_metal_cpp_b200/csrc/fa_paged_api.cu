@@ -254,12 +254,12 @@ Choice choose(const fa_paged_params* p, const Checked& c, bool vec, bool one) {
     // 128, cut in runs and in clusters: 500 keys 13.1 and 7.9 us, 2000 keys, 4
     // tiles a share, 13.6 and 11.4, 4000 keys 13.3 and 15.9; 16 requests of 1 to
     // 1000 keys, 8 tiles a share, 13.0 and 15.8. Uncut and in clusters: 200 keys
-    // 9.2 and 7.1, D = 64 8.7 and 7.5, 160 keys 7.7 and 8.0; fp32, 90 keys 9.4
-    // and 8.5, 250 keys 14.9 and 7.9.) Blocks that fill an SM go in fours: eights
+    // 9.3 and 7.0, 160 keys 8.2 and 8.1, D = 64 200 keys 8.7 and 7.5, 160 keys 7.7
+    // and 8.0; fp32, 90 keys 9.4 and 8.3, 250 keys 14.9 and 7.9.) Blocks that fill an SM go in fours: eights
     // took 17.9 us where fours take 15.9. Beside the prefix's kernel more
     // blocks find no SM free (16 requests of up to 200 keys 19.1 us, uncut 17.8).
     const bool can = h.tensor ? h.rows_per_unit == 16 : vec;
-    if (one && can && !h.shared && keys > (h.tensor ? 224 : 96)) {
+    if (one && can && !h.shared && keys > (h.tensor ? 192 : 64)) {
       const int tile = h.tensor ? 64 : 32, most = h.tensor && a.D > 128 ? 2 : 3;
       const long long tiles = (keys + tile - 1) / tile;
       int shift = 0;

@@ -19,9 +19,12 @@
 // keys); with 4 rows the registers decide the warps, and two keys give the
 // scheduler 8 independent dot products (32 heads on 8 KV heads: 739 and 770 us).
 // 16 or 32 lanes a key, for fewer registers at D = 128 and 256, double the
-// shuffles and the softmax work: 1525 us instead of 1190. 8 requests of 200 to
-// 1025 tokens, 8 heads of 64, take 10.8 us with the join, of 8000 tokens 55 us
-// (4.8 TB/s).
+// shuffles and the softmax work: 1525 us instead of 1190. Clusters (narrow
+// tables) leave warps over, so there 4 keys in flight pay (16 requests of 250
+// tokens, 16 heads of 64: 9.4 us, with one key 10.2; not above 64 columns: 8
+// requests of 250, 4 KV heads of 256, 9.8 us with two keys, 9.1 with one). 8
+// requests of 200 to 1025 tokens, 8 heads of 64, take 10.0 us, of 8000 tokens
+// 55 us (4.8 TB/s).
 #include "fa_paged.cuh"
 
 #include <algorithm>
@@ -65,7 +68,8 @@ __device__ __forceinline__ int slice_col(int sub, int i) {
 template <typename T, int DM, int R, bool VEC, bool CL>
 __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const PagedArgs a) {
   constexpr int DPL = DM / 8;
-  constexpr int U = R > 1 && DM <= 128 ? 2 : 1;  // keys a lane group has in flight
+  // Keys a lane group has in flight.
+  constexpr int U = CL && R == 1 && DM <= 64 ? 4 : R > 1 && DM <= 128 ? 2 : 1;
   __shared__ RunScratch scratch;
   __shared__ float sm_o[4][R][DM];
   __shared__ float sm_m[4][R], sm_l[4][R];

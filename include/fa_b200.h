@@ -436,7 +436,8 @@ size_t fa_paged_workspace_size(const fa_paged_params* p);
  * prompt chunk and changes nothing for a single token. Rows that see no key
  * get O = 0 and LSE = -inf; rows behind the last sequence are left as they
  * were. Slots no query of the request sees (behind its end, before its
- * window) are not read into the result whatever they hold.
+ * window) are not read into the result whatever they hold. o and lse must not
+ * overlap the inputs or each other.
  * workspace: device scratch of fa_paged_workspace_size bytes, 256-byte
  * aligned; calls that may overlap on the GPU need one each. */
 fa_status fa_paged_forward(const fa_paged_params* p, const void* q, const void* k_cache, const void* v_cache,
