@@ -238,6 +238,34 @@ def test_narrow_tables_few_requests(fa, cuda_device, dtype, lens):
         assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
 
 
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_narrow_tables_captured(fa, cuda_device, dtype):
+    """Clusters in two captured graphs that replay side by side while the lengths change."""
+    batches = [Batch(cuda_device, [300, 449, 65], hq=8, hk=4, d=d, dtype=dtype, seed=d) for d in (64, 128)]
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in batches]
+    for b in batches:
+        b.run(fa)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(b.run(fa, out_dtype="float32"))
+        graphs.append(g)
+    for lens in ([300, 449, 65], [1, 0, 64], [33, 448, 0]):
+        for b in batches:
+            b.lens = lens
+            b.seq.copy_(torch.tensor(lens, dtype=torch.int32))
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for g, st in zip(graphs, streams):
+                with torch.cuda.stream(st):
+                    g.replay()
+        torch.cuda.synchronize()
+        fa.check_status()
+        for b, o in zip(batches, outs):
+            w, _, tol, _ = b.want(out_dtype=FP)
+            ref.assert_attention(o, w, tol, f"{lens}")
+
+
 def test_window_leaves_old_pages_unread(fa, cuda_device):
     """Pages wholly before the window may have been given away: their entries and slots hold anything."""
     for qlens in ([1, 1], [5, 2], [100, 40]):
