@@ -348,7 +348,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const Paged
       for (int k = 0; k < 4; ++k) acc[c][k] *= g;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (ml[i].x == -INFINITY) continue;
+      // (a part without visible keys has the sum 0; a row of NaN scores has no
+      // maximum either, but a NaN sum, and is joined)
+      if (ml[i].y == 0.f) continue;
       const float f = exp2f(ml[i].x - top);
       l = fmaf(f, ml[i].y, l);
 #pragma unroll
