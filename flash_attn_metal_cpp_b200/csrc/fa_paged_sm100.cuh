@@ -85,6 +85,13 @@ __device__ __forceinline__ float rcp_approx(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// The smaller of both, NaN when one of them is (fminf drops a NaN, and a NaN
+// score would become the full cap).
+__device__ __forceinline__ float min_nan(float x, float y) {
+  float z;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
+  return z;
+}
 template <typename T>
 __device__ __forceinline__ uint32_t pack_p(float lo, float hi) {
   if constexpr (std::is_same<T, __half>::value) return pack_half2(lo, hi);
@@ -568,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m_cand = ext * sl2;
       if constexpr (XF == 2)
         m_cand = ext == -INFINITY ? -INFINITY
-                                  : cap_log2 * (1.f - __fdividef(2.f, 1.f + ex2_approx(fminf(ext * cap_k, 40.f))));
+                                  : cap_log2 * (1.f - __fdividef(2.f, 1.f + ex2_approx(min_nan(ext * cap_k, 40.f))));
       const float m_new = fmaxf(m_run, m_cand - weight_bias<T>());
       const bool grow = m_new > m_run + kRescaleThreshold;
       const bool any_grow = __any_sync(0xffffffffu, grow);
@@ -594,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         float2 u = make_float2(s0, s1);
         if constexpr (XF == 2) {
           u = __fmul2_rn(u, ck2);
-          u = make_float2(fminf(u.x, 40.f), fminf(u.y, 40.f));
+          u = make_float2(min_nan(u.x, 40.f), min_nan(u.y, 40.f));
           const float2 d = __fadd2_rn(make_float2(ex2_approx(u.x), ex2_approx(u.y)), make_float2(1.f, 1.f));
           const float inv = rcp_approx(d.x * d.y);
           u = __fmul2_rn(make_float2(d.y, d.x), make_float2(inv, inv));

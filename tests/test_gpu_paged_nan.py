@@ -62,3 +62,9 @@ def check_output(fa, b, **kw):
 @cases
 def test_nan_reaches_the_output(fa, cuda_device, path, where, dtype):
     check_output(fa, poisoned(cuda_device, path, dtype, where))
+
+
+@cases
+@pytest.mark.parametrize("cap", [30.0, 400.0])
+def test_nan_under_a_cap(fa, cuda_device, path, where, dtype, cap):
+    check_output(fa, poisoned(cuda_device, path, dtype, where), cap=cap)
