@@ -291,6 +291,12 @@ __device__ __forceinline__ float cap_tanh(float y) {
   return fabsf(y) < 0.25f ? series : quot;
 }
 
+// Natural-log LSE of a row with maximum m (log2 units) and sum l, and what its
+// O is multiplied by. The sum is 0 only for a row without visible keys (else its
+// largest weight is 1 or more, up to rounding); a NaN sum stays NaN in both.
+__device__ __forceinline__ float row_lse(float m, float l) { return l == 0.f ? -INFINITY : fmaf(m, kLn2, logf(l)); }
+__device__ __forceinline__ float row_inv(float l) { return l == 0.f ? 0.f : 1.f / l; }
+
 // Columns [col, col + 4) of a finished row (token, head): x holds
 // sum exp2(s - m) v and l the sum of exp2(s - m), both over the row's keys
 // (m in log2 units, -inf for no key). Writes the quotient and the row's lse,
@@ -298,8 +304,7 @@ __device__ __forceinline__ float cap_tanh(float y) {
 // to the call's own part of them.
 __device__ __forceinline__ void finish_row4(const PagedArgs& a, int token, int head, int col, float (&x)[4], float m,
                                             float l) {
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  const float lse = l > 0.f ? m * kLn2 + logf(l) : -INFINITY;
+  const float inv = row_inv(l), lse = row_lse(m, l);
 #pragma unroll
   for (int i = 0; i < 4; ++i) x[i] *= inv;
   if (a.own_part >= 0) {

@@ -462,12 +462,12 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedArgs a) {
     }
   }
   if (!on) return;
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const float inv = row_inv(l);
 #pragma unroll
   for (int k = 0; k < 4; ++k) x[k] *= inv;
   if (col < a.D) store_out4(a.o, (int64_t)tok * a.o_st + (int64_t)head * a.o_sh + col, a.out_dtype, x, 4);
   if (lane == 0 && a.lse != nullptr)
-    a.lse[(int64_t)head * a.total_q + tok] = l > 0.f ? top * kLn2 + logf(l) : -INFINITY;
+    a.lse[(int64_t)head * a.total_q + tok] = row_lse(top, l);
 }
 
 template <typename T, int DM, int R, bool VEC>

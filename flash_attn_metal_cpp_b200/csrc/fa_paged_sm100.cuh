@@ -656,8 +656,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
     }
     if (ok && b.row0 + t * BM < b.rows) {
-      const float inv_l = (l_run > 0.f) ? 1.f / l_run : 0.f;
-      const float lse = (l_run > 0.f) ? (m_run + log2f(l_run)) * kLn2 : -INFINITY;
+      const float inv_l = row_inv(l_run);
+      const float lse = l_run == 0.f ? -INFINITY : (m_run + log2f(l_run)) * kLn2;
       // 32 columns of the row's O, divided by the sum.
       auto take32 = [&](int col, float (&x)[32]) {
         uint32_t u[32];

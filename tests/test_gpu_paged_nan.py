@@ -68,3 +68,14 @@ def test_nan_reaches_the_output(fa, cuda_device, path, where, dtype):
 @pytest.mark.parametrize("cap", [30.0, 400.0])
 def test_nan_under_a_cap(fa, cuda_device, path, where, dtype, cap):
     check_output(fa, poisoned(cuda_device, path, dtype, where), cap=cap)
+
+
+@cases
+def test_nan_reaches_the_lse(fa, cuda_device, path, where, dtype):
+    # fp16 with slopes, bf16 with a cap: other scores in front of the same end of a row
+    kw = {BF: dict(cap=30.0), FP: {}, HF: dict(slopes=torch.tensor([2.0 ** -(i + 1) for i in range(8)], device=cuda_device))}[dtype]
+    got, want, tol = check_output(fa, poisoned(cuda_device, path, dtype, where), **kw)
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got.isinf(), want.isinf())
+    fin = want.isfinite()
+    assert ((got.double() - want).abs() <= tol)[fin].all()
