@@ -408,13 +408,16 @@ cudaError_t launch_store_t(const StoreArgs& a, bool vec, cudaStream_t st) {
 }  // namespace
 
 cudaError_t launch_plan_pages(const PlanArgs& a, cudaStream_t st) {
+  // Asked for once, for the largest plan: what a call may use depends neither on
+  // the calls before it nor on another thread's (the kernel's static shared
+  // memory counts against the 48 KB that need no asking).
+  constexpr int most = 2 * (kPlanMaxRequests + 1) * (int)sizeof(int);
+  static std::atomic<unsigned long long> done{0};
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(plan_pages_kernel), most, done);
+  if (e != cudaSuccess) return e;
   const size_t smem = 2 * (size_t)(a.B + 1) * sizeof(int);
-  if (smem > 48 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(plan_pages_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
-  }
   const int blocks = std::max(1, (a.rows + kPlanTokens - 1) / kPlanTokens);
-  cudaError_t e = launch_pdl(plan_pages_kernel, dim3((unsigned)blocks), dim3(kPlanThreads), smem, st, a);
+  e = launch_pdl(plan_pages_kernel, dim3((unsigned)blocks), dim3(kPlanThreads), smem, st, a);
   note_launch();
   return e;
 }
