@@ -9,6 +9,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <iterator>
 
 namespace fa {
 namespace {
@@ -331,7 +332,32 @@ fa_status fa_plan_pages(uint32_t batch, uint32_t page_size, uint32_t max_pages, 
   if ((batch && (!cached || !fresh || !seq_lens || (max_pages && !table))) || !cu || !free_end ||
       (rows && (!slots || !positions)) || (n_free && !free_pages))
     return paged_fail(FA_ERR_INVALID_ARG, "NULL plan pointer");
-  if (free_begin == free_end) return paged_fail(FA_ERR_INVALID_ARG, "free_begin and free_end must not overlap");
+  // Every block reads the lengths again while the first one writes its results.
+  // (The table has rows apart from one another, so what lies between them is
+  // the caller's.)
+  struct Span {
+    const char* name;
+    const void* p;
+    size_t bytes;
+  };
+  const size_t n = batch;
+  const Span out[] = {{"seq_lens", seq_lens, n * 4}, {"cu", cu, (n + 1) * 4}, {"slots", slots, (size_t)rows * 8},
+                      {"positions", positions, (size_t)rows * 4}, {"free_end", free_end, 4}};
+  const Span in[] = {{"cached", cached, n * 4}, {"fresh", fresh, n * 4}, {"free_pages", free_pages, (size_t)n_free * 4},
+                     {"free_begin", free_begin, free_begin ? 4u : 0u}};
+  auto meet = [](const Span& x, const Span& y) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(x.p), b = reinterpret_cast<uintptr_t>(y.p);
+    return x.bytes && y.bytes && a < b + y.bytes && b < a + x.bytes;
+  };
+  auto refuse = [](const Span& x, const Span& y) {
+    return paged_fail(FA_ERR_INVALID_ARG, std::string(x.name) + " and " + y.name + " must not overlap");
+  };
+  for (size_t i = 0; i < std::size(out); ++i) {
+    for (const Span& x : in)
+      if (meet(out[i], x)) return refuse(x, out[i]);
+    for (size_t j = 0; j < i; ++j)
+      if (meet(out[i], out[j])) return refuse(out[j], out[i]);
+  }
   unsigned* words = nullptr;
   fa_status st = paged_status_words(&words);
   if (st != FA_OK) return st;

@@ -360,7 +360,9 @@ fa_status fa_noalloc_check_status(void);
  * free_pages is read from entry free_begin[0] on (NULL = 0). When it runs out,
  * or a request outgrows its table row, the tokens without a page get slot -1
  * (and table entries -1) and the status word is set. All arrays are device
- * memory; free_end and free_begin must not overlap. batch <= 8192,
+ * memory. No output overlaps an input or another output (the next step's
+ * cached may be this step's seq_lens, in another array than this step's
+ * cached): refused, but for the table, which is not checked. batch <= 8192,
  * rows <= 2^30. */
 fa_status fa_plan_pages(uint32_t batch, uint32_t page_size, uint32_t max_pages, uint32_t n_free, uint32_t rows,
                         const int32_t* cached, const int32_t* fresh, const int32_t* free_pages,
@@ -413,7 +415,7 @@ void fa_paged_params_init(fa_paged_params* p);
  * stream is being captured; fa_pool_clear frees them, also under captured
  * graphs that use them). A position without a table row leaves its row
  * unrotated and sets the status word. Rotation is computed in float32 and
- * rounded once. */
+ * rounded once. The caches and q_out overlap neither each other nor an input. */
 fa_status fa_store_kv(const fa_paged_params* p, const void* k, const void* v, void* k_cache, void* v_cache,
                       const int64_t* slots, const int32_t* positions, const float* cos, const float* sin,
                       uint32_t table_rows, float rope_theta, const void* q, void* q_out, void* stream);
