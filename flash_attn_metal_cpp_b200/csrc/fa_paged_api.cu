@@ -259,7 +259,7 @@ Choice choose(const fa_paged_params* p, const Checked& c, bool vec, bool one) {
     // and 8.0; fp32, 90 keys 9.4 and 8.3, 250 keys 14.9 and 7.9.) Blocks that fill an SM go in fours: eights
     // took 17.9 us where fours take 15.9. Beside the prefix's kernel more
     // blocks find no SM free (16 requests of up to 200 keys 19.1 us, uncut 17.8).
-    const bool can = h.tensor ? h.rows_per_unit == 16 : vec;
+    const bool can = h.tensor ? h.rows_per_unit == 16 : vec && c.dtype == kF32;  // (the kernels with cluster variants)
     if (one && can && !h.shared && keys > (h.tensor ? 192 : 64)) {
       const int tile = h.tensor ? 64 : 32, most = h.tensor && a.D > 128 ? 2 : 3;
       const long long tiles = (keys + tile - 1) / tile;

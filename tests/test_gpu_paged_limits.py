@@ -1,12 +1,15 @@
 """Sizes, histories and launch chains of the paged-cache operators that the per-operator tests do not meet."""
 from __future__ import annotations
 
+import math
 import subprocess
 import sys
 
 import pytest
+import torch
 
 from conftest import ROOT
+from test_gpu_paged import BF, FP, HF
 
 pytestmark = pytest.mark.gpu
 
@@ -30,3 +33,17 @@ for n in (6127, 6128, 6143, 6144):
     assert torch.equal(cu, torch.arange(n + 1, device='cuda')) and torch.equal(slots, free.long() * 16)
     assert torch.equal(table[:, 0], free) and torch.equal(lens, one) and int(end) == n and not pos.any()
 """)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+def test_empty_cache_with_a_wide_table(fa, cuda_device, dtype):
+    """A cache without pages: every request is empty, whatever the table's width."""
+    kc = torch.zeros((0, 16, 2, 64), dtype=dtype, device=cuda_device)
+    q = torch.randn((3, 8, 64), device=cuda_device).to(dtype)
+    lens = torch.zeros(3, dtype=torch.int32, device=cuda_device)
+    for columns in (10, 20, 100):
+        table = torch.zeros((3, columns), dtype=torch.int32, device=cuda_device)
+        o, lse = fa.paged_forward(q, kc, kc, table, lens, 0.125, return_lse=True)
+        torch.cuda.synchronize()
+        fa.check_status()
+        assert (o == 0).all() and (lse == -math.inf).all()
