@@ -8,8 +8,9 @@ import sys
 import pytest
 import torch
 
+import paged_reference as ref
 from conftest import ROOT
-from test_gpu_paged import BF, FP, HF
+from test_gpu_paged import BF, FP, HF, Batch
 
 pytestmark = pytest.mark.gpu
 
@@ -47,3 +48,54 @@ def test_empty_cache_with_a_wide_table(fa, cuda_device, dtype):
         torch.cuda.synchronize()
         fa.check_status()
         assert (o == 0).all() and (lse == -math.inf).all()
+
+
+# ------------------------------------------- prefix, cut own keys, join, merge
+def chain(dev, dtype, qlens, seed):
+    """8 requests behind a prefix of 2000 keys (read once), own keys of 1 to 1500 cut in runs."""
+    lens = [1500, 1, 64, 777, 1200, 385, 20, 3] if qlens is None else [1500, 4, 64, 777, 1200, 385, 20, 3]
+    return Batch(dev, lens, qlens=qlens, hq=32, hk=8, d=128, dtype=dtype, prefix=2000, page=16, seed=seed)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("qlens", [None, [2, 4, 1, 0, 3, 1, 1, 2]])
+def test_prefix_beside_cut_own_keys(fa, cuda_device, dtype, qlens):
+    b = chain(cuda_device, dtype, qlens, 0)
+    n0 = fa.launch_count()
+    b.run(fa, qlens is not None)
+    assert fa.launch_count() - n0 == 4  # prefix, own keys, join of runs, merge
+    b.check(fa, "chain", causal=qlens is not None)
+    b.check(fa, "chain, window", causal=qlens is not None, window=(1700, -1))
+    b.check(fa, "chain, cap", causal=qlens is not None, cap=20.0, out_dtype=dtype)
+    first = b.run(fa, qlens is not None, return_lse=True)
+    for _ in range(5):
+        again = b.run(fa, qlens is not None, return_lse=True)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+def test_prefix_beside_cut_own_keys_captured(fa, cuda_device):
+    """Two graphs of the chain replay on two streams at once while lengths and queries change."""
+    batches = [chain(cuda_device, dtype, None, seed) for seed, dtype in enumerate((BF, HF))]
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in batches]
+    for b in batches:
+        b.run(fa)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(b.run(fa, out_dtype="float32"))
+        graphs.append(g)
+    for lens in (batches[0].lens, [1, 1, 1, 1, 1200, 0, 20, 3], [1400, 0, 33, 700, 64, 300, 1, 2]):
+        for b in batches:
+            b.lens = lens
+            b.seq.copy_(torch.tensor(lens, dtype=torch.int32))
+            b.q.copy_(torch.randn(b.q.shape, device=cuda_device).to(b.q.dtype))
+        torch.cuda.synchronize()
+        for _ in range(10):
+            for g, st in zip(graphs, streams):
+                with torch.cuda.stream(st):
+                    g.replay()
+        torch.cuda.synchronize()
+        fa.check_status()
+        for b, o in zip(batches, outs):
+            w, _, tol, _ = b.want(out_dtype=FP)
+            ref.assert_attention(o, w, tol, f"{lens}")
