@@ -99,3 +99,41 @@ def test_prefix_beside_cut_own_keys_captured(fa, cuda_device):
         for b, o in zip(batches, outs):
             w, _, tol, _ = b.want(out_dtype=FP)
             ref.assert_attention(o, w, tol, f"{lens}")
+
+
+# ------------------------------------------------------------ sizes, first calls
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("d", [136, 160, 192, 256])
+@pytest.mark.parametrize("opts", [{}, dict(cap=50.0), dict(window=(100, -1))])
+def test_wide_heads_with_many_rows(fa, cuda_device, dtype, d, opts):
+    for prefix in (0, 300):
+        b = Batch(cuda_device, [300, 129, 64], qlens=[150, 129, 33], d=d, hq=8, hk=2, dtype=dtype, prefix=prefix)
+        b.check(fa, f"d {d}", causal=True, **opts)
+
+
+@pytest.mark.parametrize("call", ["one", "few", "many", "prefix", "fp32"])
+def test_first_call_of_a_process_is_captured(fa, call):
+    """`initialize()` is enough before a capture: no kernel has to have run before."""
+    in_a_new_process(f"""
+import sys
+sys.path.insert(0, 'tests')
+import torch, paged_reference as ref
+from test_gpu_paged import Batch, BF, FP
+import flash_attn_metal_cpp_b200 as pkg
+pkg.initialize()
+fa = pkg._flash_attn_metal
+kw = dict(one=dict(lens=[900, 40], d=128), few=dict(lens=[900, 40], qlens=[3, 2], d=64), many=dict(lens=[300, 90], qlens=[100, 90], d=128),
+          prefix=dict(lens=[900, 40, 3, 60, 1, 2, 3, 4], d=128, hq=32, hk=8, prefix=2000), fp32=dict(lens=[900, 40], d=64))['{call}']
+b = Batch(torch.device('cuda', 0), dtype=FP if '{call}' == 'fp32' else BF, **kw)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    o = b.run(fa, True)
+    lens, cu, slots, pos, end = fa.plan_pages(b.seq, b.seq * 0 + 1, b.table.clone(), b.seq, 16, len(b.lens))
+    fa.store_kv(torch.ones((len(b.lens), *b.k_cache.shape[2:]), dtype=b.q.dtype, device='cuda'),
+                torch.ones((len(b.lens), *b.k_cache.shape[2:]), dtype=b.q.dtype, device='cuda'), b.k_cache.clone(), b.v_cache.clone(), slots * 0 - 1)
+g.replay()
+torch.cuda.synchronize()
+w, _, tol, _ = b.want(True)
+ref.assert_attention(o, w, tol, 'first')
+""")
