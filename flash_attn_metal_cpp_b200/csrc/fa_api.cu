@@ -370,12 +370,6 @@ fa_status rope_from_theta(DeviceState* ds, float theta, int D, int rows, cudaStr
   std::lock_guard<std::mutex> g(ds->mu);
   auto& r = ds->rope[std::make_pair(theta, D)];
   if (!(r.cs && r.rows >= rows)) {
-    if (r.cs) {
-      ds->retired.push_back(r.cs);
-      ds->retired.push_back(r.sn);
-      r.cs = r.sn = nullptr;
-      r.rows = 0;
-    }
     const size_t bytes = (size_t)rows * (D / 2) * sizeof(float) + 16;
     float *c = nullptr, *s = nullptr;
     FA_CUDA(cudaMalloc(&c, bytes));
@@ -392,6 +386,12 @@ fa_status rope_from_theta(DeviceState* ds, float theta, int D, int rows, cudaStr
       cudaFree(c);
       cudaFree(s);
       return cuda_fail(e, "RoPE tables");
+    }
+    // The smaller tables stay for captured graphs that read them; when this
+    // failed they stay in use.
+    if (r.cs) {
+      ds->retired.push_back(r.cs);
+      ds->retired.push_back(r.sn);
     }
     r.cs = c;
     r.sn = s;

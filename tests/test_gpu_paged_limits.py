@@ -36,6 +36,33 @@ for n in (6127, 6128, 6143, 6144):
 """)
 
 
+# ------------------------------------------------------------- angle tables
+def store_at(fa, dev, max_position, theta, d=256):
+    x = torch.ones((1, 1, d), dtype=BF, device=dev)
+    kc = torch.zeros((1, 16, 1, d), dtype=BF, device=dev)
+    fa.store_kv(x, x, kc, kc.clone(), torch.zeros(1, dtype=torch.int64, device=dev), rope_theta=theta,
+                positions=torch.tensor([max_position - 1], dtype=torch.int32, device=dev), max_position=max_position)
+    return kc
+
+
+def test_tables_survive_a_failed_enlargement(fa, cuda_device):
+    store_at(fa, cuda_device, 64, 23432.0)
+    with pytest.raises(RuntimeError, match="cudaMalloc"):
+        store_at(fa, cuda_device, 1 << 30, 23432.0)
+    torch.cuda.synchronize()
+    x = torch.ones((1, 1, 256), dtype=BF, device=cuda_device)
+    kc = torch.zeros((1, 16, 1, 256), dtype=BF, device=cuda_device)
+    vc, slots = kc.clone(), torch.zeros(1, dtype=torch.int64, device=cuda_device)
+    pos = torch.full((1,), 63, dtype=torch.int32, device=cuda_device)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        fa.store_kv(x, x, kc, vc, slots, positions=pos, rope_theta=23432.0, max_position=64)
+    g.replay()
+    torch.cuda.synchronize()
+    fa.check_status()
+    assert torch.equal(kc, store_at(fa, cuda_device, 64, 23432.0))
+
+
 @pytest.mark.parametrize("dtype", [BF, HF, FP])
 def test_empty_cache_with_a_wide_table(fa, cuda_device, dtype):
     """A cache without pages: every request is empty, whatever the table's width."""
