@@ -370,15 +370,26 @@ fa_status rope_from_theta(DeviceState* ds, float theta, int D, int rows, cudaStr
   std::lock_guard<std::mutex> g(ds->mu);
   auto& r = ds->rope[std::make_pair(theta, D)];
   if (!(r.cs && r.rows >= rows)) {
-    const size_t bytes = (size_t)rows * (D / 2) * sizeof(float) + 16;
+    // Tables that have to grow at least double: with a bound that follows the
+    // sequence, what was replaced stays below the size in use, and few calls
+    // build. (Exact sizes where twice the rows do not fit.)
+    const int wide = r.cs ? std::max(rows, std::min(2 * r.rows, 1 << 30)) : rows;
     float *c = nullptr, *s = nullptr;
-    FA_CUDA(cudaMalloc(&c, bytes));
-    cudaError_t e = cudaMalloc(&s, bytes);
-    if (e != cudaSuccess) {
-      cudaFree(c);
-      return cuda_fail(e, "cudaMalloc (RoPE tables)");
+    cudaError_t e = cudaSuccess;
+    int have = 0;
+    for (int n : {wide, rows}) {
+      const size_t bytes = (size_t)n * (D / 2) * sizeof(float) + 16;
+      e = cudaMalloc(&c, bytes);
+      if (e == cudaSuccess) {
+        e = cudaMalloc(&s, bytes);
+        if (e != cudaSuccess) cudaFree(c);
+      }
+      have = n;
+      if (e == cudaSuccess || n == rows) break;
+      cudaGetLastError();
     }
-    e = launch_rope_table(c, s, rows, D, (double)theta, stream);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaMalloc (RoPE tables)");
+    e = launch_rope_table(c, s, have, D, (double)theta, stream);
     // Other streams must not read the tables before they are built: finish
     // the build here (once per (theta, D) and size, outside any hot loop).
     if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
@@ -395,7 +406,7 @@ fa_status rope_from_theta(DeviceState* ds, float theta, int D, int rows, cudaStr
     }
     r.cs = c;
     r.sn = s;
-    r.rows = rows;
+    r.rows = have;
   }
   *cs = r.cs;
   *sn = r.sn;

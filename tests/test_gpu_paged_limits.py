@@ -45,6 +45,25 @@ def store_at(fa, dev, max_position, theta, d=256):
     return kc
 
 
+def test_growing_positions_do_not_pile_up_tables(fa, cuda_device):
+    """A max_position that follows the sequence: what the tables take stays within a few times the last one."""
+    theta, d, first, steps = 12321.0, 256, 20000, 60
+    store_at(fa, cuda_device, 8, theta)
+    torch.cuda.synchronize()
+    before = torch.cuda.mem_get_info()[0]
+    for i in range(steps):
+        kc = store_at(fa, cuda_device, first + i, theta)
+        inv = torch.tensor([theta ** (-2.0 * j / d) for j in range(d // 2)], dtype=torch.float64, device=cuda_device)
+        ang = (first + i - 1) * inv
+        want = torch.cat([ang.cos() - ang.sin(), ang.sin() + ang.cos()])
+        # angle tables in float32, two products and a sum, one rounding
+        assert ((kc[0, 0, 0].double() - want).abs() <= ref.U[BF] * want.abs() + 8 * 2.0 ** -24).all()
+    torch.cuda.synchronize()
+    fa.check_status()
+    one = (first + steps) * (d // 2) * 4 * 2
+    assert before - torch.cuda.mem_get_info()[0] <= 4 * one
+
+
 def test_tables_survive_a_failed_enlargement(fa, cuda_device):
     store_at(fa, cuda_device, 64, 23432.0)
     with pytest.raises(RuntimeError, match="cudaMalloc"):
