@@ -316,8 +316,9 @@ py::object attention(py::object q, py::object k_cache, py::object v_cache, const
       if (m < 0) paged_error("max_seqlen_q must not be negative");
       p.max_seqlen_q = u32(m, "max_seqlen_q");
     }
-  } else if (qv.size[0] < b) {
-    paged_error("without cu_seqlens_q, q needs one row per request");
+  } else {
+    if (qv.size[0] < b) paged_error("without cu_seqlens_q, q needs one row per request");
+    p.max_seqlen_q = 1;  // (no scratch for the routes of several tokens)
   }
   const int32_t* pre = nullptr;
   if (prefix_table) {

@@ -374,7 +374,8 @@ typedef struct fa_paged_params {
     uint32_t batch_size;      /* requests */
     uint32_t total_q;         /* query tokens (fa_store_kv: tokens), packed: rows of q */
     uint32_t max_seqlen_q;    /* most query tokens of one request, as a hint for the choice of
-                                 kernel (0 = unknown); more tokens are still computed */
+                                 kernel (0 = unknown); more tokens are still computed. 1 for
+                                 single tokens keeps the scratch small */
     uint32_t num_heads_q;
     uint32_t num_heads_k;
     uint32_t head_dim;

@@ -82,6 +82,23 @@ def test_tables_survive_a_failed_enlargement(fa, cuda_device):
     assert torch.equal(kc, store_at(fa, cuda_device, 64, 23432.0))
 
 
+# ------------------------------------------------------------------ scratch
+def test_scratch_of_single_tokens_over_a_wide_table(fa, cuda_device):
+    """A call without cu_seqlens_q asks for no scratch of the routes that only several tokens a request take."""
+    b = Batch(cuda_device, [40] * 64, hq=32, hk=8, d=128, dtype=BF, width=16384)
+    b.run(fa)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    o = b.run(fa)
+    torch.cuda.synchronize()
+    peak = torch.cuda.max_memory_allocated() - before
+    # runs of the few-rows kernel: two partial units of 16 rows for each of 296 blocks, and their records
+    most = 296 * (2 * 16 * (128 * 4 + 8) + 64) + o.numel() * 2 + (1 << 20)
+    assert peak <= most, (peak, most)
+
+
+# ------------------------------------------------------------- empty caches
 @pytest.mark.parametrize("dtype", [BF, HF, FP])
 def test_empty_cache_with_a_wide_table(fa, cuda_device, dtype):
     """A cache without pages: every request is empty, whatever the table's width."""
