@@ -214,13 +214,21 @@ fa_status device_state(DeviceState** out) {
   return FA_OK;
 }
 
-// Reads and clears the timeout word of the current device.
-fa_status take_timeout(DeviceState* ds) {
-  unsigned v = 0;
-  FA_CUDA(cudaMemcpy(&v, ds->status, sizeof(v), cudaMemcpyDeviceToHost));
-  if (v == 0) return FA_OK;
-  FA_CUDA(cudaMemset(ds->status, 0, sizeof(unsigned)));
-  return fail(FA_ERR_TIMEOUT, "a kernel wait exceeded its time limit; the kernel returned early and its output is invalid");
+// Reads the status words of the current device, with one copy, and clears the
+// one it reports: a timeout first, then (`bad_index`) an index that the paged
+// operators skipped.
+fa_status take_status(DeviceState* ds, bool bad_index) {
+  unsigned v[2] = {0, 0};
+  FA_CUDA(cudaMemcpy(v, ds->status, sizeof(v), cudaMemcpyDeviceToHost));
+  if (v[0] != 0) {
+    FA_CUDA(cudaMemset(ds->status, 0, sizeof(unsigned)));
+    return fail(FA_ERR_TIMEOUT, "a kernel wait exceeded its time limit; the kernel returned early and its output is invalid");
+  }
+  if (!bad_index || v[1] == 0) return FA_OK;
+  FA_CUDA(cudaMemset(ds->status + 1, 0, sizeof(unsigned)));
+  return fail(FA_ERR_BAD_INDEX,
+              "a paged operator met a page, slot, position or length outside its cache, table or free list; it was "
+              "skipped and the rows that needed it are unspecified");
 }
 
 // ---------------------------------------------------------------- validation
@@ -1098,7 +1106,7 @@ fa_status fa_forward_host(const fa_params* p, const void* q, const void* k, cons
   // The in-kernel status word is read back with the results (no extra sync).
   unsigned* status_host = static_cast<unsigned*>(ds->status_host);
   auto finish_status = [&]() -> fa_status {
-    if (status_host == nullptr || *status_host != 0) return take_timeout(ds);
+    if (status_host == nullptr || *status_host != 0) return take_status(ds, false);
     return FA_OK;
   };
   // Pageable outputs: copy the staged results out with the workers (the
@@ -1270,15 +1278,7 @@ fa_status fa_check_device_status(void) {
   DeviceState* ds = nullptr;
   fa_status st = device_state(&ds);
   if (st != FA_OK) return st;
-  st = take_timeout(ds);
-  if (st != FA_OK) return st;
-  unsigned bad = 0;
-  FA_CUDA(cudaMemcpy(&bad, ds->status + 1, sizeof(bad), cudaMemcpyDeviceToHost));
-  if (bad == 0) return FA_OK;
-  FA_CUDA(cudaMemset(ds->status + 1, 0, sizeof(unsigned)));
-  return fail(FA_ERR_BAD_INDEX,
-              "a paged operator met a page, slot, position or length outside its cache, table or free list; it was "
-              "skipped and the rows that needed it are unspecified");
+  return take_status(ds, true);
 }
 
 fa_status fa_set_wait_limit(double seconds) {
