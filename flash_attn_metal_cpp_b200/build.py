@@ -3,7 +3,8 @@
 Produces, inside this package directory:
   libfa_b200.so                     C ABI (include/fa_b200.h): kernels + host dispatcher
   _flash_attn_metal.<abi>.so        pybind11 module over that C ABI
-  _flash_attn_paged.<abi>.so        its paged-cache operators (pybind11 and torch)
+  _flash_attn_paged.<abi>.so        its paged-cache operators (pybind11 and torch;
+                                    left out where torch is not installed)
 
 Every CUDA translation unit is compiled for sm_100a only
 (-gencode arch=compute_100a,code=sm_100a). Objects are compiled in
@@ -79,9 +80,12 @@ def _compile(src: str, force: bool) -> str:
     return obj
 
 
-def _torch_flags() -> tuple[list[str], list[str]]:
-    """(compile, link) flags of torch's C++ interface."""
-    import torch
+def _torch_flags() -> tuple[list[str], list[str]] | None:
+    """(compile, link) flags of torch's C++ interface, None without torch."""
+    try:
+        import torch
+    except ImportError:
+        return None
 
     root = os.path.dirname(os.path.abspath(torch.__file__))
     inc = os.path.join(root, "include")
@@ -118,7 +122,12 @@ def build(force: bool = False, jobs: int | None = None) -> tuple[str, str]:
     # Two extensions over the C ABI, compiled side by side: the module itself
     # (NumPy and torch, no link to torch) and the paged-cache operators, which
     # use torch's C++ interface.
-    exts = [(EXT, "bindings.cpp", [], []), (EXT_PAGED, "bindings_paged.cpp", *_torch_flags())]
+    exts = [(EXT, "bindings.cpp", [], [])]
+    flags = _torch_flags()
+    if flags is not None:
+        exts.append((EXT_PAGED, "bindings_paged.cpp", *flags))
+    else:
+        print("torch is not installed: _flash_attn_paged (the paged-cache operators) is not built", file=sys.stderr)
     with cf.ThreadPoolExecutor(max_workers=2) as ex:
         list(ex.map(lambda e: _extension(*e, force), exts))
     return LIB, EXT
