@@ -80,8 +80,8 @@ def _compile(src: str, force: bool) -> str:
     return obj
 
 
-def _torch_flags() -> tuple[list[str], list[str]] | None:
-    """(compile, link) flags of torch's C++ interface, None without torch."""
+def _torch_flags() -> tuple[list[str], list[str], str] | None:
+    """(compile flags, link flags, version and place) of torch's C++ interface, None without torch."""
     try:
         import torch
     except ImportError:
@@ -93,19 +93,27 @@ def _torch_flags() -> tuple[list[str], list[str]] | None:
               "-isystem", os.path.join(CUDA_HOME, "include"),
               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
     lib = os.path.join(root, "lib")
-    return cflags, ["-L", lib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python", f"-Wl,-rpath,{lib}"]
+    return cflags, ["-L", lib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python",
+                    f"-Wl,-rpath,{lib}"], f"torch {torch.__version__} in {root}"
 
 
-def _extension(path: str, src: str, cflags: list[str], libs: list[str], force: bool) -> None:
-    """One pybind11 extension linked to libfa_b200.so beside it."""
+def _extension(path: str, src: str, cflags: list[str], libs: list[str], force: bool, against: str = "") -> None:
+    """One pybind11 extension linked to libfa_b200.so beside it; `against` names what else it was built against."""
     import pybind11
 
+    note = os.path.join(OBJDIR, os.path.basename(path) + ".against")
     src = os.path.join(CSRC, src)
-    if not force and _mtime(path) >= max(_mtime(src), _mtime(LIB), _mtime(os.path.join(INCLUDE, "fa_b200.h"))):
+    fresh = _mtime(path) >= max(_mtime(src), _mtime(LIB), _mtime(os.path.join(INCLUDE, "fa_b200.h")))
+    if against and fresh:
+        fresh = os.path.exists(note) and open(note).read() == against
+    if fresh and not force:
         return
     _run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-I", pybind11.get_include(),
           "-I", sysconfig.get_paths()["include"], "-I", INCLUDE, *cflags, src, "-o", path, "-L", PKG,
           "-l:libfa_b200.so", *libs, "-Wl,-rpath,$ORIGIN"])
+    if against:
+        with open(note, "w") as f:
+            f.write(against)
 
 
 def build(force: bool = False, jobs: int | None = None) -> tuple[str, str]:
@@ -122,14 +130,15 @@ def build(force: bool = False, jobs: int | None = None) -> tuple[str, str]:
     # Two extensions over the C ABI, compiled side by side: the module itself
     # (NumPy and torch, no link to torch) and the paged-cache operators, which
     # use torch's C++ interface.
-    exts = [(EXT, "bindings.cpp", [], [])]
+    exts = [(EXT, "bindings.cpp", [], [], force)]
     flags = _torch_flags()
     if flags is not None:
-        exts.append((EXT_PAGED, "bindings_paged.cpp", *flags))
+        cflags, libs, torch_is = flags
+        exts.append((EXT_PAGED, "bindings_paged.cpp", cflags, libs, force, torch_is))
     else:
         print("torch is not installed: _flash_attn_paged (the paged-cache operators) is not built", file=sys.stderr)
     with cf.ThreadPoolExecutor(max_workers=2) as ex:
-        list(ex.map(lambda e: _extension(*e, force), exts))
+        list(ex.map(lambda e: _extension(*e), exts))
     return LIB, EXT
 
 

@@ -53,3 +53,17 @@ def test_the_module_is_built_without_torch(builder, no_torch, capsys):
     builder.build()
     assert builder.ran == ["bindings.cpp"]
     assert "paged" in capsys.readouterr().err
+
+
+def test_another_torch_rebuilds_what_uses_it(builder, monkeypatch):
+    import torch
+
+    builder.build()
+    builder.ran.clear()
+    builder.build()
+    assert builder.ran == []
+    monkeypatch.setattr(torch, "__version__", "0.0.1")
+    builder.build()
+    assert builder.ran == ["bindings_paged.cpp"]
+    builder.build()
+    assert builder.ran == ["bindings_paged.cpp"]
