@@ -4,7 +4,7 @@ Produces, inside this package directory:
   libfa_b200.so                     C ABI (include/fa_b200.h): kernels + host dispatcher
   _flash_attn_metal.<abi>.so        pybind11 module over that C ABI
   _flash_attn_paged.<abi>.so        its paged-cache operators (pybind11 and torch;
-                                    left out where torch is not installed)
+                                    left out without a torch that has CUDA)
 
 Every CUDA translation unit is compiled for sm_100a only
 (-gencode arch=compute_100a,code=sm_100a). Objects are compiled in
@@ -81,10 +81,12 @@ def _compile(src: str, force: bool) -> str:
 
 
 def _torch_flags() -> tuple[list[str], list[str], str] | None:
-    """(compile flags, link flags, version and place) of torch's C++ interface, None without torch."""
+    """(compile flags, link flags, version and place) of torch's C++ interface, None without a torch that has CUDA."""
     try:
         import torch
     except ImportError:
+        return None
+    if torch.version.cuda is None:
         return None
 
     root = os.path.dirname(os.path.abspath(torch.__file__))
@@ -136,7 +138,7 @@ def build(force: bool = False, jobs: int | None = None) -> tuple[str, str]:
         cflags, libs, torch_is = flags
         exts.append((EXT_PAGED, "bindings_paged.cpp", cflags, libs, force, torch_is))
     else:
-        print("torch is not installed: _flash_attn_paged (the paged-cache operators) is not built", file=sys.stderr)
+        print("torch with CUDA is not installed: _flash_attn_paged (the paged-cache operators) is not built", file=sys.stderr)
     with cf.ThreadPoolExecutor(max_workers=2) as ex:
         list(ex.map(lambda e: _extension(*e), exts))
     return LIB, EXT

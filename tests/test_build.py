@@ -55,6 +55,14 @@ def test_the_module_is_built_without_torch(builder, no_torch, capsys):
     assert "paged" in capsys.readouterr().err
 
 
+def test_a_torch_without_cuda_counts_as_none(builder, monkeypatch):
+    import torch
+
+    monkeypatch.setattr(torch.version, "cuda", None)
+    builder.build()
+    assert builder.ran == ["bindings.cpp"]
+
+
 def test_another_torch_rebuilds_what_uses_it(builder, monkeypatch):
     import torch
 
