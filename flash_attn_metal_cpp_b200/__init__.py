@@ -48,6 +48,10 @@ def __getattr__(name):
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
+def __dir__():
+    return sorted({*globals(), *_PAGED})
+
+
 def _to_numpy(x):
     """np.array(x) of the reference wrapper (__init__.py:63-68); torch
     tensors (also CUDA ones, which np.array cannot read) via .cpu().numpy()."""
@@ -83,5 +87,5 @@ def metal_attention(q, k, v, causal=False, softmax_scale=None, dropout_p=0.0):
     )
 
 
-__all__ = ["metal_attention", "initialize", "get_device_info", "forward", "plan_pages", "store_kv", "paged_forward",
-           "shared_prefix_forward", "LIB_PATH"]
+# (without the names of _PAGED: `import *` would load torch)
+__all__ = ["metal_attention", "initialize", "get_device_info", "forward", "LIB_PATH"]
