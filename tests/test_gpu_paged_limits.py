@@ -200,3 +200,49 @@ torch.cuda.synchronize()
 w, _, tol, _ = b.want(True)
 ref.assert_attention(o, w, tol, 'first')
 """)
+
+
+# -------------------------------------------------------- offsets above 32 bits
+def moved_up(b, elements):
+    """The batch with its pages at the end of caches of more than `elements` elements."""
+    n, *shape = b.k_cache.shape
+    total = elements // math.prod(shape) + n + 1
+
+    def up(c):
+        big = torch.empty((total, *shape), dtype=c.dtype, device=c.device)
+        big[-n:] = c
+        return big
+
+    b.k_cache, b.v_cache = up(b.k_cache), up(b.v_cache)
+    b.table[b.table >= 0] += total - n
+    b.prefix_table += total - n
+    return b
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("kw", [dict(lens=[300, 449, 65]), dict(lens=[300, 449, 65], width=400), dict(lens=[300, 129, 260], qlens=[200, 129, 33]),
+                                dict(lens=[50, 9, 0] + [30] * 37, prefix=805)])
+def test_pages_behind_32_bits_of_elements(fa, cuda_device, dtype, kw):
+    b = moved_up(Batch(cuda_device, hq=8, hk=2, d=128, dtype=dtype, **kw), 1 << 32)
+    causal = any(n != 1 for n in b.qlens)
+    o = b.run(fa, causal, out_dtype="float32")
+    torch.cuda.synchronize()
+    fa.check_status()
+    w, _, tol, _ = b.want(causal, out_dtype=FP)
+    ref.assert_attention(o, w, tol, "far pages")
+
+
+@pytest.mark.parametrize("d,slots", [(128, 1 << 22), (2, 1 << 31)])
+def test_slots_behind_32_bits(fa, cuda_device, d, slots):
+    """Rows stored where the element offset passes 2^32, and slot numbers above 2^31."""
+    hk = 8 if d == 128 else 1
+    pages = slots // 1024 + 1
+    kc, vc = (torch.zeros((pages, 1024, hk, d), dtype=HF, device=cuda_device) for _ in range(2))
+    k, v = (torch.randn((3, hk, d), device=cuda_device).to(HF) for _ in range(2))
+    at = torch.tensor([pages * 1024 - 1, 5, pages * 1024 - 700], device=cuda_device)
+    fa.store_kv(k, v, kc, vc, at)
+    torch.cuda.synchronize()
+    fa.check_status()
+    for c, x in ((kc, k), (vc, v)):
+        assert torch.equal(c[at // 1024, at % 1024], x)
+        assert int(c[-1].count_nonzero()) == 2 * hk * d and int(c[0].count_nonzero()) == hk * d and not c[1:-1].any()
