@@ -320,7 +320,7 @@ __device__ __forceinline__ void finish_row4(const PagedArgs& a, int token, int h
 // Units of a few tiles are cut between the blocks of a cluster, one unit a
 // cluster, and joined through its shared memory instead of by a second kernel:
 // a launch and its wait less. (On 8 KV heads, D = 128, one request of 500 keys
-// 13.1 -> 7.7 us, 16 requests 17.0 -> 11.6 us.)
+// 12.3 -> 7.0 us, 16 requests 16.4 -> 11.0 us.)
 
 // First of a unit's tiles that block `rank` of its cluster takes.
 __device__ __forceinline__ int share_begin(const PagedArgs& a, int tiles, int rank) {

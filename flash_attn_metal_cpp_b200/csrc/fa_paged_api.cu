@@ -159,9 +159,14 @@ struct Choice {
 // tiles: 568 us in 1 part, 315 in 2 = one wave, 368 in 4 = two waves, 375 in 9
 // = four); every part writes and reads its partial rows once (about 5 TB/s).
 // One part needs no join. With the few-rows kernel running `beside`, a single
-// wave leaves it a quarter of the SMs, or costs its time (some 10 us) on top.
-// (24 requests of 4 tokens, 8 heads on one KV head, a prefix of 50001 keys: 74
-// us with 16 parts, 52 with 31, 56 with 49.)
+// wave leaves it a quarter of the SMs, or costs its time (some 10 us, from one
+// size only) on top. (24 requests of 4 tokens, 8 heads on one KV head, a prefix
+// of 50001 keys: 74 us with 16 parts, 52 with 31, 56 with 49.)
+//
+// For a request's own keys `tiles` is what its table has room for, as the host
+// does not know the lengths; parts behind a request's end cost their start and
+// their empty rows. (4 prompt chunks of 335 to 840 tokens over 1165 to 3932: 126
+// us with a table of 4272 tokens, 187 with 8192 and 32768, 573 with 2^20.)
 int choose_parts(long long blocks, long long tiles, int D, double row_bytes, bool join_anyway, bool beside) {
   const double tile = D <= 64 ? 1.8e-6 : 2.15e-6;
   const int top = (int)std::max(1ll, std::min(64ll, tiles / 2));
@@ -251,7 +256,8 @@ Choice choose(const fa_paged_params* p, const Checked& c, bool vec, bool one) {
     }
     // Units of few tiles are cut between the blocks of a cluster instead, which
     // saves the join's launch but balances nothing, so a block's share by the
-    // table's width is at most 128 KB of K and V. (One request on 8 KV heads, D =
+    // table's width is at most 128 KB of K and V. (Times of graphs of five calls,
+    // some 0.8 us above those of longer graphs. One request on 8 KV heads, D =
     // 128, cut in runs and in clusters: 500 keys 13.1 and 7.9 us, 2000 keys, 4
     // tiles a share, 13.6 and 11.4, 4000 keys 13.3 and 15.9; 16 requests of 1 to
     // 1000 keys, 8 tiles a share, 13.0 and 15.8. Uncut and in clusters: 200 keys

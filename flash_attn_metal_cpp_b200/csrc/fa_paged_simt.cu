@@ -23,8 +23,14 @@
 // tables) leave warps over, so there 4 keys in flight pay (16 requests of 250
 // tokens, 16 heads of 64: 9.4 us, with one key 10.2; not above 64 columns: 8
 // requests of 250, 4 KV heads of 256, 9.8 us with two keys, 9.1 with one). 8
-// requests of 200 to 1025 tokens, 8 heads of 64, take 10.0 us, of 8000 tokens
+// requests of 200 to 1025 tokens, 8 heads of 64, take 9.2 us, of 8000 tokens
 // 55 us (4.8 TB/s).
+//
+// More than 4 rows a unit share nothing: a prompt chunk reads its keys again
+// for every 4 rows (2 above 128 columns), from L2, and a shared prefix is read
+// by every request. 8 requests of 4 tokens over 2000, 32 heads on 8 KV heads of
+// 128, take 162 us, 4 chunks of 512 tokens over 2000 10.2 ms (7 TFLOP/s), 64
+// single tokens behind a prefix of 4096 keys 436 us.
 #include "fa_paged.cuh"
 
 #include <algorithm>

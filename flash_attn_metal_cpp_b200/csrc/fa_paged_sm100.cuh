@@ -22,12 +22,17 @@
 //   * P has V's type (one MMA takes one type): rounded to bf16 or fp16, half
 //     a step of 2^-8 or 2^-11 of each weight; everything else is fp32.
 //   * Columns beyond head_dim (below 64 or 128) are zero-filled by the TMA.
-// What bounds it: the tensor cores and the exponentials together, like the
-// contiguous kernel; K and V are read from L2 by the blocks of one KV head. A
-// step of 256 rows by 128 keys takes 2.2 us at D = 128 (1120 TFLOP/s with all
-// SMs at it), a block's start and end 6 to 9 us: a prefix of 32768 keys under
-// 2048 rows on 8 KV heads takes 290 us in 128 blocks of 128 steps, 4 prompt
-// chunks of 335 to 840 tokens over 1165 to 3932 cached ones 126 us.
+// What bounds it: the chain of a step (S = Q K^T, load, maximum, exponentials,
+// P, O += P V, and only then the tile's next S, whose columns P takes), which
+// two row tiles do not hide. No pipe is full: in prompt chunks and in a prefix
+// of 32768 keys the tensor pipe is busy 48 and 64 % of the time, the
+// exponentials' 42 and 56 %, 33 % of the issue slots are taken. K and V come
+// from L2 for all blocks of one KV head but the first. A step of 256 rows by
+// 128 keys takes 2.2 us at D = 128 (1120 TFLOP/s with all SMs at it; its MMAs
+// alone would take 1.5, its exponentials 1.1), a block's start and end 6 to 9
+// us: a prefix of 32768 keys under 2048 rows on 8 KV heads takes 290 us in 128
+// blocks of 128 steps, 4 prompt chunks of 335 to 840 tokens over 1165 to 3932
+// cached ones 126 us.
 #pragma once
 
 #include "fa_paged.cuh"
@@ -130,10 +135,12 @@ __device__ __forceinline__ int scan_block(int x, int warps, int* part, int* tota
 // one reciprocal (r1 = d2 R, r2 = d1 R, R = 1 / (d1 d2); e^(2y) is held below
 // 2^40, where r is below 2^-40 anyway, so the product stays finite): 2.5
 // special-function operations a score instead of 3, and 5 others (prefix of
-// 32768 keys, 2048 rows on 8 KV heads: 538 us; 860 us through XF 3; a quarter
-// of the weights on the FMA pipe instead 515 us, half of them 553). r is off by
-// at most 2^-22.5, the score by 2^-21 cap; caps beyond kFastCap take XF 3,
-// whose tanh is exact in the relative sense.
+// 32768 keys, 2048 rows on 8 KV heads: 528 us; 860 us through XF 3). A quarter
+// of the weights through a polynomial on the FMA pipe measured 515 where this
+// measured 538, half of them 553: left out, 4 % of one kind of call for a second
+// exponential with an error of its own. r is off by at most 2^-22.5, the score
+// by 2^-21 cap; caps beyond kFastCap take XF 3, whose tanh is exact in the
+// relative sense. A NaN score stays NaN (min_nan).
 template <int D, typename T, int XF>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_attn_sm100(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,

@@ -289,8 +289,8 @@ fa_status fa_test_stall_next_launch(int32_t k_tile);
 uint64_t fa_launch_count(void);
 
 /* Kernel timing (no counterpart in the reference): while enabled, every
- * launch of the attention kernel on the calling thread is bracketed by CUDA
- * events recorded on its own stream. fa_kernel_timing_read synchronises
+ * launch of the attention kernel on the calling thread (not of the paged
+ * operators) is bracketed by CUDA events recorded on its own stream. fa_kernel_timing_read synchronises
  * those events and returns the summed duration (ms) and the launch count
  * since the last enable, then disables timing. */
 fa_status fa_kernel_timing_enable(void);
@@ -439,8 +439,13 @@ size_t fa_paged_workspace_size(const fa_paged_params* p);
  * prompt chunk and changes nothing for a single token. Rows that see no key
  * get O = 0 and LSE = -inf; rows behind the last sequence are left as they
  * were. Slots no query of the request sees (behind its end, before its
- * window) are not read into the result whatever they hold. o and lse must not
- * overlap the inputs or each other.
+ * window) are not read into the result whatever they hold. A row that sees a
+ * NaN score gets a NaN O and LSE; a NaN or an infinity in the V row of a key
+ * may also reach rows of the same request (behind a prefix, of the batch) that
+ * mask the key while another row sees it. o and lse must not overlap the inputs
+ * or each other. Scratch and, above 32 rows a KV head (query tokens times heads
+ * of a group), time grow with the table's width (max_pages): the lengths are
+ * not known to the host.
  * workspace: device scratch of fa_paged_workspace_size bytes, 256-byte
  * aligned; calls that may overlap on the GPU need one each. */
 fa_status fa_paged_forward(const fa_paged_params* p, const void* q, const void* k_cache, const void* v_cache,
